@@ -14,7 +14,9 @@ ARCH = "gfx950"
 # instructions (SGPR-pair / op_sel operands); such code in layernorm_bwd computed whole rows wrong, now and then, when its
 # wave shared a SIMD with another kernel's bf16 MFMAs (tools/lnb_race.py).  Off for every file:
 # no measurable cost (bench.py / bench_train.py A/B/A/B; the attention launches gain 1-2 %).
-BASE_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fno-slp-vectorize"]
+# -packed-fp32-ops: ordinary float4 / float2 arithmetic becomes packed instructions too, without the vectoriser; with the
+# feature off the library holds none of them.  (The host pass warns that it does not know the feature: harmless.)
+BASE_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def sources():
