@@ -1,0 +1,466 @@
+// Cross attention over packed ragged batches: queries [Mq] of one matrix, keys / values [Mk] of another, utterance b of the
+// first against utterance b of the second (cu_q, cu_k), g = H / KV query heads to a key / value head.
+//   S = q k^T / sqrt(dk);  P = softmax over the utterance's keys;  ctx = dropout(P) v;  lse = log2 sum exp2(S log2 e)
+// An utterance without keys has ctx = 0 and lse = -inf.  Running maximum and sum in fp32; bf16 rounds P (to half a step of
+// bf16, like the operands it meets on the matrix pipe) and the result, nothing else.
+//
+// Orientation as in attention.hip: S^T = K Q^T and O^T = V^T P^T, so that a lane owns one query row and every softmax statistic
+// is lane-local; the accumulator layout of P^T is used as the next operand, V is read transposed from LDS with the same map.
+//   rows kernel: 4 waves x 16 QT packed rows, K / V tiles of 64 keys double-buffered in LDS for all four.
+//   few kernel:  at most 16 packed rows per pair (one frame at a time): the four waves share the rows and split the KEYS,
+//                each with its own 32-key tiles; K goes straight into registers, V through wave-private LDS; one merge.
+// Where the pairs alone do not fill the chip, ranges of keys go to `nsplit` workgroups and a second kernel merges.
+#include "cross_attention.h"
+
+namespace fs2 {
+
+// ctx rows of an utterance without keys
+template <typename T, int DK>
+__device__ __forceinline__ void x_zero_rows(const XArgs& a, int q0, int kvh, int r_begin, int r_end) {
+    constexpr int SL = DK / 4;
+    for (int e = threadIdx.x; e < (r_end - r_begin) * SL; e += blockDim.x) {
+        const int r = r_begin + e / SL, q = x_query(a, r), h = kvh * a.g + r - q * a.g;
+        store4<T>((T*)a.ctx + (size_t)(q0 + q) * a.ldo + h * DK + (e % SL) * 4, (f32x4){0.f, 0.f, 0.f, 0.f});
+        if (a.lse && e % SL == 0) a.lse[(size_t)h * a.Mq + q0 + q] = -INFINITY;
+    }
+}
+
+template <typename T, int DK, int QT>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel(XArgs a) {
+    typedef XTile<T, DK> TL;
+    typedef typename TL::frag_t frag_t;
+    constexpr int KS = TL::KS, DT = TL::DT, BQ = 64 * QT;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile, V tile at s * 2 * BYTES
+
+    int b, kvh, blk;
+    if (!fs2_pair_order_decode(a.order, b, kvh, blk)) return;
+    const int split = blk % a.nsplit;
+    blk /= a.nsplit;
+    int q0, lenq, k0, lenk;
+    x_range(a.cu_q, b, a.Mq, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    const int nrow = lenq * a.g;
+    if (blk * BQ >= nrow) return;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, i = lane & 15;
+    const int ntiles = (lenk + 63) / 64, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntiles);
+    if (lenk == 0 && a.nsplit == 1) {
+        x_zero_rows<T, DK>(a, q0, kvh, blk * BQ, min(nrow, blk * BQ + BQ));
+        return;
+    }
+    int qrow[QT], head[QT];
+    bool live[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int r = blk * BQ + (wave * QT + t) * 16 + i;
+        live[t] = r < nrow;
+        const int rc = min(r, nrow - 1), q = x_query(a, rc);
+        qrow[t] = q0 + q;
+        head[t] = kvh * a.g + rc - q * a.g;
+    }
+    if (t0 >= t1) {         // this split has no keys: (max, sum) = (-inf, 0)
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+            if (g == 0 && live[t]) {
+                float* ml = a.part + (size_t)a.nsplit * a.Mq * a.H * DK + (((size_t)split * a.H + head[t]) * a.Mq + qrow[t]) * 2;
+                ml[0] = -INFINITY;
+                ml[1] = 0.f;
+            }
+        return;
+    }
+    const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
+    const T* __restrict__ vb = (const T*)a.v + (size_t)k0 * a.ldv + kvh * DK;
+    auto stage = [&](int kt, int st) __attribute__((always_inline)) {
+        unsigned char* d = smem + st * 2 * TL::BYTES;
+        TL::template stage<1, 4>(kb, a.ldk, kt * 64, lenk, d, wave, lane);
+        TL::template stage<2, 4>(vb, a.ldv, kt * 64, lenk, d + TL::BYTES, wave, lane);
+    };
+    stage(t0, 0);
+
+    frag_t qf[QT][KS];
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            qf[t][ks] = *(const frag_t*)((const T*)a.q + (size_t)qrow[t] * a.ldq + head[t] * DK + ks * 32 + g * 8);
+
+    f32x4 o[QT][DT];
+    float m_run[QT], l_part[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        m_run[t] = -INFINITY;
+        l_part[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[t][dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    for (int kt = t0; kt < t1; ++kt) {
+        vm_wait_barrier<0>();         // tile kt has landed; every wave is done with the other stage
+        const int st = (kt - t0) & 1;
+        if (kt + 1 < t1) stage(kt + 1, st ^ 1);
+        const unsigned char* Ks = smem + st * 2 * TL::BYTES;
+        const unsigned char* Vs = Ks + TL::BYTES;
+
+        f32x4 s[QT][4];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) s[t][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            frag_t kf[4];
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) kf[nt] = TL::template row_frag<1>(Ks, nt * 16 + i, ks, g);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) mma16_multi<4>(kf, qf[t][ks], s[t]);
+        }
+        const int kbase = kt * 64 + 4 * g;
+        if (kt * 64 + 64 > lenk) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (kbase + nt * 16 + r >= lenk) s[t][nt][r] = -INFINITY;
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            float m_loc = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m_loc = fmaxf(m_loc, s[t][nt][r]);
+            m_loc = rows_max(m_loc) * a.scale_log2e;
+            const float m_new = fmaxf(m_run[t], m_loc);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;        // a tile of -inf scores leaves no NaN behind
+            const float alpha = __builtin_amdgcn_exp2f(m_run[t] - m_use);
+            m_run[t] = m_new;
+            float psum = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[t][nt][r], a.scale_log2e, -m_use));
+                    s[t][nt][r] = p;
+                    psum += p;
+                }
+            l_part[t] = fmaf(l_part[t], alpha, psum);
+            if (!__all(alpha == 1.0f)) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[t][dt][r] *= alpha;
+            }
+            if (a.drop.thresh) {      // the sum above is over the undropped probabilities
+                Dropout dh = a.drop;
+                dh.stream += (uint32_t)head[t];
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][nt][r] *= drop_mul(dh, (uint32_t)qrow[t], (uint32_t)(kbase + nt * 16 + r));
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            frag_t pf[QT];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) pf[t] = x_pack<T>(s[t][2 * c], s[t][2 * c + 1]);
+#pragma unroll
+            for (int dt0 = 0; dt0 < DT; dt0 += 2) {
+                frag_t vf[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) vf[u] = TL::template col_frag<2>(Vs, c, dt0 + u, g, i);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) mma16_multi<2>(vf, pf[t], &o[t][dt0]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const float l = rows_sum(l_part[t]);
+        if (!live[t]) continue;
+        if (a.nsplit == 1) {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;        // no score above -inf: a zero row
+            if (a.lse && g == 0) a.lse[(size_t)head[t] * a.Mq + qrow[t]] = m_run[t] + __log2f(l);
+            T* dst = (T*)a.ctx + (size_t)qrow[t] * a.ldo + head[t] * DK + 4 * g;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) store4<T>(dst + dt * 16, o[t][dt] * inv);
+        } else {
+            const size_t d = (size_t)a.H * DK;
+            float* dst = a.part + ((size_t)split * a.Mq + qrow[t]) * d + head[t] * DK + 4 * g;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *(f32x4*)(dst + dt * 16) = o[t][dt];
+            float* ml = a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)split * a.H + head[t]) * a.Mq + qrow[t]) * 2;
+            if (g == 0) {
+                ml[0] = m_run[t];
+                ml[1] = l;
+            }
+        }
+    }
+}
+
+// At most 16 packed rows per (utterance, shared head).  grid (nsplit, KV, B); wave w takes the 32-key tiles t0 + w, + 4, ..
+template <typename T, int DK>
+__global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
+    typedef XTile<T, DK, 32> TL;
+    typedef typename TL::frag_t frag_t;
+    constexpr int KS = TL::KS, DT = TL::DT;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // wave w: V tile at w * BYTES; then the merge
+    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    int q0, lenq, k0, lenk;
+    x_range(a.cu_q, b, a.Mq, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    const int nrow = min(lenq * a.g, 16);
+    if (nrow == 0) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, i = lane & 15;
+    if (lenk == 0 && a.nsplit == 1) {
+        x_zero_rows<T, DK>(a, q0, kvh, 0, nrow);
+        return;
+    }
+    const int rc = min(i, nrow - 1), q = x_query(a, rc), head = kvh * a.g + rc - q * a.g, qrow = q0 + q;
+    const int ntiles = (lenk + 31) / 32, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntiles);
+    frag_t qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const frag_t*)((const T*)a.q + (size_t)qrow * a.ldq + head * DK + ks * 32 + g * 8);
+
+    const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
+    const T* __restrict__ vb = (const T*)a.v + (size_t)k0 * a.ldv + kvh * DK;
+    unsigned char* Vs = smem + wave * TL::BYTES;
+    f32x4 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_part = 0.f;
+    for (int kt = t0 + wave; kt < t1; kt += 4) {
+        frag_t kf[KS][2];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+                kf[ks][nt] = *(const frag_t*)(kb + (size_t)min(kt * 32 + nt * 16 + i, lenk - 1) * a.ldk + ks * 32 + g * 8);
+        TL::template stage<2, 1>(vb, a.ldv, kt * 32, lenk, Vs, 0, lane);
+        f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) mma16_multi<2>(kf[ks], qf[ks], s);
+        const int kbase = kt * 32 + 4 * g;
+        float m_loc = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (kbase + nt * 16 + r >= lenk) s[nt][r] = -INFINITY;
+                m_loc = fmaxf(m_loc, s[nt][r]);
+            }
+        m_loc = rows_max(m_loc) * a.scale_log2e;
+        const float m_new = fmaxf(m_run, m_loc), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+        m_run = m_new;
+        float psum = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[nt][r] = __builtin_amdgcn_exp2f(fmaf(s[nt][r], a.scale_log2e, -m_use));
+                psum += s[nt][r];
+            }
+        l_part = fmaf(l_part, alpha, psum);
+        if (a.drop.thresh) {
+            Dropout dh = a.drop;
+            dh.stream += (uint32_t)head;
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[nt][r] *= drop_mul(dh, (uint32_t)qrow, (uint32_t)(kbase + nt * 16 + r));
+        }
+        const frag_t pf = x_pack<T>(s[0], s[1]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's V tile has landed (no other wave reads it)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const frag_t vf = TL::template col_frag<2>(Vs, 0, dt, g, i);
+            o[dt] = mma16(vf, pf, o[dt] * alpha);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next tile's DMA overwrites it
+    }
+    // merge of the four waves: lane (g, i) of wave w holds row i, columns 16 dt + 4 g ..
+    const float l = rows_sum(l_part);
+    __syncthreads();
+    float* mo = (float*)smem;                       // [4][16][DK]
+    float* mm = mo + 4 * 16 * DK;                   // [4][16] max, then sum
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) *(f32x4*)(mo + (wave * 16 + i) * DK + dt * 16 + 4 * g) = o[dt];
+    if (g == 0) {
+        mm[wave * 16 + i] = m_run;
+        mm[64 + wave * 16 + i] = l;
+    }
+    __syncthreads();
+    constexpr int SL = DK / 4;
+    for (int e = tid; e < nrow * SL; e += 256) {
+        const int r = e / SL, c = (e % SL) * 4;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, mm[w * 16 + r]);
+        const float mu = mx == -INFINITY ? 0.f : mx;
+        float L = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(mm[w * 16 + r] - mu);
+            L = fmaf(mm[64 + w * 16 + r], f, L);
+            acc += *(const f32x4*)(mo + (w * 16 + r) * DK + c) * f;
+        }
+        const int qq = x_query(a, r), h = kvh * a.g + r - qq * a.g;
+        if (a.nsplit == 1) {
+            store4<T>((T*)a.ctx + (size_t)(q0 + qq) * a.ldo + h * DK + c, acc * (L == 0.f ? 0.f : 1.0f / L));
+            if (a.lse && c == 0) a.lse[(size_t)h * a.Mq + q0 + qq] = mx + __log2f(L);
+        } else {
+            const size_t d = (size_t)a.H * DK;
+            *(f32x4*)(a.part + ((size_t)split * a.Mq + q0 + qq) * d + h * DK + c) = acc;
+            float* ml = a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)split * a.H + h) * a.Mq + q0 + qq) * 2;
+            if (c == 0) {
+                ml[0] = mx;
+                ml[1] = L;
+            }
+        }
+    }
+}
+
+// merge of the key ranges; one lane per (row, four channels).  Rows behind the last utterance, and rows of utterances longer
+// than max_q, were computed by nobody: cu_q[B] bounds the first, the second are the caller's breach of max_q.
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int dk) {
+    const int d = a.H * dk, dv = d >> 2;
+    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int rows = min(max(a.cu_q[B], 0), a.Mq);
+    if (idx >= (long long)rows * dv) return;
+    const int m = (int)(idx / dv), c = (int)(idx % dv) * 4, h = c / dk;
+    const float* ml = a.part + (size_t)a.nsplit * a.Mq * d + ((size_t)h * a.Mq + m) * 2;
+    const size_t step = (size_t)a.H * a.Mq * 2;
+    float mx = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) mx = fmaxf(mx, ml[s * step]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float L = 0.f;
+    bool any = false;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float l = ml[s * step + 1];
+        if (l == 0.f) continue;                  // a range without keys wrote no partial context
+        any = true;
+        const float f = __builtin_amdgcn_exp2f(ml[s * step] - mu);
+        L = fmaf(l, f, L);
+        acc += *(const f32x4*)(a.part + ((size_t)s * a.Mq + m) * d + c) * f;
+    }
+    store4<T>((T*)a.ctx + (size_t)m * a.ldo + c, any ? acc * (1.0f / L) : acc);
+    if (a.lse && c % dk == 0) a.lse[(size_t)h * a.Mq + m] = any ? mx + __log2f(L) : -INFINITY;
+}
+
+struct XPlan { bool few; int qt, nsplit; };
+
+static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dk, int dtype) {
+    XPlan p = {};
+    const int g = H / KV;
+    const long rows = (long)max_q * g, pairs = (long)B * KV;
+    p.few = rows <= 16;
+    p.nsplit = 1;
+    if (p.few) {
+        const long tiles = (max_k + 31) / 32;
+        if (tiles > 8 && pairs < 256) {
+            const long want = 512 / pairs, most = tiles / 4;
+            p.nsplit = (int)(want < most ? want : most);
+        }
+    } else {
+        p.qt = dtype == 1 && rows > 64 ? 2 : 1;
+        const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = (max_k + 63) / 64;
+        if (items < 256 && tiles >= 4) {
+            const long want = 512 / items, most = tiles / 2;
+            p.nsplit = (int)(want < most ? want : most);
+        }
+    }
+    if (p.nsplit > 32) p.nsplit = 32;
+    if (p.nsplit < 1) p.nsplit = 1;
+    return p;
+}
+
+template <typename T, int DK>
+static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipStream_t stream) {
+    if (p.few) {
+        constexpr int merge = 4 * 16 * DK * 4 + 512, tiles = 4 * XTile<T, DK, 32>::BYTES;
+        constexpr int lds = merge > tiles ? merge : tiles;
+        static unsigned long long ok = 0;
+        fs2_allow_lds((const void*)xattn_few_kernel<T, DK>, lds, &ok);
+        hipLaunchKernelGGL((xattn_few_kernel<T, DK>), dim3(a.nsplit, a.KV, B), dim3(256), lds, stream, a);
+    } else {
+        constexpr int lds = 4 * XTile<T, DK>::BYTES;
+        static unsigned long long ok[2] = {0, 0};
+        const int rows = max_q * a.g, nblk = (rows + 64 * p.qt - 1) / (64 * p.qt);
+        const dim3 grid = fs2_pair_order_grid(a.order, nblk * a.nsplit, a.KV, B, true);
+        if (p.qt == 2) {
+            if constexpr (sizeof(T) == 2) {
+                fs2_allow_lds((const void*)xattn_rows_kernel<T, DK, 2>, lds, &ok[1]);
+                hipLaunchKernelGGL((xattn_rows_kernel<T, DK, 2>), grid, dim3(256), lds, stream, a);
+            }
+        } else {
+            fs2_allow_lds((const void*)xattn_rows_kernel<T, DK, 1>, lds, &ok[0]);
+            hipLaunchKernelGGL((xattn_rows_kernel<T, DK, 1>), grid, dim3(256), lds, stream, a);
+        }
+    }
+    FS2_CHECK_LAUNCH("fs2_cross_attention");
+    if (a.nsplit > 1) {
+        const long long n = (long long)a.Mq * (a.H * dk / 4);
+        hipLaunchKernelGGL(xattn_combine_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B, dk);
+        FS2_CHECK_LAUNCH("fs2_cross_attention(merge)");
+    }
+    return FS2_OK;
+}
+
+}  // namespace fs2
+
+using namespace fs2;
+
+extern "C" long long fs2_cross_attention_workspace(int B, int max_q, int max_k, int Mq, int n_heads, int n_kv_heads, int dk,
+                                                   int dtype) {
+    if (B <= 0 || max_q <= 0 || max_k <= 0 || Mq <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return 0;
+    const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dk, dtype);
+    return p.nsplit == 1 ? 0 : (long long)p.nsplit * Mq * n_heads * (dk + 2) * (long long)sizeof(float);
+}
+
+extern "C" int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, float* lse, const int* cu_q,
+                                   const int* cu_k, void* workspace, int B, int max_q, int max_k, int Mq, int Mk, int n_heads,
+                                   int n_kv_heads, int dk, int ldq, int ldk, int ldv, int ldo, int dtype, unsigned seed,
+                                   unsigned stream_id, float rate, hipStream_t stream) {
+    const int rc = fs2_x_check("fs2_cross_attention", q, k, cu_q, cu_k, B, max_q, max_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk,
+                               dtype);
+    if (rc != FS2_OK) return rc;
+    const int epv = dtype == 0 ? 4 : 8;
+    FS2_CHECK_ARG(rate >= 0.f && rate < 1.f, "fs2_cross_attention: dropout rate must be in [0, 1)");
+    FS2_CHECK_ARG((v || Mk == 0) && (ctx || Mq == 0) && ((uintptr_t)v & 15) == 0 && ((uintptr_t)ctx & 15) == 0,
+                  "fs2_cross_attention: null or unaligned v or ctx");
+    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldo >= n_heads * dk && ldv % epv == 0 && ldo % epv == 0,
+                  "fs2_cross_attention: bad leading dims ldv=%d ldo=%d", ldv, ldo);
+    if (max_q == 0) return FS2_OK;
+    XArgs a = fs2_x_args(q, k, v, cu_q, cu_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, ldv, ldo);
+    a.ctx = ctx;
+    a.lse = lse;
+    a.drop = fs2_make_dropout(seed, stream_id, rate);
+    const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dk, dtype);
+    a.nsplit = p.nsplit;
+    a.part = (float*)workspace;
+    FS2_CHECK_ARG(p.nsplit == 1 || (workspace && ((uintptr_t)workspace & 15) == 0),
+                  "fs2_cross_attention: this shape needs fs2_cross_attention_workspace bytes, 16-byte aligned");
+#define FS2_X(TT, DKK) return launch_xattn<TT, DKK>(a, p, B, max_q, dk, stream)
+    if (dtype == 0) {
+        if (dk == 32) FS2_X(float, 32);
+        if (dk == 64) FS2_X(float, 64);
+        if (dk == 96) FS2_X(float, 96);
+        FS2_X(float, 128);
+    }
+    if (dk == 32) FS2_X(bf16_t, 32);
+    if (dk == 64) FS2_X(bf16_t, 64);
+    if (dk == 96) FS2_X(bf16_t, 96);
+    FS2_X(bf16_t, 128);
+#undef FS2_X
+}

@@ -1,0 +1,619 @@
+// Group norm of packed ragged rows with an activation, and its backward.  Utterance b owns rows cu[b] .. cu[b + 1] of
+// x [M, C] (channels last); mean and variance are taken over (its rows) x (the C / G channels of a group):
+//   xhat = (x - mean) rstd,  rstd = 1 / sqrt(var + eps);  y = dropout(act(gamma xhat + beta))
+//   dz = dropout(dy) act'(gamma xhat + beta),  dh = gamma dz
+//   dx = rstd (dh - mean_g(dh) - xhat mean_g(dh xhat));  dgamma = sum dz xhat,  dbeta = sum dz
+// Unlike BatchNorm (batchnorm.hip) no utterance sees another: a batch row equals the utterance alone.
+//
+// Memory-bound: the floor is one read of the inputs and one write of the output.  A workgroup owns a STRIP of whole groups
+// (at least GN_STRIP_BYTES of a row) of one utterance and holds its rows in REGISTERS: it reads them once, takes the mean, then
+// the centred squares (two passes over registers, no cancellation), and writes.  An utterance too long for the registers is cut
+// into chunks: a first kernel leaves (mean, centred squares) of every chunk, or the backward's channel sums, a second reads the
+// rows again and applies.  Chunks merge by M2 = sum M2_i + n_i (mean_i - mean)^2 in a fixed order; no atomics.
+#include "common.h"
+
+namespace fs2 {
+
+constexpr int GN_THREADS = 512;
+constexpr int GN_STRIP_BYTES = 64;
+
+struct GnArgs {
+    const void* x;           // [M, ldx]
+    const int* cu;           // [B + 1]
+    const float* gamma;
+    const float* beta;
+    void* out;               // [M, ldo]
+    float* stats;            // [B][G][2] mean, rstd
+    const void* dout;        // [M, ldd]
+    void* dx;                // [M, ldg]
+    float* part;             // forward chunks: [B][nchunk][G][2] mean, M2; backward: [B][nchunk][2][C] sums of dz, dz xhat
+    int M, C, G, cg, ldx, ldo, ldd, ldg, act, nchunk, nstrip;
+    int W, LX, LY;           // channels of a strip, lanes per row, rows per pass of the workgroup
+    float eps;
+    Dropout drop;
+};
+
+// ---- activations: 0 none, 1 ReLU, 2 tanh, 3 SiLU -------------------------------------------------------------------
+// tanh from one exp2 and one reciprocal, 1 - 2 / (1 + e^2z): absolute error below 2e-7.  Near zero, where that would lose
+// relative accuracy, the odd series to z^9 (the next term is below 1e-8 relative at 1/4).
+__device__ __forceinline__ float gn_tanh(float z) {
+    const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * 2.8853900817779268f));
+    const float u = z * z;
+    const float series = z * fmaf(u, fmaf(u, fmaf(u, fmaf(u, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return fabsf(z) < 0.25f ? series : t;
+}
+__device__ __forceinline__ float gn_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+}
+__device__ __forceinline__ float gn_act(float z, int act) {
+    if (act == 1) return z > 0.f ? z : (z == z ? 0.f : z);
+    if (act == 2) return gn_tanh(z);
+    if (act == 3) return z == -INFINITY ? 0.f : z * gn_sigmoid(z);
+    return z;
+}
+__device__ __forceinline__ float gn_slope(float z, int act) {
+    if (act == 1) return z > 0.f ? 1.f : 0.f;
+    if (act == 2) {
+        const float t = gn_tanh(z);
+        return fmaf(-t, t, 1.0f);
+    }
+    if (act == 3) {
+        const float s = gn_sigmoid(z);
+        return s * fmaf(z, 1.0f - s, 1.0f);
+    }
+    return 1.0f;
+}
+
+// ---- V consecutive channels of a row: raw registers and their values ---------------------------------------------------
+template <typename T, int V> struct GnVec { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ GnVec<T, V> gn_load(const T* p) {
+    GnVec<T, V> r;
+    if constexpr (V * sizeof(T) == 32) {
+        *(vec16*)&r.v[0] = *(const vec16*)p;
+        *(vec16*)&r.v[V / 2] = *(const vec16*)(p + V / 2);
+    } else if constexpr (V * sizeof(T) == 16) {
+        *(vec16*)&r.v[0] = *(const vec16*)p;
+    } else {
+        *(uint2*)&r.v[0] = *(const uint2*)p;
+    }
+    return r;
+}
+template <typename T, int V> __device__ __forceinline__ void gn_store(T* p, const float (&f)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) store4<T>(p + j, (f32x4){f[j], f[j + 1], f[j + 2], f[j + 3]});
+}
+
+struct GnPlace { int b, chunk, strip, r0, len, x, y, c0; bool on; };
+// workgroup -> (utterance, chunk, strip); thread -> (lane x of the strip's row, row y of a pass).  len: rows of THIS chunk.
+template <int V, int R> __device__ __forceinline__ GnPlace gn_place(const GnArgs& a, int& total) {
+    GnPlace p;
+    int id = blockIdx.x;
+    p.strip = id % a.nstrip;
+    id /= a.nstrip;
+    p.chunk = id % a.nchunk;
+    p.b = id / a.nchunk;
+    const int c0 = min(max(a.cu[p.b], 0), a.M), c1 = min(max(a.cu[p.b + 1], c0), a.M);
+    total = c1 - c0;
+    const int rows = a.LY * R, first = min(p.chunk * rows, total);
+    p.r0 = c0 + first;
+    p.len = min(total - first, rows);
+    p.y = threadIdx.x / a.LX;
+    p.x = threadIdx.x - p.y * a.LX;
+    p.on = p.y < a.LY;
+    p.c0 = p.strip * a.W + p.x * V;
+    return p;
+}
+
+// LDS: red [LY][W] (at most threads x V floats), mid [threads], chan [W], grp [W]
+// totals of a strip's channels over the workgroup's rows -> chan
+template <int V>
+__device__ __forceinline__ void gn_channel_sums(const GnArgs& a, const GnPlace& p, const float (&s)[V], float* red, float* mid,
+                                                float* chan) {
+    if (p.on) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) *(f32x4*)(red + p.y * a.W + p.x * V + j) = (f32x4){s[j], s[j + 1], s[j + 2], s[j + 3]};
+    }
+    __syncthreads();
+    if (a.W <= GN_THREADS) {
+        const int parts = GN_THREADS / a.W, part = threadIdx.x / a.W, c = threadIdx.x - part * a.W;
+        if (part < parts) {
+            float t = 0.f;
+            for (int y = part; y < a.LY; y += parts) t += red[y * a.W + c];
+            mid[part * a.W + c] = t;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < a.W) {
+            float t = 0.f;
+            for (int q = 0; q < parts; ++q) t += mid[q * a.W + threadIdx.x];
+            chan[threadIdx.x] = t;
+        }
+    } else {
+        for (int c = threadIdx.x; c < a.W; c += GN_THREADS) {
+            float t = 0.f;
+            for (int y = 0; y < a.LY; ++y) t += red[y * a.W + c];
+            chan[c] = t;
+        }
+    }
+    __syncthreads();
+}
+// sum over a group's channels of chan[c] (* w[c]) -> grp[group of the strip], one wave per group
+__device__ __forceinline__ void gn_group_sums(const GnArgs& a, const float* chan, const float* w, float* grp) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ng = a.W / a.cg;
+    for (int gi = wave; gi < ng; gi += GN_THREADS / 64) {
+        float t = 0.f;
+        for (int c = lane; c < a.cg; c += 64) t += w ? chan[gi * a.cg + c] * w[gi * a.cg + c] : chan[gi * a.cg + c];
+        t = wave_sum(t);
+        if (lane == 0) grp[gi] = t;
+    }
+    __syncthreads();
+}
+
+#define GN_LDS(V)                                     \
+    __shared__ float red[GN_THREADS * V];             \
+    __shared__ float mid[GN_THREADS];                 \
+    extern __shared__ float gn_dyn[]; /* chan [W], chan2 [W], grp [W / cg], grp2 [W / cg] */ \
+    float* chan = gn_dyn;                             \
+    float* chan2 = chan + a.W;                        \
+    float* grp = chan2 + a.W;                         \
+    float* grp2 = grp + a.W / a.cg
+
+// y rows from x rows in registers or memory, given the groups' mean (grp) and rstd (grp2) in LDS
+template <typename TX, typename TO, int V>
+__device__ __forceinline__ void gn_write_row(const GnArgs& a, int row, int c0, const GnVec<TX, V>& x, const float (&mean)[V],
+                                             const float (&rg)[V], const float (&be)[V]) {
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float z = gn_act(fmaf(to_f32(x.v[j]) - mean[j], rg[j], be[j]), a.act);
+        if (a.drop.thresh) z *= drop_mul(a.drop, (uint32_t)row, (uint32_t)(c0 + j));
+        o[j] = z;
+    }
+    gn_store<TO, V>((TO*)a.out + (size_t)row * a.ldo + c0, o);
+}
+
+// WHOLE: the utterance fits (nchunk == 1): statistics and output in one pass.  Else: (mean, M2) of the chunk to part.
+template <typename TX, typename TO, int R, bool WHOLE>
+__global__ __launch_bounds__(GN_THREADS) void gn_fwd_kernel(GnArgs a) {
+    constexpr int V = 16 / (int)sizeof(TX);
+    GN_LDS(V);
+    int total;
+    const GnPlace p = gn_place<V, R>(a, total);
+    if (!WHOLE && p.len == 0) return;                       // (block-uniform)
+    GnVec<TX, V> x[R];
+    const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int row = p.y + k * a.LY;
+        if (p.on && row < p.len) x[k] = gn_load<TX, V>(src + (size_t)row * a.ldx);
+    }
+    float s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+        if (p.on && p.y + k * a.LY < p.len) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] += to_f32(x[k].v[j]);
+        }
+    gn_channel_sums<V>(a, p, s, red, mid, chan);
+    gn_group_sums(a, chan, nullptr, grp);
+    const float inv_n = p.len > 0 ? 1.0f / ((float)p.len * (float)a.cg) : 0.f;
+    float mean[V];
+    int gi[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        gi[j] = p.on ? (p.x * V + j) / a.cg : 0;
+        mean[j] = grp[gi[j]] * inv_n;
+        s[j] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+        if (p.on && p.y + k * a.LY < p.len) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = to_f32(x[k].v[j]) - mean[j];
+                s[j] = fmaf(d, d, s[j]);
+            }
+        }
+    gn_channel_sums<V>(a, p, s, red, mid, chan);
+    gn_group_sums(a, chan, nullptr, grp2);
+    const int g0 = p.strip * (a.W / a.cg), ng = a.W / a.cg;
+    if (!WHOLE) {
+        float* dst = a.part + (((size_t)p.b * a.nchunk + p.chunk) * a.G + g0) * 2;
+        for (int t = threadIdx.x; t < ng; t += GN_THREADS) {
+            dst[t * 2] = grp[t] * inv_n;
+            dst[t * 2 + 1] = grp2[t];
+        }
+        return;
+    }
+    for (int t = threadIdx.x; t < ng; t += GN_THREADS) {
+        float* st = a.stats + ((size_t)p.b * a.G + g0 + t) * 2;
+        st[0] = grp[t] * inv_n;
+        st[1] = 1.0f / sqrtf(grp2[t] * inv_n + a.eps);
+    }
+    if (!p.on) return;
+    float rg[V], be[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        rg[j] = (1.0f / sqrtf(grp2[gi[j]] * inv_n + a.eps)) * a.gamma[p.c0 + j];
+        be[j] = a.beta[p.c0 + j];
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int row = p.y + k * a.LY;
+        if (row < p.len) gn_write_row<TX, TO, V>(a, p.r0 + row, p.c0, x[k], mean, rg, be);
+    }
+}
+
+// chunked forward, second kernel: merge the chunks' statistics, apply
+template <typename TX, typename TO, int R>
+__global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(GnArgs a) {
+    constexpr int V = 16 / (int)sizeof(TX);
+    extern __shared__ float gn_dyn[];
+    float *grp = gn_dyn, *grp2 = gn_dyn + a.W / a.cg;
+    int total;
+    const GnPlace p = gn_place<V, R>(a, total);
+    if (p.len == 0 && p.chunk > 0) return;
+    const int g0 = p.strip * (a.W / a.cg), ng = a.W / a.cg, rows = a.LY * R, nch = min((total + rows - 1) / rows, a.nchunk);
+    const float n_all = (float)min(total, a.nchunk * rows) * (float)a.cg;
+    for (int t = threadIdx.x; t < ng; t += GN_THREADS) {
+        const float* src = a.part + ((size_t)p.b * a.nchunk * a.G + g0 + t) * 2;
+        const size_t step = (size_t)a.G * 2;
+        float mean = 0.f, m2 = 0.f;
+        for (int c = 0; c < nch; ++c) mean = fmaf(src[c * step], (float)min(total - c * rows, rows) * (float)a.cg / n_all, mean);
+        for (int c = 0; c < nch; ++c) {
+            const float d = src[c * step] - mean;
+            m2 += fmaf(d * d, (float)min(total - c * rows, rows) * (float)a.cg, src[c * step + 1]);
+        }
+        const float rstd = 1.0f / sqrtf((n_all > 0.f ? m2 / n_all : 0.f) + a.eps);
+        grp[t] = mean;
+        grp2[t] = rstd;
+        if (p.chunk == 0) {
+            float* st = a.stats + ((size_t)p.b * a.G + g0 + t) * 2;
+            st[0] = mean;
+            st[1] = rstd;
+        }
+    }
+    __syncthreads();
+    if (!p.on) return;
+    float mean[V], rg[V], be[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int gi = (p.x * V + j) / a.cg;
+        mean[j] = grp[gi];
+        rg[j] = grp2[gi] * a.gamma[p.c0 + j];
+        be[j] = a.beta[p.c0 + j];
+    }
+    const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
+#pragma unroll 4
+    for (int k = 0; k < R; ++k) {
+        const int row = p.y + k * a.LY;
+        if (row < p.len) gn_write_row<TX, TO, V>(a, p.r0 + row, p.c0, gn_load<TX, V>(src + (size_t)row * a.ldx), mean, rg, be);
+    }
+}
+
+template <typename TD, int V>
+__device__ __forceinline__ void gn_dz(const GnArgs& a, int row, int c0, const GnVec<TD, V>& d, const float (&xh)[V],
+                                      const float (&ga)[V], const float (&be)[V], float (&dz)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float u = to_f32(d.v[j]);
+        if (a.drop.thresh) u *= drop_mul(a.drop, (uint32_t)row, (uint32_t)(c0 + j));
+        dz[j] = a.act ? u * gn_slope(fmaf(xh[j], ga[j], be[j]), a.act) : u;
+    }
+}
+
+// WHOLE: sums and dx in one pass; always: the chunk's channel sums of dz and dz xhat to part
+template <typename TX, typename TD, typename TG, int R, bool WHOLE>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_kernel(GnArgs a) {
+    constexpr int V = 16 / (int)sizeof(TX);
+    GN_LDS(V);
+    int total;
+    const GnPlace p = gn_place<V, R>(a, total);
+    float mean[V], rs[V], ga[V], be[V];
+    int gi[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        gi[j] = p.on ? (p.x * V + j) / a.cg : 0;
+        const int c = p.on ? p.c0 + j : p.strip * a.W;
+        const float* st = a.stats + ((size_t)p.b * a.G + p.strip * (a.W / a.cg) + gi[j]) * 2;
+        mean[j] = st[0];
+        rs[j] = st[1];
+        ga[j] = a.gamma[c];
+        be[j] = a.beta[c];
+    }
+    GnVec<TX, V> x[R];
+    GnVec<TD, V> d[R];
+    const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
+    const TD* sd = (const TD*)a.dout + (size_t)p.r0 * a.ldd + p.c0;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int row = p.y + k * a.LY;
+        if (p.on && row < p.len) {
+            x[k] = gn_load<TX, V>(src + (size_t)row * a.ldx);
+            d[k] = gn_load<TD, V>(sd + (size_t)row * a.ldd);
+        }
+    }
+    float s0[V], s1[V];
+    float dz[WHOLE ? R : 1][V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int row = p.y + k * a.LY;
+        if (p.on && row < p.len) {
+            float xh[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) xh[j] = (to_f32(x[k].v[j]) - mean[j]) * rs[j];
+            gn_dz<TD, V>(a, p.r0 + row, p.c0, d[k], xh, ga, be, dz[WHOLE ? k : 0]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                s0[j] += dz[WHOLE ? k : 0][j];
+                s1[j] = fmaf(dz[WHOLE ? k : 0][j], xh[j], s1[j]);
+            }
+        }
+    }
+    gn_channel_sums<V>(a, p, s0, red, mid, chan);
+    gn_channel_sums<V>(a, p, s1, red, mid, chan2);
+    float* dst = a.part + ((size_t)p.b * a.nchunk + p.chunk) * 2 * a.C + p.strip * a.W;
+    for (int c = threadIdx.x; c < a.W; c += GN_THREADS) {
+        dst[c] = chan[c];
+        dst[a.C + c] = chan2[c];
+    }
+    if (!WHOLE) return;
+    gn_group_sums(a, chan, a.gamma + p.strip * a.W, grp);
+    gn_group_sums(a, chan2, a.gamma + p.strip * a.W, grp2);
+    if (!p.on) return;
+    const float inv_n = p.len > 0 ? 1.0f / ((float)p.len * (float)a.cg) : 0.f;
+    float m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        m1[j] = grp[gi[j]] * inv_n;
+        m2[j] = grp2[gi[j]] * inv_n;
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int row = p.y + k * a.LY;
+        if (row < p.len) {
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (to_f32(x[k].v[j]) - mean[j]) * rs[j];
+                o[j] = rs[j] * (fmaf(ga[j], dz[k][j], -m1[j]) - xh * m2[j]);
+            }
+            gn_store<TG, V>((TG*)a.dx + (size_t)(p.r0 + row) * a.ldg + p.c0, o);
+        }
+    }
+}
+
+// chunked backward, second kernel: the utterance's sums from the chunks', then dx from a second read
+template <typename TX, typename TD, typename TG, int R>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(GnArgs a) {
+    constexpr int V = 16 / (int)sizeof(TX);
+    extern __shared__ float gn_dyn[];
+    float *chan = gn_dyn, *chan2 = chan + a.W, *grp = chan2 + a.W, *grp2 = grp + a.W / a.cg;
+    int total;
+    const GnPlace p = gn_place<V, R>(a, total);
+    if (p.len == 0) return;
+    const int rows = a.LY * R, nch = min((total + rows - 1) / rows, a.nchunk);
+    for (int c = threadIdx.x; c < 2 * a.W; c += GN_THREADS) {
+        const int which = c >= a.W, ch = c - which * a.W;
+        const float* src = a.part + (size_t)p.b * a.nchunk * 2 * a.C + which * a.C + p.strip * a.W + ch;
+        float t = 0.f;
+        for (int q = 0; q < nch; ++q) t += src[(size_t)q * 2 * a.C];
+        chan[c] = t;                                            // chan2 follows chan
+    }
+    __syncthreads();
+    gn_group_sums(a, chan, a.gamma + p.strip * a.W, grp);
+    gn_group_sums(a, chan2, a.gamma + p.strip * a.W, grp2);
+    if (!p.on) return;
+    const float inv_n = 1.0f / ((float)min(total, a.nchunk * rows) * (float)a.cg);
+    float mean[V], rs[V], ga[V], be[V], m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int gi = (p.x * V + j) / a.cg;
+        const float* st = a.stats + ((size_t)p.b * a.G + p.strip * (a.W / a.cg) + gi) * 2;
+        mean[j] = st[0];
+        rs[j] = st[1];
+        ga[j] = a.gamma[p.c0 + j];
+        be[j] = a.beta[p.c0 + j];
+        m1[j] = grp[gi] * inv_n;
+        m2[j] = grp2[gi] * inv_n;
+    }
+    const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
+    const TD* sd = (const TD*)a.dout + (size_t)p.r0 * a.ldd + p.c0;
+#pragma unroll 4
+    for (int k = 0; k < R; ++k) {
+        const int row = p.y + k * a.LY;
+        if (row < p.len) {
+            const GnVec<TX, V> x = gn_load<TX, V>(src + (size_t)row * a.ldx);
+            const GnVec<TD, V> d = gn_load<TD, V>(sd + (size_t)row * a.ldd);
+            float xh[V], dz[V], o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) xh[j] = (to_f32(x.v[j]) - mean[j]) * rs[j];
+            gn_dz<TD, V>(a, p.r0 + row, p.c0, d, xh, ga, be, dz);
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = rs[j] * (fmaf(ga[j], dz[j], -m1[j]) - xh[j] * m2[j]);
+            gn_store<TG, V>((TG*)a.dx + (size_t)(p.r0 + row) * a.ldg + p.c0, o);
+        }
+    }
+}
+
+// dgamma, dbeta: sums of the partial rows [n][2][C]; 64 columns x 16 row lanes per workgroup, f64 across the lanes' sums
+__global__ __launch_bounds__(1024) void gn_param_kernel(const float* __restrict__ part, int n, int C, float* __restrict__ dgamma,
+                                                        float* __restrict__ dbeta) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    float t = 0.f;
+    if (c < 2 * C)
+        for (int r = y; r < n; r += 16) t += part[(size_t)r * 2 * C + c];
+    red[y][lane] = t;
+    __syncthreads();
+    if (y == 0 && c < 2 * C) {
+        double sum = 0.0;
+        for (int k = 0; k < 16; ++k) sum += (double)red[k][lane];
+        if (c < C)
+            dbeta[c] = (float)sum;
+        else
+            dgamma[c - C] = (float)sum;
+    }
+}
+
+// ---- geometry ------------------------------------------------------------------------------------------------------
+// Strip: the narrowest run of whole groups and whole vectors that is at least GN_STRIP_BYTES wide and divides C.  R: rows
+// per thread, the smallest compiled one that holds the utterance; none does: chunks of the largest.
+struct GnPlan { int W, LX, LY, R, nchunk; bool whole; };
+
+static int gn_gcd(int a, int b) { return b ? gn_gcd(b, a % b) : a; }
+
+static GnPlan gn_plan(int max_len, int C, int G, int x_dtype, bool backward) {
+    GnPlan p;
+    const int V = x_dtype == 0 ? 4 : 8, es = x_dtype == 0 ? 4 : 2, cg = C / G;
+    const int unit = cg / gn_gcd(cg, V) * V, units = C / unit;
+    int m = 1;
+    while (m < units && (m * unit * es < GN_STRIP_BYTES || units % m)) ++m;
+    p.W = m * unit;
+    p.LX = p.W / V;
+    p.LY = GN_THREADS / p.LX;
+    const int most = !backward ? 16 : (x_dtype == 0 ? 16 : 8);
+    const int need = (max_len + p.LY - 1) / p.LY;
+    p.whole = need <= most;
+    p.R = need <= 4 ? 4 : (need <= 8 ? 8 : 16);
+    if (!p.whole) p.R = 8;
+    p.nchunk = p.whole ? 1 : (max_len + p.LY * p.R - 1) / (p.LY * p.R);
+    return p;
+}
+
+template <typename TX, typename TO, int R> static void gn_launch_fwd(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
+    const unsigned grid = (unsigned)((long long)B * p.nchunk * a.nstrip);
+    const int lds = (2 * a.W + 2 * (a.W / a.cg)) * (int)sizeof(float);
+    if (p.whole) {
+        hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, true>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+    } else if constexpr (R == 8) {
+        hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, false>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+        hipLaunchKernelGGL((gn_apply_kernel<TX, TO, R>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+    }
+}
+template <typename TX, typename TO> static void gn_launch_fwd_r(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
+    if (p.R == 4) gn_launch_fwd<TX, TO, 4>(a, p, B, s);
+    else if (p.R == 8) gn_launch_fwd<TX, TO, 8>(a, p, B, s);
+    else gn_launch_fwd<TX, TO, 16>(a, p, B, s);
+}
+
+template <typename TX, typename TD, typename TG, int R>
+static void gn_launch_bwd(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
+    const unsigned grid = (unsigned)((long long)B * p.nchunk * a.nstrip);
+    const int lds = (2 * a.W + 2 * (a.W / a.cg)) * (int)sizeof(float);
+    if (p.whole) {
+        hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, true>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+    } else if constexpr (R == 8) {
+        hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, false>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<TX, TD, TG, R>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+    }
+}
+template <typename TX, typename TD, typename TG> static void gn_launch_bwd_r(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
+    if (p.R == 4) gn_launch_bwd<TX, TD, TG, 4>(a, p, B, s);
+    else if (p.R == 8) gn_launch_bwd<TX, TD, TG, 8>(a, p, B, s);
+    else if constexpr (sizeof(TX) == 4) gn_launch_bwd<TX, TD, TG, 16>(a, p, B, s);
+}
+
+static int gn_check(const char* who, const void* x, const int* cu, const float* gamma, const float* beta, const float* stats, int B,
+                    int max_len, int M, int C, int groups, int ldx, int act, int x_dtype, float rate) {
+    FS2_CHECK_ARG(cu && gamma && beta && stats && (x || M == 0) && B > 0 && M >= 0, "%s: bad args", who);
+    FS2_CHECK_ARG(max_len >= 0 && max_len <= M && B <= (1 << 24), "%s: B=%d, max_len=%d, M=%d", who, B, max_len, M);
+    FS2_CHECK_ARG(x_dtype == 0 || x_dtype == 1, "%s: x_dtype=%d (0 fp32, 1 bf16)", who, x_dtype);
+    const int V = x_dtype == 0 ? 4 : 8;
+    FS2_CHECK_ARG(C > 0 && C <= 2048 && C % V == 0, "%s: C=%d must be a multiple of %d and at most 2048", who, C, V);
+    FS2_CHECK_ARG(groups > 0 && C % groups == 0, "%s: %d channels in %d groups", who, C, groups);
+    FS2_CHECK_ARG(ldx >= C && ldx % V == 0 && ((uintptr_t)x & 15) == 0, "%s: ldx=%d, or x unaligned", who, ldx);
+    FS2_CHECK_ARG(act >= 0 && act <= 3, "%s: act=%d (0 none, 1 ReLU, 2 tanh, 3 SiLU)", who, act);
+    FS2_CHECK_ARG(rate >= 0.f && rate < 1.f, "%s: dropout rate must be in [0, 1)", who);
+    return FS2_OK;
+}
+
+static GnArgs gn_args(const void* x, const int* cu, const float* gamma, const float* beta, float* stats, void* workspace, int M, int C,
+                      int groups, int ldx, int act, const GnPlan& p, Dropout drop) {
+    GnArgs a = {};
+    a.x = x; a.cu = cu; a.gamma = gamma; a.beta = beta; a.stats = stats; a.part = (float*)workspace;
+    a.M = M; a.C = C; a.G = groups; a.cg = C / groups; a.ldx = ldx; a.act = act;
+    a.nchunk = p.nchunk; a.nstrip = C / p.W; a.W = p.W; a.LX = p.LX; a.LY = p.LY;
+    a.drop = drop;
+    return a;
+}
+
+}  // namespace fs2
+
+using namespace fs2;
+
+extern "C" long long fs2_group_norm_workspace(int B, int max_len, int C, int groups) {
+    if (B <= 0 || C <= 0 || groups <= 0 || C % groups || C % 4) return 0;
+    long long most = 0;
+    for (int t = 0; t < (C % 8 ? 1 : 2); ++t) {
+        const GnPlan p = gn_plan(max_len, C, groups, t, false);
+        const long long n = p.whole ? 0 : (long long)B * p.nchunk * groups * 2 * (long long)sizeof(float);
+        most = n > most ? n : most;
+    }
+    return most;
+}
+
+extern "C" int fs2_group_norm(const void* x, const int* cu, const float* gamma, const float* beta, void* out, float* stats,
+                              void* workspace, int B, int max_len, int M, int C, int groups, int ldx, int ldo, float eps, int act,
+                              int x_dtype, int out_dtype, unsigned seed, unsigned site, float rate, hipStream_t stream) {
+    const int rc = gn_check("fs2_group_norm", x, cu, gamma, beta, stats, B, max_len, M, C, groups, ldx, act, x_dtype, rate);
+    if (rc != FS2_OK) return rc;
+    FS2_CHECK_ARG((out_dtype == 0 || out_dtype == 1) && (out || M == 0) && ldo >= C && ldo % 4 == 0 && ((uintptr_t)out & 15) == 0,
+                  "fs2_group_norm: out_dtype=%d, ldo=%d (a multiple of 4), or out null or unaligned", out_dtype, ldo);
+    FS2_CHECK_ARG(eps > 0.f, "fs2_group_norm: eps must be positive");
+    const GnPlan p = gn_plan(max_len, C, groups, x_dtype, false);
+    FS2_CHECK_ARG(p.whole || workspace, "fs2_group_norm: this shape needs fs2_group_norm_workspace bytes");
+    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 31), "fs2_group_norm: too many workgroups (B=%d)", B);
+    GnArgs a = gn_args(x, cu, gamma, beta, stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
+    a.out = out; a.ldo = ldo; a.eps = eps;
+    if (x_dtype == 0 && out_dtype == 0) gn_launch_fwd_r<float, float>(a, p, B, stream);
+    else if (x_dtype == 0) gn_launch_fwd_r<float, bf16_t>(a, p, B, stream);
+    else if (out_dtype == 0) gn_launch_fwd_r<bf16_t, float>(a, p, B, stream);
+    else gn_launch_fwd_r<bf16_t, bf16_t>(a, p, B, stream);
+    FS2_CHECK_LAUNCH("fs2_group_norm");
+    return FS2_OK;
+}
+
+extern "C" long long fs2_group_norm_bwd_workspace(int B, int max_len, int C, int groups) {
+    if (B <= 0 || C <= 0 || groups <= 0 || C % groups || C % 4) return 16;
+    long long most = 0;
+    for (int t = 0; t < (C % 8 ? 1 : 2); ++t) {
+        const GnPlan p = gn_plan(max_len, C, groups, t, true);
+        const long long n = (long long)B * p.nchunk * 2 * C * (long long)sizeof(float);
+        most = n > most ? n : most;
+    }
+    return most;
+}
+
+extern "C" int fs2_group_norm_bwd(const void* x, const float* stats, const int* cu, const float* gamma, const float* beta,
+                                  const void* dout, void* dx, float* dgamma, float* dbeta, void* workspace, int B, int max_len, int M,
+                                  int C, int groups, int ldx, int ldd, int ldg, int act, int x_dtype, int dout_dtype, int dx_dtype,
+                                  unsigned seed, unsigned site, float rate, hipStream_t stream) {
+    const int rc = gn_check("fs2_group_norm_bwd", x, cu, gamma, beta, stats, B, max_len, M, C, groups, ldx, act, x_dtype, rate);
+    if (rc != FS2_OK) return rc;
+    FS2_CHECK_ARG((dout_dtype == 0 || dout_dtype == 1) && (dx_dtype == 0 || dx_dtype == 1),
+                  "fs2_group_norm_bwd: dout_dtype=%d, dx_dtype=%d (0 fp32, 1 bf16)", dout_dtype, dx_dtype);
+    FS2_CHECK_ARG((M == 0 || (dout && dx)) && dgamma && dbeta && workspace, "fs2_group_norm_bwd: null argument");
+    FS2_CHECK_ARG(ldd >= C && ldg >= C && ldd % (x_dtype == 0 ? 4 : 8) == 0 && ldg % 4 == 0 &&
+                      (((uintptr_t)dout | (uintptr_t)dx) & 15) == 0,
+                  "fs2_group_norm_bwd: ldd=%d (a multiple of %d), ldg=%d (of 4), or dout or dx unaligned", ldd, x_dtype == 0 ? 4 : 8,
+                  ldg);
+    const GnPlan p = gn_plan(max_len, C, groups, x_dtype, true);
+    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 31), "fs2_group_norm_bwd: too many workgroups (B=%d)", B);
+    GnArgs a = gn_args(x, cu, gamma, beta, (float*)stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
+    a.dout = dout; a.dx = dx; a.ldd = ldd; a.ldg = ldg;
+#define FS2_GN(TX, TD)                                              \
+    if (dx_dtype == 0) gn_launch_bwd_r<TX, TD, float>(a, p, B, stream); \
+    else gn_launch_bwd_r<TX, TD, bf16_t>(a, p, B, stream)
+    if (x_dtype == 0 && dout_dtype == 0) { FS2_GN(float, float); }
+    else if (x_dtype == 0) { FS2_GN(float, bf16_t); }
+    else if (dout_dtype == 0) { FS2_GN(bf16_t, float); }
+    else { FS2_GN(bf16_t, bf16_t); }
+#undef FS2_GN
+    hipLaunchKernelGGL(gn_param_kernel, dim3((2 * C + 63) / 64), dim3(1024), 0, stream, a.part, B * p.nchunk, C, dgamma, dbeta);
+    FS2_CHECK_LAUNCH("fs2_group_norm_bwd");
+    return FS2_OK;
+}

@@ -78,6 +78,12 @@ _SIGNATURES = {
     "fs2_bn_stats": [_P, _P, _P, _I, _I, _F, _P],
     "fs2_bn_apply": [_P, _P, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _U, _U, _F, _P],
     "fs2_bn_bwd": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _U, _U, _F, _P],
+    # alignment: cross attention, attention mass, per-utterance group norm
+    "fs2_cross_attention": [_P] * 8 + [_I] * 13 + [_U, _U, _F, _P],
+    "fs2_cross_attention_bwd": [_P] * 12 + [_I] * 13 + [_U, _U, _F, _P],
+    "fs2_cross_attention_mass": [_P] * 7 + [_I] * 11 + [_P],
+    "fs2_group_norm": [_P] * 7 + [_I] * 7 + [_F] + [_I] * 3 + [_U, _U, _F, _P],
+    "fs2_group_norm_bwd": [_P] * 10 + [_I] * 12 + [_U, _U, _F, _P],
 }
 # workspace-size queries (return bytes as long long, no launch)
 _SIZE_QUERIES = {
@@ -87,6 +93,11 @@ _SIZE_QUERIES = {
     "fs2_colreduce_static_max_bytes": [],
     "fs2_bn_workspace": [_I, _I],
     "fs2_attention_keysplit_workspace": [_I, _I, _I, _I],
+    "fs2_cross_attention_workspace": [_I] * 8,
+    "fs2_cross_attention_bwd_workspace": [_I] * 9,
+    "fs2_cross_attention_mass_workspace": [_I] * 8,
+    "fs2_group_norm_workspace": [_I] * 4,
+    "fs2_group_norm_bwd_workspace": [_I] * 4,
 }
 # plain int queries (no launch, cannot fail)
 _INT_QUERIES = {

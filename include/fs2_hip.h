@@ -409,6 +409,74 @@ int fs2_bn_bwd(const float* y, const float* stats, const float* gamma, const flo
                int ldd, float* dgamma, float* dbeta, void* dy_t, int ldt, float* workspace, int M, int C, int dtype,
                unsigned seed, unsigned site, float rate, hipStream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Alignment: the operators between a text and its frames that the reference leaves to a teacher model (it reads the
+ * durations of its corpus from files, run/train_decode.py:118-149): frames attending to phones, what every phone receives,
+ * and the per-utterance normalisation of the conv stacks around them.  No counterpart in the reference.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Cross attention over packed rows: utterance b's queries, rows cu_q[b] .. cu_q[b+1] of q [Mq, ldq], against its keys and
+ * values, rows cu_k[b] .. cu_k[b+1] of k [Mk, ldk] and v [Mk, ldv].  n_heads query heads over n_kv_heads key / value heads
+ * (n_kv_heads divides n_heads, at most 128 to one; head h reads shared head h / (n_heads / n_kv_heads)); head h sits at
+ * columns h * dk of q and ctx, a shared head j at columns j * dk of k and v (a fused k | v projection: v = k + n_kv_heads * dk,
+ * ldk = ldv).  dk in {32, 64, 96, 128}; T = fp32 or bf16; leading dims multiples of 16 bytes.
+ *   ctx = dropout(softmax(q k^T / sqrt(dk))) v  [Mq, ldo] T;   lse [n_heads][Mq] (may be NULL): log2-domain log-sum-exp
+ * An utterance without keys gets ctx = 0, lse = -inf; rows behind cu_q[B] are left as they were.  max_q / max_k: at least the
+ * longest utterance of either side, at most Mq / Mk (queries beyond max_q of an utterance are not computed).  Serves one
+ * query per utterance (autoregressive decoding against fixed encoder states) to whole batches; the kernel and a split of the
+ * keys over workgroups follow from the shape.  Softmax statistics and sums are fp32; bf16 rounds the probabilities and the
+ * result.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row = packed query row, col =
+ * key index inside the utterance; rate 0 = none).
+ * workspace: fs2_cross_attention_workspace bytes, 16-byte aligned (0: NULL is fine).  It is written by every call: two calls
+ * that may overlap (streams, captured graphs) need one each. */
+long long fs2_cross_attention_workspace(int B, int max_q, int max_k, int Mq, int n_heads, int n_kv_heads, int dk, int dtype);
+int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, float* lse, const int* cu_q, const int* cu_k,
+                        void* workspace, int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk, int ldq,
+                        int ldk, int ldv, int ldo, int dtype, unsigned seed, unsigned stream_id, float rate, hipStream_t stream);
+
+/* Its backward, from ctx and lse as fs2_cross_attention left them and dctx [Mq, ldo] T: dq [Mq, ldq], dk_out [Mk, ldk],
+ * dv [Mk, ldv] T (the leading dims of q, k, v; written, not added to; gradients of a shared head sum over its query heads).
+ * Probabilities are recomputed; every element has one writer and every sum a fixed order.  workspace:
+ * fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, never NULL; one per call that may overlap. */
+long long fs2_cross_attention_bwd_workspace(int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk,
+                                            int dtype);
+int fs2_cross_attention_bwd(const void* q, const void* k, const void* v, const void* ctx, const void* dctx, const float* lse,
+                            void* dq, void* dk_out, void* dv, const int* cu_q, const int* cu_k, void* workspace, int B, int max_q,
+                            int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk, int ldq, int ldk, int ldv, int ldo,
+                            int dtype, unsigned seed, unsigned stream_id, float rate, hipStream_t stream);
+
+/* mass [n_heads][Mk] fp32: the attention every key received, mass[h][m] = sum over its utterance's queries of
+ * softmax(q k^T / sqrt(dk))[query, m], from lse as fs2_cross_attention left it (no dropout: the undropped probabilities).
+ * With frames as queries and phones as keys this is the expected duration of each phone in frames; a head's masses of an
+ * utterance sum to its frame count.  Elements of rows behind cu_k[B] are left as they were.  workspace:
+ * fs2_cross_attention_mass_workspace bytes (0: NULL is fine). */
+long long fs2_cross_attention_mass_workspace(int B, int max_q, int max_k, int Mk, int n_heads, int n_kv_heads, int dk, int dtype);
+int fs2_cross_attention_mass(const void* q, const void* k, const float* lse, float* mass, const int* cu_q, const int* cu_k,
+                             void* workspace, int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk,
+                             int ldq, int ldk, int dtype, hipStream_t stream);
+
+/* Group norm of each utterance's rows with an activation, channels last: x [M, ldx] (x_dtype), utterance b = rows
+ * cu[b] .. cu[b+1] (at most max_len <= M of them); mean and biased variance over its rows x the C / groups channels of a group,
+ *   out [M, ldo] (out_dtype) = dropout(act(gamma * (x - mean) / sqrt(var + eps) + beta)),
+ * act 0 none, 1 ReLU, 2 tanh, 3 SiLU; dropout element (site, row, col) as in the other training kernels.  stats
+ * [B][groups][2] = mean, 1 / sqrt(var + eps) (0, 1 / sqrt(eps) for an utterance without rows).  Dtypes 0 fp32, 1 bf16, each on
+ * its own; C % 4 == 0 (fp32 x) or 8 (bf16 x), C <= 2048, any group size; ldo % 4 == 0.  The per-utterance counterpart of
+ * fs2_bn_stats + fs2_bn_apply: a batch row equals the utterance alone.  Statistics in fp32 from centred squares.
+ * workspace: fs2_group_norm_workspace bytes (0: NULL is fine). */
+long long fs2_group_norm_workspace(int B, int max_len, int C, int groups);
+int fs2_group_norm(const void* x, const int* cu, const float* gamma, const float* beta, void* out, float* stats, void* workspace,
+                   int B, int max_len, int M, int C, int groups, int ldx, int ldo, float eps, int act, int x_dtype, int out_dtype,
+                   unsigned seed, unsigned site, float rate, hipStream_t stream);
+
+/* Its backward from x and stats alone (activation and dropout are recomputed): dout [M, ldd] (dout_dtype, ldd a multiple of 16
+ * bytes of x's type), dx [M, ldg] (dx_dtype), dgamma, dbeta fp32 [C] (sums over all utterances in a fixed order).  workspace:
+ * fs2_group_norm_bwd_workspace bytes, never NULL. */
+long long fs2_group_norm_bwd_workspace(int B, int max_len, int C, int groups);
+int fs2_group_norm_bwd(const void* x, const float* stats, const int* cu, const float* gamma, const float* beta, const void* dout,
+                       void* dx, float* dgamma, float* dbeta, void* workspace, int B, int max_len, int M, int C, int groups, int ldx,
+                       int ldd, int ldg, int act, int x_dtype, int dout_dtype, int dx_dtype, unsigned seed, unsigned site,
+                       float rate, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
