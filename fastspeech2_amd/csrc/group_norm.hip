@@ -14,7 +14,10 @@
 
 namespace fs2 {
 
-constexpr int GN_THREADS = 512;
+// Threads of a workgroup: 512 where it holds a whole utterance's strip, 256 where it streams a chunk (80 channels, 256
+// utterances of 800 rows, backward sums: 50 us with 512 threads, 27 with 256: the small groups overlap each other's phases).
+constexpr int GN_WHOLE_THREADS = 512, GN_CHUNK_THREADS = 256;
+constexpr int GN_CHUNK_ROWS = 8;          // rows per thread of a chunk
 constexpr int GN_STRIP_BYTES = 64;
 
 struct GnArgs {
@@ -28,19 +31,21 @@ struct GnArgs {
     void* dx;                // [M, ldg]
     float* part;             // forward chunks: [B][nchunk][G][2] mean, M2; backward: [B][nchunk][2][C] sums of dz, dz xhat
     int M, C, G, cg, ldx, ldo, ldd, ldg, act, nchunk, nstrip;
+    int units;               // B * nchunk
     int W, LX, LY;           // channels of a strip, lanes per row, rows per pass of the workgroup
+    float inv_lx, inv_cg;    // 1 / LX, 1 / cg
     float eps;
     Dropout drop;
 };
 
 // ---- activations: 0 none, 1 ReLU, 2 tanh, 3 SiLU -------------------------------------------------------------------
 // tanh from one exp2 and one reciprocal, 1 - 2 / (1 + e^2z): absolute error below 2e-7.  Near zero, where that would lose
-// relative accuracy, the odd series to z^9 (the next term is below 1e-8 relative at 1/4).
+// relative accuracy, the odd series to z^5 (the next term is below 4e-9 relative at 1/16).
 __device__ __forceinline__ float gn_tanh(float z) {
-    const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * 2.8853900817779268f));
+    const float t = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * 2.8853900817779268f)), 1.0f);
     const float u = z * z;
-    const float series = z * fmaf(u, fmaf(u, fmaf(u, fmaf(u, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    return fabsf(z) < 0.25f ? series : t;
+    const float series = z * fmaf(u, fmaf(u, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
+    return fabsf(z) < 0.0625f ? series : t;
 }
 __device__ __forceinline__ float gn_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
@@ -65,16 +70,32 @@ __device__ __forceinline__ float gn_slope(float z, int act) {
 }
 
 // ---- V consecutive channels of a row: raw registers and their values ---------------------------------------------------
-template <typename T, int V> struct GnVec { T v[V]; };
+template <typename T, int V> struct GnVec {
+    uint32_t w[V * sizeof(T) / 4];
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[j]);
+        return __builtin_bit_cast(float, j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+    }
+    // the registers as they are: keeps the compiler from holding the widened values of a bf16 vector between two passes
+    __device__ __forceinline__ void keep_raw() {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < (int)(V * sizeof(T) / 4); ++j) asm volatile("" : "+v"(w[j]));
+        }
+    }
+};
 template <typename T, int V> __device__ __forceinline__ GnVec<T, V> gn_load(const T* p) {
     GnVec<T, V> r;
-    if constexpr (V * sizeof(T) == 32) {
-        *(vec16*)&r.v[0] = *(const vec16*)p;
-        *(vec16*)&r.v[V / 2] = *(const vec16*)(p + V / 2);
-    } else if constexpr (V * sizeof(T) == 16) {
-        *(vec16*)&r.v[0] = *(const vec16*)p;
+    constexpr int N = V * sizeof(T) / 4;
+    if constexpr (N == 2) {
+        const uint2 t = *(const uint2*)p;
+        r.w[0] = t.x; r.w[1] = t.y;
     } else {
-        *(uint2*)&r.v[0] = *(const uint2*)p;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const vec16 t = *((const vec16*)p + j / 4);
+            r.w[j] = t.x; r.w[j + 1] = t.y; r.w[j + 2] = t.z; r.w[j + 3] = t.w;
+        }
     }
     return r;
 }
@@ -84,78 +105,143 @@ template <typename T, int V> __device__ __forceinline__ void gn_store(T* p, cons
 }
 
 struct GnPlace { int b, chunk, strip, r0, len, x, y, c0; bool on; };
-// workgroup -> (utterance, chunk, strip); thread -> (lane x of the strip's row, row y of a pass).  len: rows of THIS chunk.
+// n / d for 0 <= n < 2^13, d >= 1: the error of the fp32 quotient stays below the half that is added
+__device__ __forceinline__ int gn_div(int n, float inv) { return (int)(((float)n + 0.5f) * inv); }
+
+// workgroup -> (utterance, chunk, strip): the strips of one chunk share cache lines of its rows, so they are dealt to one XCD
+// (workgroup ids go round-robin over the 8).  Thread -> (lane x of the strip's row, row y of a pass): whole rows to a wave
+// where a row has at most 64 lanes.  len: rows of THIS chunk.
 template <int V, int R> __device__ __forceinline__ GnPlace gn_place(const GnArgs& a, int& total) {
     GnPlace p;
-    int id = blockIdx.x;
-    p.strip = id % a.nstrip;
-    id /= a.nstrip;
-    p.chunk = id % a.nchunk;
-    p.b = id / a.nchunk;
+    int unit;
+    if (a.units >= 8) {
+        const int slot = blockIdx.x >> 3;
+        unit = (blockIdx.x & 7) + 8 * (slot / a.nstrip);
+        p.strip = slot % a.nstrip;
+    } else {
+        unit = blockIdx.x / a.nstrip;
+        p.strip = blockIdx.x % a.nstrip;
+    }
+    total = 0;
+    p.b = -1;
+    if (unit >= a.units) return p;
+    p.chunk = unit % a.nchunk;
+    p.b = unit / a.nchunk;
     const int c0 = min(max(a.cu[p.b], 0), a.M), c1 = min(max(a.cu[p.b + 1], c0), a.M);
     total = c1 - c0;
     const int rows = a.LY * R, first = min(p.chunk * rows, total);
     p.r0 = c0 + first;
     p.len = min(total - first, rows);
-    p.y = threadIdx.x / a.LX;
-    p.x = threadIdx.x - p.y * a.LX;
-    p.on = p.y < a.LY;
+    if (a.LX <= 64) {
+        const int lane = threadIdx.x & 63, rw = gn_div(64, a.inv_lx), y = gn_div(lane, a.inv_lx);
+        p.x = lane - y * a.LX;
+        p.on = y < rw;
+        p.y = (threadIdx.x >> 6) * rw + y;
+    } else {
+        p.y = gn_div(threadIdx.x, a.inv_lx);
+        p.x = threadIdx.x - p.y * a.LX;
+        p.on = p.y < a.LY;
+    }
     p.c0 = p.strip * a.W + p.x * V;
     return p;
 }
 
-// LDS: red [LY][W] (at most threads x V floats), mid [threads], chan [W], grp [W]
-// totals of a strip's channels over the workgroup's rows -> chan
-template <int V>
-__device__ __forceinline__ void gn_channel_sums(const GnArgs& a, const GnPlace& p, const float (&s)[V], float* red, float* mid,
-                                                float* chan) {
-    if (p.on) {
+// Sums of a strip's columns over the workgroup's rows -> red [entries][w], w = LX * N columns (N values of a lane), entries =
+// waves, or the rows of a pass where a row takes several waves.  In a wave: through its own N * 64 floats of `tmp`, every
+// column read by as many lanes as there are for it, those joined by shuffles (half the LDS traffic of shuffling all N values
+// over all rows).  The caller puts a barrier behind it.
+template <int N> __device__ __forceinline__ void gn_put_sums(const GnArgs& a, const GnPlace& p, const float (&s)[N], float* tmp, float* red) {
+    const int w = a.LX * N;
+    if (a.LX > 64) {
+        if (p.on) {
 #pragma unroll
-        for (int j = 0; j < V; j += 4) *(f32x4*)(red + p.y * a.W + p.x * V + j) = (f32x4){s[j], s[j + 1], s[j + 2], s[j + 3]};
+            for (int j = 0; j < N; ++j) red[p.y * w + p.x * N + j] = s[j];
+        }
+        return;
     }
-    __syncthreads();
-    if (a.W <= GN_THREADS) {
-        const int parts = GN_THREADS / a.W, part = threadIdx.x / a.W, c = threadIdx.x - part * a.W;
-        if (part < parts) {
-            float t = 0.f;
-            for (int y = part; y < a.LY; y += parts) t += red[y * a.W + c];
-            mid[part * a.W + c] = t;
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < a.W) {
-            float t = 0.f;
-            for (int q = 0; q < parts; ++q) t += mid[q * a.W + threadIdx.x];
-            chan[threadIdx.x] = t;
-        }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = gn_div(64, a.inv_lx);
+    float* t = tmp + wave * 64 * N;
+    if constexpr (N == 1) {
+        t[lane] = s[0];
     } else {
-        for (int c = threadIdx.x; c < a.W; c += GN_THREADS) {
-            float t = 0.f;
-            for (int y = 0; y < a.LY; ++y) t += red[y * a.W + c];
-            chan[c] = t;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *(f32x4*)(t + lane * N + j) = (f32x4){s[j], s[j + 1], s[j + 2], s[j + 3]};
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (w <= 64) {
+        const float inv_w = a.inv_lx * (1.0f / N);
+        int parts = min(gn_div(64, inv_w), rows);
+        const int part = gn_div(lane, inv_w), c = lane - part * w;
+        float v = 0.f;
+        if (part < parts)
+            for (int y = part; y < rows; y += parts) v += t[y * w + c];
+        while (parts > 1) {                      // (uniform)
+            const int half = (parts + 1) >> 1;
+            const float o = __shfl(v, lane + half * w, 64);
+            if (part + half < parts) v += o;
+            parts = half;
+        }
+        if (part == 0) red[wave * w + c] = v;
+    } else {
+        for (int c = lane; c < w; c += 64) {
+            float v = 0.f;
+            for (int y = 0; y < rows; ++y) v += t[y * w + c];
+            red[wave * w + c] = v;
         }
     }
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();
 }
-// sum over a group's channels of chan[c] (* w[c]) -> grp[group of the strip], one wave per group
-__device__ __forceinline__ void gn_group_sums(const GnArgs& a, const float* chan, const float* w, float* grp) {
+// sum over red's entries and a group's `n` columns (* weight[column]) -> grp[group of the strip], one wave per group
+template <int NT>
+__device__ __forceinline__ void gn_group_sums(const GnArgs& a, const float* red, int w, int n, const float* weight, float* grp) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ng = a.W / a.cg;
-    for (int gi = wave; gi < ng; gi += GN_THREADS / 64) {
+    const int entries = a.LX <= 64 ? NT / 64 : a.LY;
+    for (int gi = wave; gi < ng; gi += NT / 64) {
         float t = 0.f;
-        for (int c = lane; c < a.cg; c += 64) t += w ? chan[gi * a.cg + c] * w[gi * a.cg + c] : chan[gi * a.cg + c];
+        for (int c = gi * n + lane; c < gi * n + n; c += 64) {
+            float u = 0.f;
+#pragma unroll 4
+            for (int e = 0; e < entries; ++e) u += red[e * w + c];
+            t += weight ? u * weight[c] : u;
+        }
         t = wave_sum(t);
         if (lane == 0) grp[gi] = t;
+    }
+}
+// the group sums of per-channel values: a lane whose vector lies inside one group adds it up first
+template <int V, int NT>
+__device__ __forceinline__ void gn_reduce(const GnArgs& a, const GnPlace& p, const float (&s)[V], float* tmp, float* red, float* grp) {
+    if (a.cg % V == 0) {
+        float t[1] = {0.f};
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[0] += s[j];
+        gn_put_sums<1>(a, p, t, tmp, red);
+        __syncthreads();
+        gn_group_sums<NT>(a, red, a.LX, a.cg / V, nullptr, grp);
+    } else {
+        gn_put_sums<V>(a, p, s, tmp, red);
+        __syncthreads();
+        gn_group_sums<NT>(a, red, a.W, a.cg, nullptr, grp);
     }
     __syncthreads();
 }
 
-#define GN_LDS(V)                                     \
-    __shared__ float red[GN_THREADS * V];             \
-    __shared__ float mid[GN_THREADS];                 \
-    extern __shared__ float gn_dyn[]; /* chan [W], chan2 [W], grp [W / cg], grp2 [W / cg] */ \
-    float* chan = gn_dyn;                             \
-    float* chan2 = chan + a.W;                        \
-    float* grp = chan2 + a.W;                         \
-    float* grp2 = grp + a.W / a.cg
+// LDS: a wave's staging, the entries of one or two sums, then two values per group of the strip
+#define GN_LDS(V, NT, N)                                                   \
+    __shared__ __attribute__((aligned(16))) float tmp[NT * V];             \
+    __shared__ __attribute__((aligned(16))) float red[N][NT * V];          \
+    extern __shared__ float gn_dyn[];                                      \
+    float* grp = gn_dyn;                                                   \
+    float* grp2 = gn_dyn + a.W / a.cg
+
+template <int V> __device__ __forceinline__ void gn_params(const float* src, float (&f)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+        const f32x4 t = *(const f32x4*)(src + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[j + e] = t[e];
+    }
+}
 
 // y rows from x rows in registers or memory, given the groups' mean (grp) and rstd (grp2) in LDS
 template <typename TX, typename TO, int V>
@@ -164,7 +250,7 @@ __device__ __forceinline__ void gn_write_row(const GnArgs& a, int row, int c0, c
     float o[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float z = gn_act(fmaf(to_f32(x.v[j]) - mean[j], rg[j], be[j]), a.act);
+        float z = gn_act(fmaf(x.get(j) - mean[j], rg[j], be[j]), a.act);
         if (a.drop.thresh) z *= drop_mul(a.drop, (uint32_t)row, (uint32_t)(c0 + j));
         o[j] = z;
     }
@@ -173,12 +259,13 @@ __device__ __forceinline__ void gn_write_row(const GnArgs& a, int row, int c0, c
 
 // WHOLE: the utterance fits (nchunk == 1): statistics and output in one pass.  Else: (mean, M2) of the chunk to part.
 template <typename TX, typename TO, int R, bool WHOLE>
-__global__ __launch_bounds__(GN_THREADS) void gn_fwd_kernel(GnArgs a) {
+__global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void gn_fwd_kernel(GnArgs a) {
+    constexpr int NT = WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS;
     constexpr int V = 16 / (int)sizeof(TX);
-    GN_LDS(V);
+    GN_LDS(V, NT, 1);
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
-    if (!WHOLE && p.len == 0) return;                       // (block-uniform)
+    if (p.b < 0 || (!WHOLE && p.len == 0)) return;          // (block-uniform)
     GnVec<TX, V> x[R];
     const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
 #pragma unroll
@@ -193,51 +280,52 @@ __global__ __launch_bounds__(GN_THREADS) void gn_fwd_kernel(GnArgs a) {
     for (int k = 0; k < R; ++k)
         if (p.on && p.y + k * a.LY < p.len) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[j] += to_f32(x[k].v[j]);
+            for (int j = 0; j < V; ++j) s[j] += x[k].get(j);
         }
-    gn_channel_sums<V>(a, p, s, red, mid, chan);
-    gn_group_sums(a, chan, nullptr, grp);
+    gn_reduce<V, NT>(a, p, s, tmp, red[0], grp);
     const float inv_n = p.len > 0 ? 1.0f / ((float)p.len * (float)a.cg) : 0.f;
     float mean[V];
     int gi[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        gi[j] = p.on ? (p.x * V + j) / a.cg : 0;
+        gi[j] = p.on ? gn_div(p.x * V + j, a.inv_cg) : 0;
         mean[j] = grp[gi[j]] * inv_n;
         s[j] = 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < R; ++k) x[k].keep_raw();
 #pragma unroll
     for (int k = 0; k < R; ++k)
         if (p.on && p.y + k * a.LY < p.len) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = to_f32(x[k].v[j]) - mean[j];
+                const float d = x[k].get(j) - mean[j];
                 s[j] = fmaf(d, d, s[j]);
             }
         }
-    gn_channel_sums<V>(a, p, s, red, mid, chan);
-    gn_group_sums(a, chan, nullptr, grp2);
+    gn_reduce<V, NT>(a, p, s, tmp, red[0], grp2);
     const int g0 = p.strip * (a.W / a.cg), ng = a.W / a.cg;
     if (!WHOLE) {
         float* dst = a.part + (((size_t)p.b * a.nchunk + p.chunk) * a.G + g0) * 2;
-        for (int t = threadIdx.x; t < ng; t += GN_THREADS) {
+        for (int t = threadIdx.x; t < ng; t += NT) {
             dst[t * 2] = grp[t] * inv_n;
             dst[t * 2 + 1] = grp2[t];
         }
         return;
     }
-    for (int t = threadIdx.x; t < ng; t += GN_THREADS) {
+    for (int t = threadIdx.x; t < ng; t += NT) {
         float* st = a.stats + ((size_t)p.b * a.G + g0 + t) * 2;
         st[0] = grp[t] * inv_n;
         st[1] = 1.0f / sqrtf(grp2[t] * inv_n + a.eps);
     }
     if (!p.on) return;
     float rg[V], be[V];
+    gn_params<V>(a.gamma + p.c0, rg);
+    gn_params<V>(a.beta + p.c0, be);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        rg[j] = (1.0f / sqrtf(grp2[gi[j]] * inv_n + a.eps)) * a.gamma[p.c0 + j];
-        be[j] = a.beta[p.c0 + j];
-    }
+    for (int j = 0; j < V; ++j) rg[j] *= 1.0f / sqrtf(grp2[gi[j]] * inv_n + a.eps);
+#pragma unroll
+    for (int k = 0; k < R; ++k) x[k].keep_raw();
 #pragma unroll
     for (int k = 0; k < R; ++k) {
         const int row = p.y + k * a.LY;
@@ -247,16 +335,17 @@ __global__ __launch_bounds__(GN_THREADS) void gn_fwd_kernel(GnArgs a) {
 
 // chunked forward, second kernel: merge the chunks' statistics, apply
 template <typename TX, typename TO, int R>
-__global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(GnArgs a) {
+__global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_apply_kernel(GnArgs a) {
+    constexpr int NT = GN_CHUNK_THREADS;
     constexpr int V = 16 / (int)sizeof(TX);
     extern __shared__ float gn_dyn[];
     float *grp = gn_dyn, *grp2 = gn_dyn + a.W / a.cg;
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
-    if (p.len == 0 && p.chunk > 0) return;
+    if (p.b < 0 || (p.len == 0 && p.chunk > 0)) return;
     const int g0 = p.strip * (a.W / a.cg), ng = a.W / a.cg, rows = a.LY * R, nch = min((total + rows - 1) / rows, a.nchunk);
     const float n_all = (float)min(total, a.nchunk * rows) * (float)a.cg;
-    for (int t = threadIdx.x; t < ng; t += GN_THREADS) {
+    for (int t = threadIdx.x; t < ng; t += NT) {
         const float* src = a.part + ((size_t)p.b * a.nchunk * a.G + g0 + t) * 2;
         const size_t step = (size_t)a.G * 2;
         float mean = 0.f, m2 = 0.f;
@@ -277,12 +366,13 @@ __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(GnArgs a) {
     __syncthreads();
     if (!p.on) return;
     float mean[V], rg[V], be[V];
+    gn_params<V>(a.gamma + p.c0, rg);
+    gn_params<V>(a.beta + p.c0, be);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int gi = (p.x * V + j) / a.cg;
+        const int gi = gn_div(p.x * V + j, a.inv_cg);
         mean[j] = grp[gi];
-        rg[j] = grp2[gi] * a.gamma[p.c0 + j];
-        be[j] = a.beta[p.c0 + j];
+        rg[j] *= grp2[gi];
     }
     const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
 #pragma unroll 4
@@ -297,80 +387,105 @@ __device__ __forceinline__ void gn_dz(const GnArgs& a, int row, int c0, const Gn
                                       const float (&ga)[V], const float (&be)[V], float (&dz)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float u = to_f32(d.v[j]);
+        float u = d.get(j);
         if (a.drop.thresh) u *= drop_mul(a.drop, (uint32_t)row, (uint32_t)(c0 + j));
         dz[j] = a.act ? u * gn_slope(fmaf(xh[j], ga[j], be[j]), a.act) : u;
     }
 }
 
-// WHOLE: sums and dx in one pass; always: the chunk's channel sums of dz and dz xhat to part
-template <typename TX, typename TD, typename TG, int R, bool WHOLE>
-__global__ __launch_bounds__(GN_THREADS) void gn_bwd_kernel(GnArgs a) {
-    constexpr int V = 16 / (int)sizeof(TX);
-    GN_LDS(V);
-    int total;
-    const GnPlace p = gn_place<V, R>(a, total);
-    float mean[V], rs[V], ga[V], be[V];
-    int gi[V];
+// mean, rstd, gamma, beta of a lane's channels
+template <int V>
+__device__ __forceinline__ void gn_lane_params(const GnArgs& a, const GnPlace& p, float (&mean)[V], float (&rs)[V], float (&ga)[V],
+                                               float (&be)[V]) {
+    const int c0 = p.on ? p.c0 : p.strip * a.W;
+    const float* st = a.stats + (size_t)p.b * a.G * 2;
+    gn_params<V>(a.gamma + c0, ga);
+    gn_params<V>(a.beta + c0, be);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        gi[j] = p.on ? (p.x * V + j) / a.cg : 0;
-        const int c = p.on ? p.c0 + j : p.strip * a.W;
-        const float* st = a.stats + ((size_t)p.b * a.G + p.strip * (a.W / a.cg) + gi[j]) * 2;
-        mean[j] = st[0];
-        rs[j] = st[1];
-        ga[j] = a.gamma[c];
-        be[j] = a.beta[c];
+        const int gi = gn_div(c0 + j, a.inv_cg);
+        mean[j] = st[gi * 2];
+        rs[j] = st[gi * 2 + 1];
     }
-    GnVec<TX, V> x[R];
-    GnVec<TD, V> d[R];
+}
+
+// WHOLE: sums and dx in one pass; always: the chunk's channel sums of dz and dz xhat to part
+template <typename TX, typename TD, typename TG, int R, bool WHOLE>
+__global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void gn_bwd_kernel(GnArgs a) {
+    constexpr int NT = WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS;
+    constexpr int V = 16 / (int)sizeof(TX);
+    GN_LDS(V, NT, 2);
+    int total;
+    const GnPlace p = gn_place<V, R>(a, total);
+    if (p.b < 0) return;
+    constexpr int HOLD = WHOLE ? R : 4;                     // rows in registers at a time
+    GnVec<TX, V> x[HOLD];
+    GnVec<TD, V> d[HOLD];
+    float dz[WHOLE ? R : 1][V];
     const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
     const TD* sd = (const TD*)a.dout + (size_t)p.r0 * a.ldd + p.c0;
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-        const int row = p.y + k * a.LY;
-        if (p.on && row < p.len) {
-            x[k] = gn_load<TX, V>(src + (size_t)row * a.ldx);
-            d[k] = gn_load<TD, V>(sd + (size_t)row * a.ldd);
-        }
-    }
+    float mean[V], rs[V], ga[V], be[V];
+    if (!WHOLE) gn_lane_params<V>(a, p, mean, rs, ga, be);
     float s0[V], s1[V];
-    float dz[WHOLE ? R : 1][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
+#pragma unroll 1
+    for (int k0 = 0; k0 < R; k0 += HOLD) {
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-        const int row = p.y + k * a.LY;
-        if (p.on && row < p.len) {
-            float xh[V];
+        for (int k = 0; k < HOLD; ++k) {
+            const int row = p.y + (k0 + k) * a.LY;
+            if (p.on && row < p.len) {
+                x[k] = gn_load<TX, V>(src + (size_t)row * a.ldx);
+                d[k] = gn_load<TD, V>(sd + (size_t)row * a.ldd);
+            }
+        }
+        if (WHOLE) gn_lane_params<V>(a, p, mean, rs, ga, be);       // behind the rows' loads
 #pragma unroll
-            for (int j = 0; j < V; ++j) xh[j] = (to_f32(x[k].v[j]) - mean[j]) * rs[j];
-            gn_dz<TD, V>(a, p.r0 + row, p.c0, d[k], xh, ga, be, dz[WHOLE ? k : 0]);
+        for (int k = 0; k < HOLD; ++k) {
+            const int row = p.y + (k0 + k) * a.LY;
+            if (p.on && row < p.len) {
+                float xh[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                s0[j] += dz[WHOLE ? k : 0][j];
-                s1[j] = fmaf(dz[WHOLE ? k : 0][j], xh[j], s1[j]);
+                for (int j = 0; j < V; ++j) xh[j] = (x[k].get(j) - mean[j]) * rs[j];
+                gn_dz<TD, V>(a, p.r0 + row, p.c0, d[k], xh, ga, be, dz[WHOLE ? k : 0]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    s0[j] += dz[WHOLE ? k : 0][j];
+                    s1[j] = fmaf(dz[WHOLE ? k : 0][j], xh[j], s1[j]);
+                }
             }
         }
     }
-    gn_channel_sums<V>(a, p, s0, red, mid, chan);
-    gn_channel_sums<V>(a, p, s1, red, mid, chan2);
+    gn_put_sums<V>(a, p, s0, tmp, red[0]);
+    gn_put_sums<V>(a, p, s1, tmp, red[1]);
+    __syncthreads();
     float* dst = a.part + ((size_t)p.b * a.nchunk + p.chunk) * 2 * a.C + p.strip * a.W;
-    for (int c = threadIdx.x; c < a.W; c += GN_THREADS) {
-        dst[c] = chan[c];
-        dst[a.C + c] = chan2[c];
+    const int entries = a.LX <= 64 ? NT / 64 : a.LY;
+    for (int c = threadIdx.x; c < a.W; c += NT) {
+        float t0 = 0.f, t1 = 0.f;
+#pragma unroll 8
+        for (int e = 0; e < entries; ++e) {
+            t0 += red[0][e * a.W + c];
+            t1 += red[1][e * a.W + c];
+        }
+        dst[c] = t0;
+        dst[a.C + c] = t1;
     }
     if (!WHOLE) return;
-    gn_group_sums(a, chan, a.gamma + p.strip * a.W, grp);
-    gn_group_sums(a, chan2, a.gamma + p.strip * a.W, grp2);
+    gn_group_sums<NT>(a, red[0], a.W, a.cg, a.gamma + p.strip * a.W, grp);
+    gn_group_sums<NT>(a, red[1], a.W, a.cg, a.gamma + p.strip * a.W, grp2);
+    __syncthreads();
     if (!p.on) return;
     const float inv_n = p.len > 0 ? 1.0f / ((float)p.len * (float)a.cg) : 0.f;
     float m1[V], m2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        m1[j] = grp[gi[j]] * inv_n;
-        m2[j] = grp2[gi[j]] * inv_n;
+        const int gi = gn_div(p.x * V + j, a.inv_cg);
+        m1[j] = grp[gi] * inv_n;
+        m2[j] = grp2[gi] * inv_n;
     }
+#pragma unroll
+    for (int k = 0; k < R; ++k) x[k].keep_raw();
 #pragma unroll
     for (int k = 0; k < R; ++k) {
         const int row = p.y + k * a.LY;
@@ -378,7 +493,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_kernel(GnArgs a) {
             float o[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = (to_f32(x[k].v[j]) - mean[j]) * rs[j];
+                const float xh = (x[k].get(j) - mean[j]) * rs[j];
                 o[j] = rs[j] * (fmaf(ga[j], dz[k][j], -m1[j]) - xh * m2[j]);
             }
             gn_store<TG, V>((TG*)a.dx + (size_t)(p.r0 + row) * a.ldg + p.c0, o);
@@ -388,35 +503,44 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_kernel(GnArgs a) {
 
 // chunked backward, second kernel: the utterance's sums from the chunks', then dx from a second read
 template <typename TX, typename TD, typename TG, int R>
-__global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(GnArgs a) {
+__global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_bwd_apply_kernel(GnArgs a) {
+    constexpr int NT = GN_CHUNK_THREADS;
     constexpr int V = 16 / (int)sizeof(TX);
     extern __shared__ float gn_dyn[];
-    float *chan = gn_dyn, *chan2 = chan + a.W, *grp = chan2 + a.W, *grp2 = grp + a.W / a.cg;
+    float *grp = gn_dyn, *grp2 = grp + a.W / a.cg;
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
-    if (p.len == 0) return;
-    const int rows = a.LY * R, nch = min((total + rows - 1) / rows, a.nchunk);
-    for (int c = threadIdx.x; c < 2 * a.W; c += GN_THREADS) {
-        const int which = c >= a.W, ch = c - which * a.W;
-        const float* src = a.part + (size_t)p.b * a.nchunk * 2 * a.C + which * a.C + p.strip * a.W + ch;
-        float t = 0.f;
-        for (int q = 0; q < nch; ++q) t += src[(size_t)q * 2 * a.C];
-        chan[c] = t;                                            // chan2 follows chan
+    if (p.b < 0 || p.len == 0) return;
+    const int rows = a.LY * R, nch = min((total + rows - 1) / rows, a.nchunk), ng = a.W / a.cg;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float* part = a.part + (size_t)p.b * a.nchunk * 2 * a.C + p.strip * a.W;
+    for (int gi = wave; gi < ng; gi += NT / 64) {
+        float t0 = 0.f, t1 = 0.f;
+        for (int c = gi * a.cg + lane; c < gi * a.cg + a.cg; c += 64) {
+            float u0 = 0.f, u1 = 0.f;
+            for (int q = 0; q < nch; ++q) {
+                u0 += part[(size_t)q * 2 * a.C + c];
+                u1 += part[(size_t)q * 2 * a.C + a.C + c];
+            }
+            const float w = a.gamma[p.strip * a.W + c];
+            t0 = fmaf(u0, w, t0);
+            t1 = fmaf(u1, w, t1);
+        }
+        t0 = wave_sum(t0);
+        t1 = wave_sum(t1);
+        if (lane == 0) {
+            grp[gi] = t0;
+            grp2[gi] = t1;
+        }
     }
     __syncthreads();
-    gn_group_sums(a, chan, a.gamma + p.strip * a.W, grp);
-    gn_group_sums(a, chan2, a.gamma + p.strip * a.W, grp2);
     if (!p.on) return;
     const float inv_n = 1.0f / ((float)min(total, a.nchunk * rows) * (float)a.cg);
     float mean[V], rs[V], ga[V], be[V], m1[V], m2[V];
+    gn_lane_params<V>(a, p, mean, rs, ga, be);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int gi = (p.x * V + j) / a.cg;
-        const float* st = a.stats + ((size_t)p.b * a.G + p.strip * (a.W / a.cg) + gi) * 2;
-        mean[j] = st[0];
-        rs[j] = st[1];
-        ga[j] = a.gamma[p.c0 + j];
-        be[j] = a.beta[p.c0 + j];
+        const int gi = gn_div(p.x * V + j, a.inv_cg);
         m1[j] = grp[gi] * inv_n;
         m2[j] = grp2[gi] * inv_n;
     }
@@ -430,7 +554,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(GnArgs a) {
             const GnVec<TD, V> d = gn_load<TD, V>(sd + (size_t)row * a.ldd);
             float xh[V], dz[V], o[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) xh[j] = (to_f32(x.v[j]) - mean[j]) * rs[j];
+            for (int j = 0; j < V; ++j) xh[j] = (x.get(j) - mean[j]) * rs[j];
             gn_dz<TD, V>(a, p.r0 + row, p.c0, d, xh, ga, be, dz);
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = rs[j] * (fmaf(ga[j], dz[j], -m1[j]) - xh[j] * m2[j]);
@@ -439,19 +563,22 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(GnArgs a) {
     }
 }
 
-// dgamma, dbeta: sums of the partial rows [n][2][C]; 64 columns x 16 row lanes per workgroup, f64 across the lanes' sums
+// dgamma, dbeta: sums of the partial rows [n][2][C]; 16 columns x 64 row lanes per workgroup, f64 over the row lanes' sums
 __global__ __launch_bounds__(1024) void gn_param_kernel(const float* __restrict__ part, int n, int C, float* __restrict__ dgamma,
                                                         float* __restrict__ dbeta) {
-    __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    __shared__ float red[64][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
     float t = 0.f;
-    if (c < 2 * C)
-        for (int r = y; r < n; r += 16) t += part[(size_t)r * 2 * C + c];
-    red[y][lane] = t;
+    if (c < 2 * C) {
+#pragma unroll 4
+        for (int r = y; r < n; r += 64) t += part[(size_t)r * 2 * C + c];
+    }
+    red[y][x] = t;
     __syncthreads();
     if (y == 0 && c < 2 * C) {
         double sum = 0.0;
-        for (int k = 0; k < 16; ++k) sum += (double)red[k][lane];
+#pragma unroll 8
+        for (int k = 0; k < 64; ++k) sum += (double)red[k][x];
         if (c < C)
             dbeta[c] = (float)sum;
         else
@@ -474,47 +601,53 @@ static GnPlan gn_plan(int max_len, int C, int G, int x_dtype, bool backward) {
     while (m < units && (m * unit * es < GN_STRIP_BYTES || units % m)) ++m;
     p.W = m * unit;
     p.LX = p.W / V;
-    p.LY = GN_THREADS / p.LX;
-    const int most = !backward ? 16 : (x_dtype == 0 ? 16 : 8);
-    const int need = (max_len + p.LY - 1) / p.LY;
-    p.whole = need <= most;
-    p.R = need <= 4 ? 4 : (need <= 8 ? 8 : 16);
-    if (!p.whole) p.R = 8;
-    p.nchunk = p.whole ? 1 : (max_len + p.LY * p.R - 1) / (p.LY * p.R);
+    const int most = !backward || x_dtype == 0 ? 16 : 8;
+    for (int nt = GN_WHOLE_THREADS;; nt = GN_CHUNK_THREADS) {
+        p.LY = p.LX <= 64 ? nt / 64 * (64 / p.LX) : nt / p.LX;
+        const int need = (max_len + p.LY - 1) / p.LY;
+        p.whole = nt == GN_WHOLE_THREADS && need <= most;
+        p.R = !p.whole ? GN_CHUNK_ROWS : (need <= 4 ? 4 : (need <= 8 ? 8 : 16));
+        p.nchunk = p.whole ? 1 : (max_len + p.LY * p.R - 1) / (p.LY * p.R);
+        if (p.whole || nt == GN_CHUNK_THREADS) break;
+    }
     return p;
 }
 
-template <typename TX, typename TO, int R> static void gn_launch_fwd(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
-    const unsigned grid = (unsigned)((long long)B * p.nchunk * a.nstrip);
-    const int lds = (2 * a.W + 2 * (a.W / a.cg)) * (int)sizeof(float);
+static unsigned gn_grid(const GnArgs& a) {
+    return (unsigned)(a.units >= 8 ? 8LL * a.nstrip * ((a.units + 7) / 8) : (long long)a.units * a.nstrip);
+}
+
+template <typename TX, typename TO, int R> static void gn_launch_fwd(const GnArgs& a, const GnPlan& p, hipStream_t s) {
+    const unsigned grid = gn_grid(a);
+    const int lds = 2 * (a.W / a.cg) * (int)sizeof(float);
     if (p.whole) {
-        hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, true>), dim3(grid), dim3(GN_THREADS), lds, s, a);
-    } else if constexpr (R == 8) {
-        hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, false>), dim3(grid), dim3(GN_THREADS), lds, s, a);
-        hipLaunchKernelGGL((gn_apply_kernel<TX, TO, R>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+        hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, true>), dim3(grid), dim3(GN_WHOLE_THREADS), lds, s, a);
+    } else if constexpr (R == GN_CHUNK_ROWS) {
+        hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, false>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
+        hipLaunchKernelGGL((gn_apply_kernel<TX, TO, R>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
     }
 }
-template <typename TX, typename TO> static void gn_launch_fwd_r(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
-    if (p.R == 4) gn_launch_fwd<TX, TO, 4>(a, p, B, s);
-    else if (p.R == 8) gn_launch_fwd<TX, TO, 8>(a, p, B, s);
-    else gn_launch_fwd<TX, TO, 16>(a, p, B, s);
+template <typename TX, typename TO> static void gn_launch_fwd_r(const GnArgs& a, const GnPlan& p, hipStream_t s) {
+    if (p.R == 4) gn_launch_fwd<TX, TO, 4>(a, p, s);
+    else if (p.R == 8) gn_launch_fwd<TX, TO, 8>(a, p, s);
+    else gn_launch_fwd<TX, TO, 16>(a, p, s);
 }
 
 template <typename TX, typename TD, typename TG, int R>
-static void gn_launch_bwd(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
-    const unsigned grid = (unsigned)((long long)B * p.nchunk * a.nstrip);
-    const int lds = (2 * a.W + 2 * (a.W / a.cg)) * (int)sizeof(float);
+static void gn_launch_bwd(const GnArgs& a, const GnPlan& p, hipStream_t s) {
+    const unsigned grid = gn_grid(a);
+    const int lds = 2 * (a.W / a.cg) * (int)sizeof(float);
     if (p.whole) {
-        hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, true>), dim3(grid), dim3(GN_THREADS), lds, s, a);
-    } else if constexpr (R == 8) {
-        hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, false>), dim3(grid), dim3(GN_THREADS), lds, s, a);
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<TX, TD, TG, R>), dim3(grid), dim3(GN_THREADS), lds, s, a);
+        hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, true>), dim3(grid), dim3(GN_WHOLE_THREADS), lds, s, a);
+    } else if constexpr (R == GN_CHUNK_ROWS) {
+        hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, false>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<TX, TD, TG, R>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
     }
 }
-template <typename TX, typename TD, typename TG> static void gn_launch_bwd_r(const GnArgs& a, const GnPlan& p, int B, hipStream_t s) {
-    if (p.R == 4) gn_launch_bwd<TX, TD, TG, 4>(a, p, B, s);
-    else if (p.R == 8) gn_launch_bwd<TX, TD, TG, 8>(a, p, B, s);
-    else if constexpr (sizeof(TX) == 4) gn_launch_bwd<TX, TD, TG, 16>(a, p, B, s);
+template <typename TX, typename TD, typename TG> static void gn_launch_bwd_r(const GnArgs& a, const GnPlan& p, hipStream_t s) {
+    if (p.R == 4) gn_launch_bwd<TX, TD, TG, 4>(a, p, s);
+    else if (p.R == 8) gn_launch_bwd<TX, TD, TG, 8>(a, p, s);
+    else if constexpr (sizeof(TX) == 4) gn_launch_bwd<TX, TD, TG, 16>(a, p, s);
 }
 
 static int gn_check(const char* who, const void* x, const int* cu, const float* gamma, const float* beta, const float* stats, int B,
@@ -523,7 +656,8 @@ static int gn_check(const char* who, const void* x, const int* cu, const float* 
     FS2_CHECK_ARG(max_len >= 0 && max_len <= M && B <= (1 << 24), "%s: B=%d, max_len=%d, M=%d", who, B, max_len, M);
     FS2_CHECK_ARG(x_dtype == 0 || x_dtype == 1, "%s: x_dtype=%d (0 fp32, 1 bf16)", who, x_dtype);
     const int V = x_dtype == 0 ? 4 : 8;
-    FS2_CHECK_ARG(C > 0 && C <= 2048 && C % V == 0, "%s: C=%d must be a multiple of %d and at most 2048", who, C, V);
+    FS2_CHECK_ARG((((uintptr_t)gamma | (uintptr_t)beta) & 15) == 0, "%s: gamma or beta unaligned", who);
+    FS2_CHECK_ARG(C > 0 && C <= 1024 && C % V == 0, "%s: C=%d must be a multiple of %d and at most 1024", who, C, V);
     FS2_CHECK_ARG(groups > 0 && C % groups == 0, "%s: %d channels in %d groups", who, C, groups);
     FS2_CHECK_ARG(ldx >= C && ldx % V == 0 && ((uintptr_t)x & 15) == 0, "%s: ldx=%d, or x unaligned", who, ldx);
     FS2_CHECK_ARG(act >= 0 && act <= 3, "%s: act=%d (0 none, 1 ReLU, 2 tanh, 3 SiLU)", who, act);
@@ -531,12 +665,13 @@ static int gn_check(const char* who, const void* x, const int* cu, const float* 
     return FS2_OK;
 }
 
-static GnArgs gn_args(const void* x, const int* cu, const float* gamma, const float* beta, float* stats, void* workspace, int M, int C,
+static GnArgs gn_args(int B, const void* x, const int* cu, const float* gamma, const float* beta, float* stats, void* workspace, int M, int C,
                       int groups, int ldx, int act, const GnPlan& p, Dropout drop) {
     GnArgs a = {};
     a.x = x; a.cu = cu; a.gamma = gamma; a.beta = beta; a.stats = stats; a.part = (float*)workspace;
     a.M = M; a.C = C; a.G = groups; a.cg = C / groups; a.ldx = ldx; a.act = act;
     a.nchunk = p.nchunk; a.nstrip = C / p.W; a.W = p.W; a.LX = p.LX; a.LY = p.LY;
+    a.units = B * p.nchunk; a.inv_lx = 1.0f / (float)p.LX; a.inv_cg = 1.0f / (float)a.cg;
     a.drop = drop;
     return a;
 }
@@ -566,13 +701,13 @@ extern "C" int fs2_group_norm(const void* x, const int* cu, const float* gamma, 
     FS2_CHECK_ARG(eps > 0.f, "fs2_group_norm: eps must be positive");
     const GnPlan p = gn_plan(max_len, C, groups, x_dtype, false);
     FS2_CHECK_ARG(p.whole || workspace, "fs2_group_norm: this shape needs fs2_group_norm_workspace bytes");
-    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 31), "fs2_group_norm: too many workgroups (B=%d)", B);
-    GnArgs a = gn_args(x, cu, gamma, beta, stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
+    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 30), "fs2_group_norm: too many workgroups (B=%d)", B);
+    GnArgs a = gn_args(B, x, cu, gamma, beta, stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
     a.out = out; a.ldo = ldo; a.eps = eps;
-    if (x_dtype == 0 && out_dtype == 0) gn_launch_fwd_r<float, float>(a, p, B, stream);
-    else if (x_dtype == 0) gn_launch_fwd_r<float, bf16_t>(a, p, B, stream);
-    else if (out_dtype == 0) gn_launch_fwd_r<bf16_t, float>(a, p, B, stream);
-    else gn_launch_fwd_r<bf16_t, bf16_t>(a, p, B, stream);
+    if (x_dtype == 0 && out_dtype == 0) gn_launch_fwd_r<float, float>(a, p, stream);
+    else if (x_dtype == 0) gn_launch_fwd_r<float, bf16_t>(a, p, stream);
+    else if (out_dtype == 0) gn_launch_fwd_r<bf16_t, float>(a, p, stream);
+    else gn_launch_fwd_r<bf16_t, bf16_t>(a, p, stream);
     FS2_CHECK_LAUNCH("fs2_group_norm");
     return FS2_OK;
 }
@@ -602,18 +737,18 @@ extern "C" int fs2_group_norm_bwd(const void* x, const float* stats, const int* 
                   "fs2_group_norm_bwd: ldd=%d (a multiple of %d), ldg=%d (of 4), or dout or dx unaligned", ldd, x_dtype == 0 ? 4 : 8,
                   ldg);
     const GnPlan p = gn_plan(max_len, C, groups, x_dtype, true);
-    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 31), "fs2_group_norm_bwd: too many workgroups (B=%d)", B);
-    GnArgs a = gn_args(x, cu, gamma, beta, (float*)stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
+    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 30), "fs2_group_norm_bwd: too many workgroups (B=%d)", B);
+    GnArgs a = gn_args(B, x, cu, gamma, beta, (float*)stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
     a.dout = dout; a.dx = dx; a.ldd = ldd; a.ldg = ldg;
 #define FS2_GN(TX, TD)                                              \
-    if (dx_dtype == 0) gn_launch_bwd_r<TX, TD, float>(a, p, B, stream); \
-    else gn_launch_bwd_r<TX, TD, bf16_t>(a, p, B, stream)
+    if (dx_dtype == 0) gn_launch_bwd_r<TX, TD, float>(a, p, stream); \
+    else gn_launch_bwd_r<TX, TD, bf16_t>(a, p, stream)
     if (x_dtype == 0 && dout_dtype == 0) { FS2_GN(float, float); }
     else if (x_dtype == 0) { FS2_GN(float, bf16_t); }
     else if (dout_dtype == 0) { FS2_GN(bf16_t, float); }
     else { FS2_GN(bf16_t, bf16_t); }
 #undef FS2_GN
-    hipLaunchKernelGGL(gn_param_kernel, dim3((2 * C + 63) / 64), dim3(1024), 0, stream, a.part, B * p.nchunk, C, dgamma, dbeta);
+    hipLaunchKernelGGL(gn_param_kernel, dim3((2 * C + 15) / 16), dim3(1024), 0, stream, a.part, B * p.nchunk, C, dgamma, dbeta);
     FS2_CHECK_LAUNCH("fs2_group_norm_bwd");
     return FS2_OK;
 }

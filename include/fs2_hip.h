@@ -460,7 +460,7 @@ int fs2_cross_attention_mass(const void* q, const void* k, const float* lse, flo
  *   out [M, ldo] (out_dtype) = dropout(act(gamma * (x - mean) / sqrt(var + eps) + beta)),
  * act 0 none, 1 ReLU, 2 tanh, 3 SiLU; dropout element (site, row, col) as in the other training kernels.  stats
  * [B][groups][2] = mean, 1 / sqrt(var + eps) (0, 1 / sqrt(eps) for an utterance without rows).  Dtypes 0 fp32, 1 bf16, each on
- * its own; C % 4 == 0 (fp32 x) or 8 (bf16 x), C <= 2048, any group size; ldo % 4 == 0.  The per-utterance counterpart of
+ * its own; C % 4 == 0 (fp32 x) or 8 (bf16 x), C <= 1024, any group size; ldo % 4 == 0.  The per-utterance counterpart of
  * fs2_bn_stats + fs2_bn_apply: a batch row equals the utterance alone.  Statistics in fp32 from centred squares.
  * workspace: fs2_group_norm_workspace bytes (0: NULL is fine). */
 long long fs2_group_norm_workspace(int B, int max_len, int C, int groups);

@@ -99,7 +99,7 @@ def _norm(**kw):
 NORM_REFUSED = [
     (dict(cu=None), "bad args"), (dict(gamma=None), "bad args"), (dict(beta=None), "bad args"), (dict(stats=None), "bad args"),
     (dict(x=None), "bad args"), (dict(B=0), "bad args"), (dict(max_len=17), "max_len=17"), (dict(x_dtype=2), "x_dtype=2"),
-    (dict(C=82, G=2), "C=82"), (dict(C=84, G=2, x_dtype=1), "C=84"), (dict(C=4096), "C=4096"), (dict(G=3), "80 channels in 3"),
+    (dict(C=82, G=2), "C=82"), (dict(C=84, G=2, x_dtype=1), "C=84"), (dict(C=1040, ldx=1040, ldo=1040), "C=1040"), (dict(G=3), "80 channels in 3"),
     (dict(ldx=76), "ldx=76"), (dict(ldx=82), "ldx=82"), (dict(x=P + 8), "unaligned"), (dict(act=4), "act=4"), (dict(rate=1.0), "dropout"),
 ]
 

@@ -436,8 +436,8 @@ NORMS = [
     ([900], 80, 2, "none"),
     ([2100, 40], 64, 4, "tanh"),                         # chunks for the backward
     ([9000, 3], 40, 8, "silu"),                          # chunks both ways
-    ([40, 3], 2048, 2, "none"),
-    ([70], 2048, 2048, "tanh"),
+    ([40, 3], 1024, 2, "none"),
+    ([70], 1024, 1024, "tanh"),
 ]
 
 
