@@ -23,7 +23,8 @@ struct XArgs {
     unsigned magic;      // floor(2^32 / g) + 1 (g > 1): r / g = umulhi(r, magic) for r < 2^24, g <= 128
     float scale_log2e;   // log2(e) / sqrt(dk)
     float scale;         // 1 / sqrt(dk)
-    PairOrder order;     // workgroup order over (utterance, shared head) pairs
+    int nblk, pairs;     // blocks of a pair, (utterance, head) pairs: see x_decode
+    unsigned kv_magic;   // 1 / heads-per-utterance of the pair index
     Dropout drop;        // dropout of the probabilities: site drop.stream + head, row = packed query row, col = key index
     int nsplit;          // ranges of the summed axis over workgroups (1: none), partial results to `part`
     float* part;
@@ -46,101 +47,246 @@ __device__ __forceinline__ void x_range(const int* cu, int b, int M, int& r0, in
 // packed row -> query index inside the utterance; head in group = r - q * g
 __device__ __forceinline__ int x_query(const XArgs& a, int r) { return a.g == 1 ? r : (int)__umulhi((unsigned)r, a.magic); }
 
-// Tiles of ROWS rows x DK in LDS: unpadded rows whose 16-byte slots are rotated by ROT * (row >> RSH), so that fragment reads
-// of 16 rows (ROT = 1) and transposed reads of 4 rows x 64 bytes (ROT = 2) spread over the banks; rows narrower than 256
-// bytes share a rotation where several of them make up one pass over the banks.  Filled by LDS-DMA (lane-linear on the LDS
-// side): the rotation goes into the source address.
-template <typename T, int DK, int ROWS = 64> struct XTile {
-    static constexpr int ROWB = DK * (int)sizeof(T);
+// Workgroup order.  Ids are dealt round-robin to the 8 XCDs, each with its own L2; the blocks of one (utterance, head) pair read
+// the same keys (or queries), so they go to one XCD: grid (8 nblk, pairs / 8, nsplit), pair 8 y + x % 8, block x / 8.  Fewer than 8
+// pairs would leave XCDs idle: grid (nblk, pairs, nsplit), dealt as they come.  Without a division but the pair's.
+__device__ __forceinline__ bool x_decode(const XArgs& a, int heads, int& b, int& h, int& blk, int& split) {
+    split = blockIdx.z;
+    int pair;
+    if (a.pairs >= 8) {
+        blk = blockIdx.x >> 3;
+        pair = blockIdx.y * 8 + (blockIdx.x & 7);
+    } else {
+        blk = blockIdx.x;
+        pair = blockIdx.y;
+    }
+    if (pair >= a.pairs) return false;
+    b = heads == 1 ? pair : (int)__umulhi((unsigned)pair, a.kv_magic);       // pair < 2^24, heads <= 4096: exact
+    h = pair - b * heads;
+    return true;
+}
+
+// ---- operands ---------------------------------------------------------------------------------------------------------
+// Both types run on the bf16 matrix pipe (v_mfma_f32_16x16x32_bf16, fp32 accumulation).
+//   XB16: bf16 operands as they are.
+//   XF32: an fp32 value is the exact sum of three bf16 numbers, its significand cut 8 + 8 + 8 bits (x0 = top half of x, x1 = top half of
+//         x - x0, x2 = the rest): a product of two is x0 y0 + (x0 y1 + x1 y0) + (x0 y2 + x1 y1 + x2 y0) up to 2^-23 |x y|, six MFMAs of
+//         16 cycles where the fp32 MFMA form of the same tile (eight 16x16x4, 32 cycles each) takes 256.
+struct XB16 { typedef bf16_t mem; static constexpr int PL = 1; };
+struct XF32 { typedef float mem; static constexpr int PL = 3; };
+template <typename E> struct XFrag { bf16x8 p[E::PL]; };
+
+template <typename E, int N> __device__ __forceinline__ void x_mma(const XFrag<E> (&a)[N], const XFrag<E>& b, f32x4* c) {
+    if constexpr (E::PL == 1) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) c[n] = mma16(a[n].p[0], b.p[0], c[n]);
+    } else {
+        constexpr int ia[6] = {2, 1, 0, 1, 0, 0}, ib[6] = {0, 1, 2, 0, 1, 0};        // small terms first
+#pragma unroll
+        for (int t = 0; t < 6; ++t)
+#pragma unroll
+            for (int n = 0; n < N; ++n) c[n] = mma16(a[n].p[ia[t]], b.p[ib[t]], c[n]);
+    }
+}
+
+// the three planes of two values, packed in pairs.  CHECK: an infinity stays one (its rest is not a number otherwise)
+template <bool CHECK> __device__ __forceinline__ void x_split2(float a, float b, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
+    const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
+    w0 = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+    const float a0 = __builtin_bit_cast(float, ua & 0xffff0000u), b0 = __builtin_bit_cast(float, ub & 0xffff0000u);
+    float ra = a - a0, rb = b - b0;
+    if (CHECK) {
+        ra = a == a0 ? 0.f : ra;
+        rb = b == b0 ? 0.f : rb;
+    }
+    const uint32_t va = __builtin_bit_cast(uint32_t, ra), vb = __builtin_bit_cast(uint32_t, rb);
+    w1 = __builtin_amdgcn_perm(vb, va, 0x07060302u);
+    const float sa = ra - __builtin_bit_cast(float, va & 0xffff0000u), sb = rb - __builtin_bit_cast(float, vb & 0xffff0000u);
+    w2 = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, sb), __builtin_bit_cast(uint32_t, sa), 0x07060302u);
+}
+struct XRaw { float v[8]; };          // eight consecutive fp32 values on their way to a fragment
+template <bool CHECK> __device__ __forceinline__ XFrag<XF32> x_split8(const XRaw& x) {
+    uint4 w[3];
+    x_split2<CHECK>(x.v[0], x.v[1], w[0].x, w[1].x, w[2].x);
+    x_split2<CHECK>(x.v[2], x.v[3], w[0].y, w[1].y, w[2].y);
+    x_split2<CHECK>(x.v[4], x.v[5], w[0].z, w[1].z, w[2].z);
+    x_split2<CHECK>(x.v[6], x.v[7], w[0].w, w[1].w, w[2].w);
+    XFrag<XF32> f;
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl) f.p[pl] = __builtin_bit_cast(bf16x8, w[pl]);
+    return f;
+}
+__device__ __forceinline__ XRaw x_raw(const float* p) {
+    XRaw r;
+    *(f32x4*)&r.v[0] = *(const f32x4*)p;
+    *(f32x4*)&r.v[4] = *(const f32x4*)(p + 4);
+    return r;
+}
+// eight consecutive elements of memory as an operand
+template <typename E> __device__ __forceinline__ XFrag<E> x_load(const typename E::mem* p) {
+    if constexpr (E::PL == 1) {
+        XFrag<E> f;
+        f.p[0] = *(const bf16x8*)p;
+        return f;
+    } else {
+        return x_split8<true>(x_raw(p));
+    }
+}
+// accumulator pair -> operand (k-slot (g, jj) <-> row 16 (jj / 4) + 4 g + jj % 4 of the 32)
+template <typename E> __device__ __forceinline__ XFrag<E> x_pack(const f32x4& lo, const f32x4& hi) {
+    if constexpr (E::PL == 1) {
+        XFrag<E> f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            f.p[0][r] = (bf16_t)lo[r];
+            f.p[0][4 + r] = (bf16_t)hi[r];
+        }
+        return f;
+    } else {
+        XRaw x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            x.v[r] = lo[r];
+            x.v[4 + r] = hi[r];
+        }
+        return x_split8<false>(x);
+    }
+}
+
+// ---- tiles of ROWS rows x DK in LDS ---------------------------------------------------------------------------------
+// One plane of bf16 rows (three for XF32), unpadded, their 16-byte slots rotated by ROT * (row >> RSH) so that fragment reads of 16
+// rows and transposed reads of 4 rows x 64 bytes spread over the banks; rows narrower than 256 bytes share a rotation where several
+// of them make up one pass over the banks.
+template <typename E, int DK, int ROWS = 64> struct XTile {
+    typedef typename E::mem T;
+    typedef XFrag<E> frag_t;
+    static constexpr int ROWB = DK * 2;
     static constexpr int NS = ROWB / 16;
-    static constexpr int BYTES = ROWS * ROWB;
-    static constexpr int PIECES = BYTES / 1024;
-    static constexpr int EPS = 16 / (int)sizeof(T);
+    static constexpr int PLANE = ROWS * ROWB;
+    static constexpr int BYTES = E::PL * PLANE;
     static constexpr int KS = DK / 32;
     static constexpr int DT = DK / 16;
     static constexpr int RSH = ROWB == 128 ? 1 : (ROWB == 64 ? 2 : 0);
-    typedef typename Frag<T>::type frag_t;
 
     template <int ROT> static __device__ __forceinline__ int rot(int row) { return (ROT * (row >> RSH)) % NS; }
 
-    // rows [first, first + ROWS) of a plain matrix, clamped to its last row (`len` > 0)
-    template <int ROT, int NW>
-    static __device__ __forceinline__ void stage(const T* __restrict__ base, int ld, int first, int len, unsigned char* dst,
-                                                 int wave, int lane) {
-        static_assert(PIECES % NW == 0, "the same number of pieces for every wave");
-#pragma unroll
-        for (int pp = 0; pp < PIECES / NW; ++pp) {
-            const int p = wave + NW * pp;
-            const int off = p * 1024 + lane * 16, row = off / ROWB, slot = (off % ROWB) >> 4;
-            const int r = min(first + row, len - 1);
-            const int s = (slot + NS - rot<ROT>(row)) % NS;      // physical slot `slot` holds logical slot s
-            __builtin_amdgcn_global_load_lds((x_gbl_void*)(base + (size_t)r * ld + s * EPS), (x_lds_void*)(dst + p * 1024), 16, 0, 0);
-        }
-    }
-    // packed rows [first, first + ROWS) of the g heads that share a key head: `base` at the group's first head
-    template <int ROT, int NW>
-    static __device__ __forceinline__ void stage_rows(const XArgs& a, const T* __restrict__ base, int ld, int first, int nrow,
-                                                      unsigned char* dst, int wave, int lane) {
-        static_assert(PIECES % NW == 0, "the same number of pieces for every wave");
-#pragma unroll
-        for (int pp = 0; pp < PIECES / NW; ++pp) {
-            const int p = wave + NW * pp;
-            const int off = p * 1024 + lane * 16, row = off / ROWB, slot = (off % ROWB) >> 4;
-            const int r = min(first + row, nrow - 1);
-            const int q = x_query(a, r);
-            const int s = (slot + NS - rot<ROT>(row)) % NS;
-            __builtin_amdgcn_global_load_lds((x_gbl_void*)(base + (size_t)q * ld + (r - q * a.g) * DK + s * EPS),
-                                             (x_lds_void*)(dst + p * 1024), 16, 0, 0);
-        }
-    }
     // row `row`, elements 32 ks + 8 g .. + 7
     template <int ROT> static __device__ __forceinline__ frag_t row_frag(const unsigned char* img, int row, int ks, int g) {
-        const unsigned char* rowp = img + row * ROWB;
-        if constexpr (sizeof(T) == 2) {
-            return *(const frag_t*)(rowp + (((ks * 4 + g) + rot<ROT>(row)) % NS) * 16);
-        } else {
-            const f32x4 v0 = *(const f32x4*)(rowp + (((ks * 8 + 2 * g) + rot<ROT>(row)) % NS) * 16);
-            const f32x4 v1 = *(const f32x4*)(rowp + (((ks * 8 + 2 * g + 1) + rot<ROT>(row)) % NS) * 16);
-            return (frag_t){v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-        }
+        frag_t f;
+        const unsigned char* at = img + row * ROWB + (((ks * 4 + g) + rot<ROT>(row)) % NS) * 16;
+#pragma unroll
+        for (int pl = 0; pl < E::PL; ++pl) f.p[pl] = *(const bf16x8*)(at + pl * PLANE);
+        return f;
     }
-    // column 16 dt + i, rows 32 c + {4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3}: the slot map of an accumulator used as operand
+    // column 16 dt + i, rows 32 c + {4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3}: the slot map of an accumulator used as operand.
+    // Transposed 4 x 16 block reads: lane 4 q + p of a 16-lane group supplies row q, columns 4 p .. 4 p + 3
     template <int ROT> static __device__ __forceinline__ frag_t col_frag(const unsigned char* img, int c, int dt, int g, int i) {
         frag_t f;
-        if constexpr (sizeof(T) == 2) {
-            // transposed 4 x 16 block read: lane 4 q + p of a 16-lane group supplies row q, columns 4 p .. 4 p + 3
-            const int row0 = 32 * c + 4 * g + (i >> 2), row1 = row0 + 16;
-            const int slot = dt * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
-            const unsigned char* p0 = img + row0 * ROWB + ((slot + rot<ROT>(row0)) % NS) * 16 + sub;
-            const unsigned char* p1 = img + row1 * ROWB + ((slot + rot<ROT>(row1)) % NS) * 16 + sub;
-            const bf16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)p0);
-            const bf16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)p1);
+        const int row0 = 32 * c + 4 * g + (i >> 2), row1 = row0 + 16;
+        const int slot = dt * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+        const unsigned char* p0 = img + row0 * ROWB + ((slot + rot<ROT>(row0)) % NS) * 16 + sub;
+        const unsigned char* p1 = img + row1 * ROWB + ((slot + rot<ROT>(row1)) % NS) * 16 + sub;
+#pragma unroll
+        for (int pl = 0; pl < E::PL; ++pl) {
+            const bf16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p0 + pl * PLANE));
+            const bf16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p1 + pl * PLANE));
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                f[r] = lo4[r];
-                f[4 + r] = hi4[r];
-            }
-        } else {
-#pragma unroll
-            for (int jj = 0; jj < 8; ++jj) {
-                const int row = 32 * c + 16 * (jj >> 2) + 4 * g + (jj & 3), col = dt * 16 + i;
-                f[jj] = *(const T*)(img + row * ROWB + (((col >> 2) + rot<ROT>(row)) % NS) * 16 + (col & 3) * 4);
+                f.p[pl][r] = lo4[r];
+                f.p[pl][4 + r] = hi4[r];
             }
         }
         return f;
     }
 };
 
-// accumulator pair -> operand fragment (k-slot (g, jj) <-> row 16 (jj / 4) + 4 g + jj % 4 of the 32)
-template <typename T> __device__ __forceinline__ typename Frag<T>::type x_pack(const f32x4& lo, const f32x4& hi) {
-    typename Frag<T>::type f;
+// Keys of a tile: 64 where two tiles of K and V (bf16: double-buffered by LDS-DMA) or one in three planes (fp32: loaded ahead into
+// registers, split on the way into LDS) leave room for two workgroups on a CU, else 32.
+template <typename E, int DK> constexpr int x_kb() { return E::PL == 3 && DK == 128 ? 32 : 64; }
+
+// ---- memory -> tile, by NW waves ---------------------------------------------------------------------------------------
+// fetch() starts the rows [0, left) at `tile` (clamped to the last of them), put() finishes.  Sources are 32-bit byte offsets from the
+// tile's first row, clamped by min() (of offsets in one column: the offset of the smaller row).
+//   XB16: fetch is LDS-DMA (16 bytes a lane, lane-linear on the LDS side: the rotation goes into the source), put nothing; the caller
+//         waits vmcnt(0).  Power-of-two rows: the swizzle repeats every (NS << RSH) / ROT rows, a wave needs one period's offsets.
+//   XF32: fetch loads into registers (32 bytes a lane and 16-byte slot), put splits them and writes the three planes.
+// Packed rows of the g > 1 query heads of a shared head (`rows`): the address is worked out row by row.
+template <typename E, int DK, int ROWS, int ROT, int NW> struct XFetch;
+
+template <int DK, int ROWS, int ROT, int NW> struct XFetch<XB16, DK, ROWS, ROT, NW> {
+    typedef XTile<XB16, DK, ROWS> TL;
+    static constexpr int PIECES = TL::BYTES / 1024, PP = PIECES / NW, NS = TL::NS, ROWB = TL::ROWB;
+    static_assert(PIECES % NW == 0, "the same number of pieces for every wave");
+    static constexpr bool POW2 = (NS & (NS - 1)) == 0;
+    static constexpr int STEP = NW * 1024 / ROWB, PERIOD = (NS << TL::RSH) / ROT;          // rows between a wave's pieces
+    static constexpr int N = !POW2 ? PP : (PERIOD <= STEP ? 1 : (PERIOD / STEP < PP ? PERIOD / STEP : PP));
+    unsigned off[N], col[N];
+    __device__ __forceinline__ XFetch(int ld, int wave, int lane) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        f[r] = from_f32<T>(lo[r]);
-        f[4 + r] = from_f32<T>(hi[r]);
+        for (int n = 0; n < N; ++n) {
+            const int o = (wave + NW * n) * 1024 + lane * 16, row = o / ROWB, slot = (o % ROWB) >> 4;
+            col[n] = (unsigned)((slot + NS - TL::template rot<ROT>(row)) % NS) * 16u;       // physical slot `slot` holds this one
+            off[n] = (unsigned)row * (unsigned)ld * 2u + col[n];
+        }
     }
-    return f;
-}
+    __device__ __forceinline__ void fetch(const bf16_t* __restrict__ tile, int ld, int left, unsigned char* dst, int wave, int) {
+        const unsigned ldb = (unsigned)ld * 2u, last = (unsigned)(min(left, ROWS) - 1) * ldb;
+#pragma unroll
+        for (int pp = 0; pp < PP; ++pp) {
+            const unsigned so = min(off[pp % N] + (unsigned)(pp / N * N * STEP) * ldb, last + col[pp % N]);
+            __builtin_amdgcn_global_load_lds((x_gbl_void*)((const unsigned char*)tile + so), (x_lds_void*)(dst + (wave + NW * pp) * 1024),
+                                             16, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void fetch_rows(const XArgs& a, const bf16_t* __restrict__ base, int ld, int first, int nrow,
+                                               unsigned char* dst, int wave, int lane) {
+#pragma unroll 1
+        for (int pp = 0; pp < PP; ++pp) {
+            const int p = wave + NW * pp, o = p * 1024 + lane * 16, row = o / ROWB, slot = (o % ROWB) >> 4;
+            const int r = min(first + row, nrow - 1), q = x_query(a, r);
+            const int s = (slot + NS - TL::template rot<ROT>(row)) % NS;
+            __builtin_amdgcn_global_load_lds((x_gbl_void*)(base + (size_t)q * ld + (r - q * a.g) * DK + s * 8), (x_lds_void*)(dst + p * 1024),
+                                             16, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void put(unsigned char*, int, int) {}
+};
+
+template <int DK, int ROWS, int ROT, int NW> struct XFetch<XF32, DK, ROWS, ROT, NW> {
+    typedef XTile<XF32, DK, ROWS> TL;
+    static constexpr int SPR = DK / 8, SLOTS = ROWS * SPR;                 // 8-element slots of a row, of the tile
+    static constexpr int N = (SLOTS + 64 * NW - 1) / (64 * NW);                // of a lane (the last of them may be missing)
+    static __device__ __forceinline__ bool has(int id) { return SLOTS % (64 * NW) == 0 || id < SLOTS; }
+    XRaw r[N];
+    __device__ __forceinline__ XFetch(int, int, int) {}
+    __device__ __forceinline__ void fetch(const float* __restrict__ tile, int ld, int left, unsigned char*, int wave, int lane) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int id = n * 64 * NW + wave * 64 + lane, row = id / SPR, s = id - row * SPR;
+            if (has(id)) r[n] = x_raw((const float*)((const unsigned char*)tile + (unsigned)min(row, left - 1) * (unsigned)ld * 4u + (unsigned)s * 32u));
+        }
+    }
+    __device__ __forceinline__ void fetch_rows(const XArgs& a, const float* __restrict__ base, int ld, int first, int nrow, unsigned char*,
+                                               int wave, int lane) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int id = n * 64 * NW + wave * 64 + lane, row = id / SPR, s = id - row * SPR;
+            const int rr = min(first + row, nrow - 1), q = x_query(a, rr);
+            if (has(id)) r[n] = x_raw(base + (size_t)q * ld + (rr - q * a.g) * DK + s * 8);
+        }
+    }
+    __device__ __forceinline__ void put(unsigned char* dst, int wave, int lane) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int id = n * 64 * NW + wave * 64 + lane, row = id / SPR, s = id - row * SPR;
+            if (!has(id)) continue;
+            const XFrag<XF32> f = x_split8<true>(r[n]);
+            unsigned char* at = dst + row * TL::ROWB + ((s + TL::template rot<ROT>(row)) % TL::NS) * 16;
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl) *(bf16x8*)(at + pl * TL::PLANE) = f.p[pl];
+        }
+    }
+};
 
 }  // namespace fs2
 
@@ -156,13 +302,22 @@ static inline int fs2_x_check(const char* who, const void* q, const void* k, con
                   max_q, Mq, max_k, Mk);
     FS2_CHECK_ARG((long long)max_q * (H / KV) <= (1 << 24), "%s: max_q=%d with %d heads to a key head", who, max_q, H / KV);
     const long long longest = (long long)max_q * (H / KV) > max_k ? (long long)max_q * (H / KV) : max_k;
-    FS2_CHECK_ARG((long long)B * H * ((longest + 63) / 64) < (1ll << 30), "%s: B=%d x %d heads x %lld rows in one launch", who, B, H,
-                  longest);
+    FS2_CHECK_ARG((long long)B * H <= (1 << 19) && (long long)B * H * ((longest + 31) / 32) < (1ll << 30),
+                  "%s: B=%d x %d heads x %lld rows in one launch", who, B, H, longest);
     const int epv = dtype == 0 ? 4 : 8;
+    FS2_CHECK_ARG(ldq <= (1 << 20) && ldk <= (1 << 20), "%s: leading dims ldq=%d, ldk=%d beyond 2^20", who, ldq, ldk);
     FS2_CHECK_ARG(ldq >= H * dk && ldk >= KV * dk && ldq % epv == 0 && ldk % epv == 0, "%s: bad leading dims ldq=%d ldk=%d", who, ldq,
                   ldk);
     FS2_CHECK_ARG(((uintptr_t)q & 15) == 0 && ((uintptr_t)k & 15) == 0, "%s: unaligned q or k", who);
     return FS2_OK;
+}
+
+// grid of x_decode
+static inline dim3 fs2_x_grid(fs2::XArgs& a, int nblk, int heads, int B) {
+    a.nblk = nblk;
+    a.pairs = B * heads;
+    a.kv_magic = heads > 1 ? (unsigned)((1ull << 32) / heads + 1) : 0u;
+    return a.pairs >= 8 ? dim3(8 * nblk, (a.pairs + 7) / 8, a.nsplit) : dim3(nblk, a.pairs, a.nsplit);
 }
 
 static inline fs2::XArgs fs2_x_args(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, int Mq, int Mk, int H,

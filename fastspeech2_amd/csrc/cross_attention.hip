@@ -25,17 +25,17 @@ __device__ __forceinline__ void x_zero_rows(const XArgs& a, int q0, int kvh, int
     }
 }
 
-template <typename T, int DK, int QT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel(XArgs a) {
-    typedef XTile<T, DK> TL;
+template <typename E, int DK, int QT, bool DROP>
+__global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
+    typedef typename E::mem T;
+    constexpr int KB = x_kb<E, DK>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
+    typedef XTile<E, DK, KB> TL;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT, BQ = 64 * QT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile, V tile at s * 2 * BYTES
 
-    int b, kvh, blk;
-    if (!fs2_pair_order_decode(a.order, b, kvh, blk)) return;
-    const int split = blk % a.nsplit;
-    blk /= a.nsplit;
+    int b, kvh, blk, split;
+    if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, q0, lenq);
     x_range(a.cu_k, b, a.Mk, k0, lenk);
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, i = lane & 15;
-    const int ntiles = (lenk + 63) / 64, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int ntiles = (lenk + KB - 1) / KB, per = a.nsplit == 1 ? ntiles : (ntiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * per, t1 = min(t0 + per, ntiles);
     if (lenk == 0 && a.nsplit == 1) {
         x_zero_rows<T, DK>(a, q0, kvh, blk * BQ, min(nrow, blk * BQ + BQ));
@@ -53,14 +53,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel
     }
     int qrow[QT], head[QT];
     bool live[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
+    auto place = [&](int t) __attribute__((always_inline)) {
         const int r = blk * BQ + (wave * QT + t) * 16 + i;
         live[t] = r < nrow;
         const int rc = min(r, nrow - 1), q = x_query(a, rc);
         qrow[t] = q0 + q;
         head[t] = kvh * a.g + rc - q * a.g;
-    }
+    };
+#pragma unroll
+    for (int t = 0; t < QT; ++t) place(t);
     if (t0 >= t1) {         // this split has no keys: (max, sum) = (-inf, 0)
 #pragma unroll
         for (int t = 0; t < QT; ++t)
@@ -73,19 +74,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel
     }
     const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
     const T* __restrict__ vb = (const T*)a.v + (size_t)k0 * a.ldv + kvh * DK;
-    auto stage = [&](int kt, int st) __attribute__((always_inline)) {
+    XFetch<E, DK, KB, 1, 4> fk(a.ldk, wave, lane);
+    XFetch<E, DK, KB, 2, 4> fv(a.ldv, wave, lane);
+    auto fetch = [&](int kt, int st) __attribute__((always_inline)) {
         unsigned char* d = smem + st * 2 * TL::BYTES;
-        TL::template stage<1, 4>(kb, a.ldk, kt * 64, lenk, d, wave, lane);
-        TL::template stage<2, 4>(vb, a.ldv, kt * 64, lenk, d + TL::BYTES, wave, lane);
+        fk.fetch(kb + (size_t)kt * KB * a.ldk, a.ldk, lenk - kt * KB, d, wave, lane);
+        fv.fetch(vb + (size_t)kt * KB * a.ldv, a.ldv, lenk - kt * KB, d + TL::BYTES, wave, lane);
     };
-    stage(t0, 0);
+    fetch(t0, 0);
 
     frag_t qf[QT][KS];
 #pragma unroll
     for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-            qf[t][ks] = *(const frag_t*)((const T*)a.q + (size_t)qrow[t] * a.ldq + head[t] * DK + ks * 32 + g * 8);
+            qf[t][ks] = x_load<E>((const T*)a.q + (size_t)qrow[t] * a.ldq + head[t] * DK + ks * 32 + g * 8);
 
     f32x4 o[QT][DT];
     float m_run[QT], l_part[QT];
@@ -97,31 +100,47 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel
         for (int dt = 0; dt < DT; ++dt) o[t][dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     for (int kt = t0; kt < t1; ++kt) {
-        vm_wait_barrier<0>();         // tile kt has landed; every wave is done with the other stage
-        const int st = (kt - t0) & 1;
-        if (kt + 1 < t1) stage(kt + 1, st ^ 1);
-        const unsigned char* Ks = smem + st * 2 * TL::BYTES;
-        const unsigned char* Vs = Ks + TL::BYTES;
+        const int st = NST == 2 ? (kt - t0) & 1 : 0;
+        unsigned char* Ks = smem + st * 2 * TL::BYTES;
+        unsigned char* Vs = Ks + TL::BYTES;
+        if constexpr (E::PL == 1) {
+            vm_wait_barrier<0>();         // tile kt has landed; every wave is done with the other stage
+        } else {
+            if (kt > t0) __syncthreads();                // every wave is done with the tile before
+            fk.put(Ks, wave, lane);
+            fv.put(Vs, wave, lane);
+            __syncthreads();
+            if (kt + 1 < t1) fetch(kt + 1, 0);
+        }
 
-        f32x4 s[QT][4];
+        f32x4 s[QT][NT];
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) s[t][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int nt = 0; nt < NT; ++nt) s[t][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            frag_t kf[4];
+            frag_t kf[NT];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) kf[nt] = TL::template row_frag<1>(Ks, nt * 16 + i, ks, g);
+            for (int nt = 0; nt < NT; ++nt) kf[nt] = TL::template row_frag<1>(Ks, nt * 16 + i, ks, g);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) mma16_multi<4>(kf, qf[t][ks], s[t]);
+            for (int t = 0; t < QT; ++t) x_mma<E, NT>(kf, qf[t][ks], s[t]);
         }
-        const int kbase = kt * 64 + 4 * g;
-        if (kt * 64 + 64 > lenk) {
+        // bf16: the V^T fragments of the first 32 keys are requested now and land under the softmax, those of the second 32 land
+        // under the first ones' products.  The next tile's DMA is issued behind all of them: the compiler lets no transposed LDS read
+        // pass an LDS-DMA in flight (it waits vmcnt(0)), so in front of them it would be waited for here.
+        frag_t vf[E::PL == 1 ? NC : 1][DT];
+        if constexpr (E::PL == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) vf[0][dt] = TL::template col_frag<2>(Vs, 0, dt, g, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int kbase = kt * KB + 4 * g;
+        if (kt * KB + KB > lenk) {
 #pragma unroll
             for (int t = 0; t < QT; ++t)
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (kbase + nt * 16 + r >= lenk) s[t][nt][r] = -INFINITY;
@@ -130,57 +149,77 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel
         for (int t = 0; t < QT; ++t) {
             float m_loc = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) m_loc = fmaxf(m_loc, s[t][nt][r]);
             m_loc = rows_max(m_loc) * a.scale_log2e;
-            const float m_new = fmaxf(m_run[t], m_loc);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;        // a tile of -inf scores leaves no NaN behind
-            const float alpha = __builtin_amdgcn_exp2f(m_run[t] - m_use);
-            m_run[t] = m_new;
+            // the reference point moves only when a score is more than 2^8 above it (weights then stay below 2^8, which costs fp32
+            // sums and bf16 weights nothing): a row's later tiles hardly ever rescale
+            const bool moves = m_loc > m_run[t] + 8.0f;
+            float m_use = moves ? m_loc : m_run[t];
+            if (kt > t0 && !__all(!moves)) {
+                const float alpha = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[t] - m_use);
+                l_part[t] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[t][dt][r] *= alpha;
+            }
+            m_run[t] = m_use;
+            m_use = m_use == -INFINITY ? 0.f : m_use;                    // nothing but -inf scores so far: no NaN
             float psum = 0.f;
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(s[t][nt][r], a.scale_log2e, -m_use));
                     s[t][nt][r] = p;
                     psum += p;
                 }
-            l_part[t] = fmaf(l_part[t], alpha, psum);
-            if (!__all(alpha == 1.0f)) {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[t][dt][r] *= alpha;
-            }
-            if (a.drop.thresh) {      // the sum above is over the undropped probabilities
+            l_part[t] += psum;
+            if constexpr (DROP) {      // the sum above is over the undropped probabilities
                 Dropout dh = a.drop;
                 dh.stream += (uint32_t)head[t];
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[t][nt][r] *= drop_mul(dh, (uint32_t)qrow[t], (uint32_t)(kbase + nt * 16 + r));
             }
         }
+        if constexpr (E::PL == 1) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+            for (int c = 1; c < NC; ++c)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) vf[c][dt] = TL::template col_frag<2>(Vs, c, dt, g, i);
+            if (kt + 1 < t1) fetch(kt + 1, st ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
             frag_t pf[QT];
 #pragma unroll
-            for (int t = 0; t < QT; ++t) pf[t] = x_pack<T>(s[t][2 * c], s[t][2 * c + 1]);
+            for (int t = 0; t < QT; ++t) pf[t] = x_pack<E>(s[t][2 * c], s[t][2 * c + 1]);
+            if constexpr (E::PL == 1) {
 #pragma unroll
-            for (int dt0 = 0; dt0 < DT; dt0 += 2) {
-                frag_t vf[2];
+                for (int t = 0; t < QT; ++t) x_mma<E, DT>(vf[c], pf[t], o[t]);
+            } else {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) vf[u] = TL::template col_frag<2>(Vs, c, dt0 + u, g, i);
+                for (int dt0 = 0; dt0 < DT; dt0 += 2) {
+                    frag_t v2[2];
 #pragma unroll
-                for (int t = 0; t < QT; ++t) mma16_multi<2>(vf, pf[t], &o[t][dt0]);
+                    for (int u = 0; u < 2; ++u) v2[u] = TL::template col_frag<2>(Vs, c, dt0 + u, g, i);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) x_mma<E, 2>(v2, pf[t], &o[t][dt0]);
+                }
             }
         }
     }
+    if constexpr (!DROP) asm volatile("" : "+s"(blk));       // the rows' places are worked out again, not carried through the loop
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const float l = rows_sum(l_part[t]);
+        place(t);
         if (!live[t]) continue;
         if (a.nsplit == 1) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;        // no score above -inf: a zero row
@@ -203,9 +242,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_rows_kernel
 }
 
 // At most 16 packed rows per (utterance, shared head).  grid (nsplit, KV, B); wave w takes the 32-key tiles t0 + w, + 4, ..
-template <typename T, int DK>
+template <typename E, int DK>
 __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
-    typedef XTile<T, DK, 32> TL;
+    typedef typename E::mem T;
+    typedef XTile<E, DK, 32> TL;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // wave w: V tile at w * BYTES; then the merge
@@ -223,30 +263,36 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
         return;
     }
     const int rc = min(i, nrow - 1), q = x_query(a, rc), head = kvh * a.g + rc - q * a.g, qrow = q0 + q;
-    const int ntiles = (lenk + 31) / 32, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int ntiles = (lenk + 31) / 32, per = a.nsplit == 1 ? ntiles : (ntiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * per, t1 = min(t0 + per, ntiles);
     frag_t qf[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const frag_t*)((const T*)a.q + (size_t)qrow * a.ldq + head * DK + ks * 32 + g * 8);
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = x_load<E>((const T*)a.q + (size_t)qrow * a.ldq + head * DK + ks * 32 + g * 8);
 
     const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
     const T* __restrict__ vb = (const T*)a.v + (size_t)k0 * a.ldv + kvh * DK;
     unsigned char* Vs = smem + wave * TL::BYTES;
+    XFetch<E, DK, 32, 2, 1> fv(a.ldv, 0, lane);
     f32x4 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_part = 0.f;
     for (int kt = t0 + wave; kt < t1; kt += 4) {
-        frag_t kf[KS][2];
+        fv.fetch(vb + (size_t)kt * 32 * a.ldv, a.ldv, lenk - kt * 32, Vs, 0, lane);
+        f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        frag_t kf[E::PL == 1 ? KS : 1][2];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks) {
+            frag_t (&f)[2] = kf[E::PL == 1 ? ks : 0];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
-                kf[ks][nt] = *(const frag_t*)(kb + (size_t)min(kt * 32 + nt * 16 + i, lenk - 1) * a.ldk + ks * 32 + g * 8);
-        TL::template stage<2, 1>(vb, a.ldv, kt * 32, lenk, Vs, 0, lane);
-        f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                f[nt] = x_load<E>(kb + (size_t)min(kt * 32 + nt * 16 + i, lenk - 1) * a.ldk + ks * 32 + g * 8);
+            if constexpr (E::PL == 3) x_mma<E, 2>(f, qf[ks], s);
+        }
+        if constexpr (E::PL == 1) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) mma16_multi<2>(kf[ks], qf[ks], s);
+            for (int ks = 0; ks < KS; ++ks) x_mma<E, 2>(kf[ks], qf[ks], s);
+        }
         const int kbase = kt * 32 + 4 * g;
         float m_loc = -INFINITY;
 #pragma unroll
@@ -277,14 +323,20 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[nt][r] *= drop_mul(dh, (uint32_t)qrow, (uint32_t)(kbase + nt * 16 + r));
         }
-        const frag_t pf = x_pack<T>(s[0], s[1]);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's V tile has landed (no other wave reads it)
+        const frag_t pf = x_pack<E>(s[0], s[1]);
+        fv.put(Vs, 0, lane);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // this wave's V tile has landed (no other wave reads it)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const frag_t vf = TL::template col_frag<2>(Vs, 0, dt, g, i);
-            o[dt] = mma16(vf, pf, o[dt] * alpha);
+        for (int dt0 = 0; dt0 < DT; dt0 += 2) {
+            frag_t v2[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                v2[u] = TL::template col_frag<2>(Vs, 0, dt0 + u, g, i);
+                o[dt0 + u] = o[dt0 + u] * alpha;
+            }
+            x_mma<E, 2>(v2, pf, &o[dt0]);
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next tile's DMA overwrites it
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next tile overwrites it
     }
     // merge of the four waves: lane (g, i) of wave w holds row i, columns 16 dt + 4 g ..
     const float l = rows_sum(l_part);
@@ -385,27 +437,33 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dk, int dtyp
     return p;
 }
 
-template <typename T, int DK>
+template <typename E, int DK, int QT, bool DROP> static void launch_xattn_rows(const XArgs& a, dim3 grid, hipStream_t stream) {
+    constexpr int lds = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_kb<E, DK>()>::BYTES;
+    static unsigned long long ok = 0;
+    fs2_allow_lds((const void*)xattn_rows_kernel<E, DK, QT, DROP>, lds, &ok);
+    hipLaunchKernelGGL((xattn_rows_kernel<E, DK, QT, DROP>), grid, dim3(256), lds, stream, a);
+}
+
+template <typename E, int DK>
 static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipStream_t stream) {
+    typedef typename E::mem T;
     if (p.few) {
-        constexpr int merge = 4 * 16 * DK * 4 + 512, tiles = 4 * XTile<T, DK, 32>::BYTES;
+        constexpr int merge = 4 * 16 * DK * 4 + 512, tiles = 4 * XTile<E, DK, 32>::BYTES;
         constexpr int lds = merge > tiles ? merge : tiles;
         static unsigned long long ok = 0;
-        fs2_allow_lds((const void*)xattn_few_kernel<T, DK>, lds, &ok);
-        hipLaunchKernelGGL((xattn_few_kernel<T, DK>), dim3(a.nsplit, a.KV, B), dim3(256), lds, stream, a);
+        fs2_allow_lds((const void*)xattn_few_kernel<E, DK>, lds, &ok);
+        hipLaunchKernelGGL((xattn_few_kernel<E, DK>), dim3(a.nsplit, a.KV, B), dim3(256), lds, stream, a);
     } else {
-        constexpr int lds = 4 * XTile<T, DK>::BYTES;
-        static unsigned long long ok[2] = {0, 0};
         const int rows = max_q * a.g, nblk = (rows + 64 * p.qt - 1) / (64 * p.qt);
-        const dim3 grid = fs2_pair_order_grid(a.order, nblk * a.nsplit, a.KV, B, true);
+        const dim3 grid = fs2_x_grid(a, nblk, a.KV, B);
         if (p.qt == 2) {
-            if constexpr (sizeof(T) == 2) {
-                fs2_allow_lds((const void*)xattn_rows_kernel<T, DK, 2>, lds, &ok[1]);
-                hipLaunchKernelGGL((xattn_rows_kernel<T, DK, 2>), grid, dim3(256), lds, stream, a);
+            if constexpr (E::PL == 1) {
+                if (a.drop.thresh) launch_xattn_rows<E, DK, 2, true>(a, grid, stream);
+                else launch_xattn_rows<E, DK, 2, false>(a, grid, stream);
             }
         } else {
-            fs2_allow_lds((const void*)xattn_rows_kernel<T, DK, 1>, lds, &ok[0]);
-            hipLaunchKernelGGL((xattn_rows_kernel<T, DK, 1>), grid, dim3(256), lds, stream, a);
+            if (a.drop.thresh) launch_xattn_rows<E, DK, 1, true>(a, grid, stream);
+            else launch_xattn_rows<E, DK, 1, false>(a, grid, stream);
         }
     }
     FS2_CHECK_LAUNCH("fs2_cross_attention");
@@ -439,7 +497,7 @@ extern "C" int fs2_cross_attention(const void* q, const void* k, const void* v, 
     FS2_CHECK_ARG(rate >= 0.f && rate < 1.f, "fs2_cross_attention: dropout rate must be in [0, 1)");
     FS2_CHECK_ARG((v || Mk == 0) && (ctx || Mq == 0) && ((uintptr_t)v & 15) == 0 && ((uintptr_t)ctx & 15) == 0,
                   "fs2_cross_attention: null or unaligned v or ctx");
-    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldo >= n_heads * dk && ldv % epv == 0 && ldo % epv == 0,
+    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldv <= (1 << 20) && ldo >= n_heads * dk && ldv % epv == 0 && ldo % epv == 0,
                   "fs2_cross_attention: bad leading dims ldv=%d ldo=%d", ldv, ldo);
     if (max_q == 0) return FS2_OK;
     XArgs a = fs2_x_args(q, k, v, cu_q, cu_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, ldv, ldo);
@@ -453,14 +511,14 @@ extern "C" int fs2_cross_attention(const void* q, const void* k, const void* v, 
                   "fs2_cross_attention: this shape needs fs2_cross_attention_workspace bytes, 16-byte aligned");
 #define FS2_X(TT, DKK) return launch_xattn<TT, DKK>(a, p, B, max_q, dk, stream)
     if (dtype == 0) {
-        if (dk == 32) FS2_X(float, 32);
-        if (dk == 64) FS2_X(float, 64);
-        if (dk == 96) FS2_X(float, 96);
-        FS2_X(float, 128);
+        if (dk == 32) FS2_X(XF32, 32);
+        if (dk == 64) FS2_X(XF32, 64);
+        if (dk == 96) FS2_X(XF32, 96);
+        FS2_X(XF32, 128);
     }
-    if (dk == 32) FS2_X(bf16_t, 32);
-    if (dk == 64) FS2_X(bf16_t, 64);
-    if (dk == 96) FS2_X(bf16_t, 96);
-    FS2_X(bf16_t, 128);
+    if (dk == 32) FS2_X(XB16, 32);
+    if (dk == 64) FS2_X(XB16, 64);
+    if (dk == 96) FS2_X(XB16, 96);
+    FS2_X(XB16, 128);
 #undef FS2_X
 }

@@ -4,24 +4,30 @@
 //   delta = sum_dv dO o O
 //   dP = dO v^T o D,  dS = P o (dP - delta)
 //   dq = dS k / sqrt(dk)                                          xattn_dq_kernel: one wave per 16 packed rows
-//   dk = dS^T q / sqrt(dk),  dv = (P o D)^T dO                    xattn_dkv_kernel: one wave per 16 keys, over ALL packed rows
+//   dk = dS^T q / sqrt(dk),  dv = (P o D)^T dO                    xattn_dkv32_kernel (bf16), xattn_dkv_kernel (fp32)
 //   mass[h][key] = sum_q P                                        xattn_mass_kernel
 // The packed rows of a shared head are its g query heads, so the sum over the group that dk and dv need is part of the loop.
 // Every output element has one writer and every sum a fixed order: no atomics, the same bits every time.
 #include "cross_attention.h"
+#include <type_traits>
 
 namespace fs2 {
 
 // ---- dq and delta: one workgroup per (utterance, shared head, 64 packed rows) -------------------------------------
-template <typename T, int DK>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_dq_kernel(XArgs a) {
-    typedef XTile<T, DK> TL;
+// (64-key tiles of dk = 96 in three planes need 37 registers more than there are)
+template <typename E, int DK> constexpr int x_dq_kb() { return E::PL == 3 && DK >= 96 ? 32 : 64; }
+
+template <typename E, int DK, bool DROP>
+__global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
+    typedef typename E::mem T;
+    constexpr int KB = x_dq_kb<E, DK>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
+    typedef XTile<E, DK, KB> TL;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile (rotation 2), V tile (rotation 1)
 
-    int b, kvh, blk;
-    if (!fs2_pair_order_decode(a.order, b, kvh, blk)) return;
+    int b, kvh, blk, split;
+    if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, q0, lenq);
     x_range(a.cu_k, b, a.Mk, k0, lenk);
@@ -36,23 +42,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_dq_kernel(X
 
     const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
     const T* __restrict__ vb = (const T*)a.v + (size_t)k0 * a.ldv + kvh * DK;
-    auto stage = [&](int kt, int st) __attribute__((always_inline)) {
+    XFetch<E, DK, KB, 2, 4> fk(a.ldk, wave, lane);
+    XFetch<E, DK, KB, 1, 4> fv(a.ldv, wave, lane);
+    auto fetch = [&](int kt, int st) __attribute__((always_inline)) {
         unsigned char* d = smem + st * 2 * TL::BYTES;
-        TL::template stage<2, 4>(kb, a.ldk, kt * 64, lenk, d, wave, lane);
-        TL::template stage<1, 4>(vb, a.ldv, kt * 64, lenk, d + TL::BYTES, wave, lane);
+        fk.fetch(kb + (size_t)kt * KB * a.ldk, a.ldk, lenk - kt * KB, d, wave, lane);
+        fv.fetch(vb + (size_t)kt * KB * a.ldv, a.ldv, lenk - kt * KB, d + TL::BYTES, wave, lane);
     };
-    if (lenk > 0) stage(0, 0);
+    if (lenk > 0) fetch(0, 0);
 
     frag_t qf[KS], dof[KS];
     float del = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         const int c = head * DK + ks * 32 + g * 8;
-        qf[ks] = *(const frag_t*)((const T*)a.q + (size_t)qrow * a.ldq + c);
-        dof[ks] = *(const frag_t*)((const T*)a.dctx + (size_t)qrow * a.ldo + c);
-        const frag_t of = *(const frag_t*)((const T*)a.ctx + (size_t)qrow * a.ldo + c);
+        const T* od = (const T*)a.dctx + (size_t)qrow * a.ldo + c;
+        const T* oc = (const T*)a.ctx + (size_t)qrow * a.ldo + c;
+        qf[ks] = x_load<E>((const T*)a.q + (size_t)qrow * a.ldq + c);
+        dof[ks] = x_load<E>(od);
+        if constexpr (E::PL == 1) {
+            const bf16x8 of = *(const bf16x8*)oc;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) del = fmaf(to_f32(dof[ks][j]), to_f32(of[j]), del);
+            for (int j = 0; j < 8; ++j) del = fmaf(to_f32(dof[ks].p[0][j]), to_f32(of[j]), del);
+        } else {
+            const XRaw u = x_raw(od), v = x_raw(oc);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) del = fmaf(u.v[j], v.v[j], del);
+        }
     }
     del = rows_sum(del);
     if (g == 0 && r < nrow) a.delta[(size_t)head * a.Mq + qrow] = del;
@@ -63,40 +79,74 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_dq_kernel(X
     for (int dt = 0; dt < DT; ++dt) dq[dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     Dropout dh = a.drop;
     dh.stream += (uint32_t)head;
-    const int ntiles = (lenk + 63) / 64;
+    const int ntiles = (lenk + KB - 1) / KB;
     for (int kt = 0; kt < ntiles; ++kt) {
-        vm_wait_barrier<0>();      // tile kt has landed; every wave is done with the other stage
-        if (kt + 1 < ntiles) stage(kt + 1, (kt + 1) & 1);
-        const unsigned char* Ks = smem + (kt & 1) * 2 * TL::BYTES;
-        const unsigned char* Vs = Ks + TL::BYTES;
-        f32x4 s[4], dp[4];
+        const int st = NST == 2 ? kt & 1 : 0;
+        unsigned char* Ks = smem + st * 2 * TL::BYTES;
+        unsigned char* Vs = Ks + TL::BYTES;
+        if constexpr (E::PL == 1) {
+            vm_wait_barrier<0>();      // tile kt has landed; every wave is done with the other stage
+        } else {
+            if (kt > 0) __syncthreads();
+            fk.put(Ks, wave, lane);
+            fv.put(Vs, wave, lane);
+            __syncthreads();
+            if (kt + 1 < ntiles) fetch(kt + 1, 0);
+        }
+        f32x4 s[NT], dp[NT];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) s[nt] = dp[nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int nt = 0; nt < NT; ++nt) s[nt] = dp[nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            frag_t kf[4];
+            frag_t kf[NT];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) kf[nt] = TL::template row_frag<2>(Ks, nt * 16 + i, ks, g);
-            mma16_multi<4>(kf, qf[ks], s);
+            for (int nt = 0; nt < NT; ++nt) kf[nt] = TL::template row_frag<2>(Ks, nt * 16 + i, ks, g);
+            x_mma<E, NT>(kf, qf[ks], s);
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) kf[nt] = TL::template row_frag<1>(Vs, nt * 16 + i, ks, g);
-            mma16_multi<4>(kf, dof[ks], dp);
+            for (int nt = 0; nt < NT; ++nt) kf[nt] = TL::template row_frag<1>(Vs, nt * 16 + i, ks, g);
+            x_mma<E, NT>(kf, dof[ks], dp);
+        }
+        // bf16: K^T fragments before the next tile's DMA (no transposed LDS read passes one), under the arithmetic
+        frag_t kc[E::PL == 1 ? NC : 1][DT];
+        if constexpr (E::PL == 1) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) kc[c][dt] = TL::template col_frag<2>(Ks, c, dt, g, i);
+            __builtin_amdgcn_sched_barrier(0);
+            if (kt + 1 < ntiles) fetch(kt + 1, st ^ 1);
         }
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int key = kt * 64 + nt * 16 + 4 * g + e;
-                const float p = key < lenk ? __builtin_amdgcn_exp2f(fmaf(s[nt][e], a.scale_log2e, -lse_q)) : 0.f;
+                const int key = kt * KB + nt * 16 + 4 * g + e;
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[nt][e], a.scale_log2e, -lse_q));
                 float dpv = dp[nt][e];
-                if (a.drop.thresh) dpv *= drop_mul(dh, (uint32_t)qrow, (uint32_t)key);
-                s[nt][e] = key < lenk ? p * (dpv - del) : 0.f;
+                if constexpr (DROP) dpv *= drop_mul(dh, (uint32_t)qrow, (uint32_t)key);
+                s[nt][e] = p * (dpv - del);
             }
+        if (kt * KB + KB > lenk) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const frag_t dsf = x_pack<T>(s[2 * c], s[2 * c + 1]);
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) dq[dt] = mma16(TL::template col_frag<2>(Ks, c, dt, g, i), dsf, dq[dt]);
+                for (int e = 0; e < 4; ++e)
+                    if (kt * KB + nt * 16 + 4 * g + e >= lenk) s[nt][e] = 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const frag_t dsf = x_pack<E>(s[2 * c], s[2 * c + 1]);
+            if constexpr (E::PL == 1) {
+                x_mma<E, DT>(kc[c], dsf, dq);
+            } else {
+#pragma unroll
+                for (int dt0 = 0; dt0 < DT; dt0 += 2) {
+                    frag_t k2[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) k2[u] = TL::template col_frag<2>(Ks, c, dt0 + u, g, i);
+                    x_mma<E, 2>(k2, dsf, &dq[dt0]);
+                }
+            }
         }
     }
     if (r < nrow) {
@@ -106,20 +156,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_dq_kernel(X
     }
 }
 
-// ---- dk, dv: one workgroup per (utterance, shared head, 64 keys, range of packed rows) ----------------------------
-template <typename T, int DK>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_dkv_kernel(XArgs a) {
-    typedef XTile<T, DK> TL;
+// ---- dk, dv -----------------------------------------------------------------------------------------------------------
+// fp32: one workgroup per (utterance, shared head, 64 keys, range of packed rows), a wave to 16 keys, its K and V operands in
+// registers; row tiles of 32 in LDS for all four.
+template <int DK, bool DROP>
+__global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs a) {
+    typedef XF32 E;
+    typedef float T;
+    typedef XTile<E, DK, 32> TL;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT;
-    // stage s: Q tile, dO tile (rotation 2: read both ways), then the 64 lse and 64 delta values of those rows
-    constexpr int STAGE = 2 * TL::BYTES + 512;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // Q tile, dO tile (rotation 2), 32 lse, 32 delta
 
-    int b, kvh, blk;
-    if (!fs2_pair_order_decode(a.order, b, kvh, blk)) return;
-    const int split = blk % a.nsplit;
-    blk /= a.nsplit;
+    int b, kvh, blk, split;
+    if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, q0, lenq);
     x_range(a.cu_k, b, a.Mk, k0, lenk);
@@ -129,80 +179,80 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_dkv_kernel(
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int key = blk * 64 + wave * 16 + i, kc = min(key, lenk - 1);
-    const int ntiles = (nrow + 63) / 64, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int ntiles = (nrow + 31) / 32, per = a.nsplit == 1 ? ntiles : (ntiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * per, t1 = min(t0 + per, ntiles);
+    unsigned char *Qs = smem, *Ds = smem + TL::BYTES;
+    float* rows_s = (float*)(smem + 2 * TL::BYTES);
 
     const T* __restrict__ qb = (const T*)a.q + (size_t)q0 * a.ldq + kvh * a.g * DK;
     const T* __restrict__ db = (const T*)a.dctx + (size_t)q0 * a.ldo + kvh * a.g * DK;
-    auto stage = [&](int qt, int st) __attribute__((always_inline)) {
-        unsigned char* d = smem + st * STAGE;
-        TL::template stage_rows<2, 4>(a, qb, a.ldq, qt * 64, nrow, d, wave, lane);
-        TL::template stage_rows<2, 4>(a, db, a.ldo, qt * 64, nrow, d + TL::BYTES, wave, lane);
-        if (wave < 2) {
-            const int r = min(qt * 64 + lane, nrow - 1), q = x_query(a, r);
-            const size_t at = (size_t)(kvh * a.g + r - q * a.g) * a.Mq + q0 + q;
-            __builtin_amdgcn_global_load_lds((x_gbl_void*)((wave ? a.delta : a.lse) + at),
-                                             (x_lds_void*)(d + 2 * TL::BYTES + wave * 256), 4, 0, 0);
+    XFetch<E, DK, 32, 2, 4> fq(a.ldq, wave, lane), fd(a.ldo, wave, lane);
+    float stat = 0.f;
+    auto fetch = [&](int qt) __attribute__((always_inline)) {
+        fq.fetch_rows(a, qb, a.ldq, qt * 32, nrow, Qs, wave, lane);
+        fd.fetch_rows(a, db, a.ldo, qt * 32, nrow, Ds, wave, lane);
+        if (tid < 64) {
+            const int r = min(qt * 32 + (tid & 31), nrow - 1), q = x_query(a, r);
+            stat = (tid < 32 ? a.lse : a.delta)[(size_t)(kvh * a.g + r - q * a.g) * a.Mq + q0 + q];
         }
     };
-    if (t0 < t1) stage(t0, 0);
+    if (t0 < t1) fetch(t0);
     frag_t kf[KS], vf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        kf[ks] = *(const frag_t*)((const T*)a.k + (size_t)(k0 + kc) * a.ldk + kvh * DK + ks * 32 + g * 8);
-        vf[ks] = *(const frag_t*)((const T*)a.v + (size_t)(k0 + kc) * a.ldv + kvh * DK + ks * 32 + g * 8);
+        kf[ks] = x_load<E>((const T*)a.k + (size_t)(k0 + kc) * a.ldk + kvh * DK + ks * 32 + g * 8);
+        vf[ks] = x_load<E>((const T*)a.v + (size_t)(k0 + kc) * a.ldv + kvh * DK + ks * 32 + g * 8);
     }
     f32x4 dk_[DT], dv_[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dk_[dt] = dv_[dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     for (int qt = t0; qt < t1; ++qt) {
-        vm_wait_barrier<0>();
-        const int st = (qt - t0) & 1;
-        if (qt + 1 < t1) stage(qt + 1, st ^ 1);
-        const unsigned char* Qs = smem + st * STAGE;
-        const unsigned char* Ds = Qs + TL::BYTES;
-        const float* lse_s = (const float*)(Qs + 2 * TL::BYTES);
-        f32x4 s[4], dp[4];
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) s[nt] = dp[nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (qt > t0) __syncthreads();
+        fq.put(Qs, wave, lane);
+        fd.put(Ds, wave, lane);
+        if (tid < 64) rows_s[tid] = stat;
+        __syncthreads();
+        if (qt + 1 < t1) fetch(qt + 1);
+        f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, dp[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            frag_t f[4];
+            frag_t f[2];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) f[nt] = TL::template row_frag<2>(Qs, nt * 16 + i, ks, g);
-            mma16_multi<4>(f, kf[ks], s);            // rows: packed rows qt 64 + 16 nt + 4 g + e, column: key i
+            for (int rt = 0; rt < 2; ++rt) f[rt] = TL::template row_frag<2>(Qs, rt * 16 + i, ks, g);
+            x_mma<E, 2>(f, kf[ks], s);               // rows: packed rows qt 32 + 16 rt + 4 g + e, column: key i
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) f[nt] = TL::template row_frag<2>(Ds, nt * 16 + i, ks, g);
-            mma16_multi<4>(f, vf[ks], dp);
+            for (int rt = 0; rt < 2; ++rt) f[rt] = TL::template row_frag<2>(Ds, rt * 16 + i, ks, g);
+            x_mma<E, 2>(f, vf[ks], dp);
         }
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-            const f32x4 lse4 = *(const f32x4*)(lse_s + nt * 16 + 4 * g);
-            const f32x4 del4 = *(const f32x4*)(lse_s + 64 + nt * 16 + 4 * g);
+        for (int rt = 0; rt < 2; ++rt) {
+            const f32x4 lse4 = *(const f32x4*)(rows_s + rt * 16 + 4 * g), del4 = *(const f32x4*)(rows_s + 32 + rt * 16 + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = qt * 64 + nt * 16 + 4 * g + e;
+                const int r = qt * 32 + rt * 16 + 4 * g + e;
                 const bool ok = r < nrow;
-                const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[nt][e], a.scale_log2e, -lse4[e])) : 0.f;
+                const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[rt][e], a.scale_log2e, -lse4[e])) : 0.f;
                 float mul = 1.0f;
-                if (a.drop.thresh) {
+                if constexpr (DROP) {
                     const int rr = min(r, nrow - 1), q = x_query(a, rr);
                     Dropout dh = a.drop;
                     dh.stream += (uint32_t)(kvh * a.g + rr - q * a.g);
                     mul = drop_mul(dh, (uint32_t)(q0 + q), (uint32_t)kc);
                 }
-                dp[nt][e] = ok ? p * (dp[nt][e] * mul - del4[e]) : 0.f;
-                s[nt][e] = p * mul;
+                dp[rt][e] = ok ? p * (dp[rt][e] * mul - del4[e]) : 0.f;
+                s[rt][e] = p * mul;
             }
         }
+        const frag_t pf = x_pack<E>(s[0], s[1]), dsf = x_pack<E>(dp[0], dp[1]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const frag_t pf = x_pack<T>(s[2 * c], s[2 * c + 1]), dsf = x_pack<T>(dp[2 * c], dp[2 * c + 1]);
+        for (int dt0 = 0; dt0 < DT; dt0 += 2) {
+            frag_t f[2];
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                dv_[dt] = mma16(TL::template col_frag<2>(Ds, c, dt, g, i), pf, dv_[dt]);
-                dk_[dt] = mma16(TL::template col_frag<2>(Qs, c, dt, g, i), dsf, dk_[dt]);
-            }
+            for (int u = 0; u < 2; ++u) f[u] = TL::template col_frag<2>(Ds, 0, dt0 + u, g, i);
+            x_mma<E, 2>(f, pf, &dv_[dt0]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) f[u] = TL::template col_frag<2>(Qs, 0, dt0 + u, g, i);
+            x_mma<E, 2>(f, dsf, &dk_[dt0]);
         }
     }
     if (key >= lenk) return;
@@ -221,6 +271,173 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void xattn_dkv_kernel(
         for (int dt = 0; dt < DT; ++dt) {
             *(f32x4*)(dst + dt * 16) = dk_[dt] * a.scale;
             *(f32x4*)(dst + half + dt * 16) = dv_[dt];
+        }
+    }
+}
+
+// bf16: one workgroup of four waves per (utterance, shared head, 32 keys, range of packed rows).  The 32 keys stay in LDS; each wave
+// streams its OWN tiles of 32 rows through a private LDS buffer (read row-wise for S and dP, transposed for dV and dK) and keeps a
+// dK, dV of its own, so the loop has no barrier; the four are added through LDS at the end.  64 keys to a workgroup and one row tile
+// for all four waves (the fp32 form above) left half the chip without a workgroup at 32 x 120 phones unless the rows were split,
+// and wrote four times the gradients as partial sums: 27 + 5 us against 
+template <int DK, int KT, bool DROP>
+__global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
+    typedef XB16 E;
+    typedef bf16_t T;
+    typedef XTile<E, DK, 32> TL;
+    constexpr int KB = 16 * KT;
+    typedef XTile<E, DK, KB> TK;
+    typedef typename TL::frag_t frag_t;
+    constexpr int KS = TL::KS, DT = TL::DT, NP = TK::BYTES / 1024, NWK = NP % 4 == 0 ? 4 : (NP % 2 == 0 ? 2 : 1);
+    constexpr int WAVE = 2 * TL::BYTES;                  // a wave's Q tile, dO tile: 80 KB in all at dk = 128, two workgroups per CU
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // K tile, V tile (rotation 1), then the waves'
+
+    int b, kvh, blk, split;
+    if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
+    int q0, lenq, k0, lenk;
+    x_range(a.cu_q, b, a.Mq, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    if (blk * KB >= lenk) return;
+    const int nrow = lenq * a.g;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, i = lane & 15;
+    const int ntiles = (nrow + 31) / 32, per = a.nsplit == 1 ? ntiles : (ntiles + a.nsplit - 1) / a.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntiles);
+    unsigned char *Ks = smem, *Vs = smem + TK::BYTES;
+    unsigned char* Qs = smem + 2 * TK::BYTES + wave * WAVE;
+    unsigned char* Ds = Qs + TL::BYTES;
+    float stat = 0.f;                                    // lane l: lse of row l of the tile, from lane 32 on delta of row l - 32
+
+    if (wave < NWK) {
+        XFetch<E, DK, KB, 1, NWK> fk(a.ldk, wave, lane), fv(a.ldv, wave, lane);
+        const size_t first = (size_t)(k0 + blk * KB);
+        fk.fetch((const T*)a.k + first * a.ldk + kvh * DK, a.ldk, lenk - blk * KB, Ks, wave, lane);
+        fv.fetch((const T*)a.v + first * a.ldv + kvh * DK, a.ldv, lenk - blk * KB, Vs, wave, lane);
+    }
+    const T* __restrict__ qb = (const T*)a.q + (size_t)q0 * a.ldq + kvh * a.g * DK;
+    const T* __restrict__ db = (const T*)a.dctx + (size_t)q0 * a.ldo + kvh * a.g * DK;
+    XFetch<E, DK, 32, 2, 1> fq(a.ldq, 0, lane), fd(a.ldo, 0, lane);
+    auto stage = [&](int qt) __attribute__((always_inline)) {
+        if (a.g == 1) {
+            fq.fetch(qb + (size_t)qt * 32 * a.ldq, a.ldq, nrow - qt * 32, Qs, 0, lane);
+            fd.fetch(db + (size_t)qt * 32 * a.ldo, a.ldo, nrow - qt * 32, Ds, 0, lane);
+        } else {
+            fq.fetch_rows(a, qb, a.ldq, qt * 32, nrow, Qs, 0, lane);
+            fd.fetch_rows(a, db, a.ldo, qt * 32, nrow, Ds, 0, lane);
+        }
+        const int r = min(qt * 32 + (lane & 31), nrow - 1), q = x_query(a, r);
+        const size_t at = (size_t)(kvh * a.g + r - q * a.g) * a.Mq + q0 + q;
+        stat = (lane < 32 ? a.lse : a.delta)[at];
+    };
+    if (t0 + wave < t1) stage(t0 + wave);
+
+    f32x4 dk_[DT][KT], dv_[DT][KT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) dk_[dt][kt] = dv_[dt][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    vm_wait_barrier<0>();                    // the keys have landed, for every wave
+    for (int qt = t0 + wave; qt < t1; qt += 4) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's rows have landed (no other wave reads them)
+        f32x4 s[2][KT], dp[2][KT];             // [16 rows][16 keys]: lane (g, i) has rows 4 g + e, key i
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[rt][kt] = dp[rt][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            frag_t rf[2], kf[KT];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) rf[u] = TL::template row_frag<2>(Qs, u * 16 + i, ks, g);
+#pragma unroll
+            for (int u = 0; u < KT; ++u) kf[u] = TK::template row_frag<1>(Ks, u * 16 + i, ks, g);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) s[rt][kt] = mma16(rf[rt].p[0], kf[kt].p[0], s[rt][kt]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) rf[u] = TL::template row_frag<2>(Ds, u * 16 + i, ks, g);
+#pragma unroll
+            for (int u = 0; u < KT; ++u) kf[u] = TK::template row_frag<1>(Vs, u * 16 + i, ks, g);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) dp[rt][kt] = mma16(rf[rt].p[0], kf[kt].p[0], dp[rt][kt]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float lse_r = __shfl(stat, rt * 16 + 4 * g + e, 64), del_r = __shfl(stat, 32 + rt * 16 + 4 * g + e, 64);
+                const int r = qt * 32 + rt * 16 + 4 * g + e;
+                const bool ok = r < nrow;
+                Dropout dh = a.drop;
+                int q = 0;
+                if constexpr (DROP) {
+                    const int rr = min(r, nrow - 1);
+                    q = x_query(a, rr);
+                    dh.stream += (uint32_t)(kvh * a.g + rr - q * a.g);
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[rt][kt][e], a.scale_log2e, -lse_r)) : 0.f;
+                    float mul = 1.0f;
+                    if constexpr (DROP) mul = drop_mul(dh, (uint32_t)(q0 + q), (uint32_t)min(blk * KB + kt * 16 + i, lenk - 1));
+                    dp[rt][kt][e] = ok ? p * (dp[rt][kt][e] * mul - del_r) : 0.f;
+                    s[rt][kt][e] = p * mul;
+                }
+            }
+        }
+        frag_t pf[KT], dsf[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            pf[kt] = x_pack<E>(s[0][kt], s[1][kt]);
+            dsf[kt] = x_pack<E>(dp[0][kt], dp[1][kt]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const frag_t dot = TL::template col_frag<2>(Ds, 0, dt, g, i);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) dv_[dt][kt] = mma16(dot.p[0], pf[kt].p[0], dv_[dt][kt]);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const frag_t qtr = TL::template col_frag<2>(Qs, 0, dt, g, i);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) dk_[dt][kt] = mma16(qtr.p[0], dsf[kt].p[0], dk_[dt][kt]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next tile's DMA overwrites it
+        if (qt + 4 < t1) stage(qt + 4);
+    }
+    // add the four waves' gradients: [wave][32 keys][DK + 4] floats, dv then dk
+    constexpr int LDR = DK + 4, SL = DK / 4;
+    float* red = (float*)smem;
+    const size_t w = (size_t)a.KV * DK, half = (size_t)a.Mk * w;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+                *(f32x4*)(red + (wave * KB + kt * 16 + i) * LDR + dt * 16 + 4 * g) = which == 0 ? dv_[dt][kt] : dk_[dt][kt] * a.scale;
+        __syncthreads();
+        for (int e = tid; e < KB * SL; e += 256) {
+            const int key = e / SL, c = (e % SL) * 4;
+            if (blk * KB + key >= lenk) continue;
+            f32x4 sum = *(const f32x4*)(red + key * LDR + c);
+#pragma unroll
+            for (int u = 1; u < 4; ++u) sum += *(const f32x4*)(red + (u * KB + key) * LDR + c);
+            const size_t m = (size_t)(k0 + blk * KB + key);
+            if (a.nsplit > 1)                          // part[split][dk, dv][Mk][KV * DK]
+                *(f32x4*)(a.part + (size_t)split * 2 * half + (which == 0 ? half : 0) + m * w + kvh * DK + c) = sum;
+            else if (which == 0)
+                store4<T>((T*)a.dv + m * a.ldv + kvh * DK + c, sum);
+            else
+                store4<T>((T*)a.dk + m * a.ldk + kvh * DK + c, sum);
         }
     }
 }
@@ -245,75 +462,82 @@ __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int 
         store4<T>((T*)a.dk + (size_t)m * a.ldk + c, sum);
 }
 
-// ---- mass: one workgroup per (utterance, head, KB keys, range of queries) ------------------------------------------
-// The KB keys stay in LDS; the four waves stream the queries, 16 at a time, straight from memory into registers (each row is
-// read once per key block).  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds its own queries' weights over the
-// whole loop, and the 16 queries of a row of lanes meet only at the end.
-template <typename T, int DK, int KB>
-__global__ __launch_bounds__(256, 1) void xattn_mass_kernel(XArgs a) {
-    typedef XTile<T, DK, KB> TL;
-    typedef typename TL::frag_t frag_t;
-    constexpr int KS = TL::KS, NT = KB / 16;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    int b, h, blk;
-    if (!fs2_pair_order_decode(a.order, b, h, blk)) return;
-    const int split = blk % a.nsplit;
-    blk /= a.nsplit;
+// ---- mass: one workgroup per (utterance, head, 32 keys, range of queries) -----------------------------------------------
+// The 32 keys are operands in the registers of every wave; the waves stream the queries, 16 at a time, straight from memory into
+// registers, the next 16 under way.  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds up its own queries' weights over
+// the whole loop, and the 16 queries of a row of lanes meet only at the end.  16 waves (bf16; 8 in three planes): at 32 x 800
+// queries x 120 keys about one workgroup per CU, whose loads are all in flight together.
+template <typename E> constexpr int x_mass_waves() { return E::PL == 1 ? 16 : 8; }
+
+template <typename E, int DK>
+__global__ __launch_bounds__(64 * x_mass_waves<E>(), E::PL == 1 ? 4 : 2) void xattn_mass_kernel(XArgs a) {
+    typedef typename E::mem T;
+    constexpr int KS = DK / 32, NW = x_mass_waves<E>();
+    __shared__ float red[NW][32];
+    int b, h, blk, split;
+    if (!x_decode(a, a.H, b, h, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, q0, lenq);
     x_range(a.cu_k, b, a.Mk, k0, lenk);
-    if (blk * KB >= lenk) return;
+    if (blk * 32 >= lenk) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, i = lane & 15;
-    const int kvh = h / a.g;
-    TL::template stage<1, 4>((const T*)a.k + (size_t)k0 * a.ldk + kvh * DK, a.ldk, blk * KB, lenk, smem, wave, lane);
-    const int ntiles = (lenq + 15) / 16, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int kvh = x_query(a, h);                       // h / g
+    const int ntiles = (lenq + 15) / 16, per = a.nsplit == 1 ? ntiles : (ntiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * per, t1 = min(t0 + per, ntiles);
-    f32x4 acc[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const T* __restrict__ qb = (const T*)a.q + (size_t)q0 * a.ldq + h * DK;
+    const T* __restrict__ qb = (const T*)a.q + (size_t)q0 * a.ldq + h * DK + g * 8;
     const float* __restrict__ lse = a.lse + (size_t)h * a.Mq + q0;
-    vm_wait_barrier<0>();
-    for (int qt = t0 + wave; qt < t1; qt += 4) {
+    typename std::conditional<E::PL == 1, XFrag<E>, XRaw>::type raw[KS];
+    float l = INFINITY;
+    auto fetch = [&](int qt) __attribute__((always_inline)) {
         const int q = qt * 16 + i, qc = min(q, lenq - 1);
-        frag_t qf[KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const frag_t*)(qb + (size_t)qc * a.ldq + ks * 32 + g * 8);
-        float l = lse[qc];
-        if (q >= lenq || !(fabsf(l) < INFINITY)) l = INFINITY;          // no such query: no weight
-#pragma unroll
-        for (int n4 = 0; n4 < NT; n4 += 4) {
-            f32x4 s[4];
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt) s[nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                frag_t kf[4];
-#pragma unroll
-                for (int nt = 0; nt < 4; ++nt) kf[nt] = TL::template row_frag<1>(smem, (n4 + nt) * 16 + i, ks, g);
-                mma16_multi<4>(kf, qf[ks], s);
-            }
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n4 + nt][e] += __builtin_amdgcn_exp2f(fmaf(s[nt][e], a.scale_log2e, -l));
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (E::PL == 1) raw[ks] = x_load<E>(qb + (size_t)qc * a.ldq + ks * 32);
+            else raw[ks] = x_raw(qb + (size_t)qc * a.ldq + ks * 32);
         }
-    }
-    __syncthreads();
-    float* red = (float*)smem;          // [4][KB]
+        l = lse[qc];
+        if (q >= lenq || !(fabsf(l) < INFINITY)) l = INFINITY;          // no such query: no weight
+    };
+    if (t0 + wave < t1) fetch(t0 + wave);
+    XFrag<E> kf[KS][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+            kf[ks][kt] = x_load<E>((const T*)a.k + (size_t)(k0 + min(blk * 32 + kt * 16 + i, lenk - 1)) * a.ldk + kvh * DK + ks * 32 + g * 8);
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int qt = t0 + wave; qt < t1; qt += NW) {
+        XFrag<E> qf[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (E::PL == 1) qf[ks] = raw[ks];
+            else qf[ks] = x_split8<true>(raw[ks]);
+        }
+        const float lq = l;
+        if (qt + NW < t1) fetch(qt + NW);
+        f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x_mma<E, 2>(kf[ks], qf[ks], s);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[kt][e] += __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2e, -lq));
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float v = row16_sum(acc[nt][e]);
-            if (i == 0) red[wave * KB + nt * 16 + 4 * g + e] = v;
+            const float v = row16_sum(acc[kt][e]);
+            if (i == 0) red[wave][kt * 16 + 4 * g + e] = v;
         }
     __syncthreads();
-    const int key = blk * KB + tid;
-    if (tid < KB && key < lenk) {
-        const float v = red[tid] + red[KB + tid] + red[2 * KB + tid] + red[3 * KB + tid];
+    const int key = blk * 32 + tid;
+    if (tid < 32 && key < lenk) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += red[w][tid];
         float* dst = a.nsplit == 1 ? a.mass : a.part + (size_t)split * a.H * a.Mk;
         dst[(size_t)h * a.Mk + k0 + key] = v;
     }
@@ -329,35 +553,63 @@ __global__ __launch_bounds__(256) void xattn_mass_sum_kernel(XArgs a, int B) {
     a.mass[at] = sum;
 }
 
-constexpr int X_MASS_KB = 128;
-
-static int x_dkv_split(int B, int max_q, int max_k, int H, int KV) {
-    const long items = (long)B * KV * ((max_k + 63) / 64), tiles = ((long)max_q * (H / KV) + 63) / 64;
-    if (items >= 256 || tiles < 4) return 1;
-    const long want = 512 / items, most = tiles / 2, n = want < most ? want : most;
+// Row ranges of the key kernels, chosen from the shape: a workgroup for every CU where the keys alone do not give one, and at least
+// four row tiles to a wave (bf16) or to the workgroup (fp32).  More would only add partial sums.
+static int x_dkv_split(int B, int max_q, int max_k, int H, int KV, int dtype) {
+    const int kb = dtype == 1 ? 32 : 64;
+    const long items = (long)B * KV * ((max_k + kb - 1) / kb), tiles = ((long)max_q * (H / KV) + 31) / 32;
+    if (items >= 192 || tiles < 8) return 1;
+    const long want = 512 / items, most = dtype == 1 ? tiles / 8 : tiles / 4, n = want < most ? want : most;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
-static int x_mass_split(int B, int max_q, int max_k, int H) {
-    const long items = (long)B * H * ((max_k + X_MASS_KB - 1) / X_MASS_KB), tiles = (max_q + 15) / 16;
-    if (items >= 256 || tiles < 8) return 1;
-    const long want = 512 / items, most = tiles / 4, n = want < most ? want : most;
-    return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
+static int x_mass_split(int B, int max_q, int max_k, int H, int dtype) {
+    const long items = (long)B * H * ((max_k + 31) / 32), trips = (max_q + 15) / 16 / (dtype == 1 ? 16 : 8);
+    if (items >= 192 || trips < 8) return 1;
+    const long want = 512 / items, most = trips / 2, n = want < most ? want : most;
+    return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
 
-template <typename T, int DK>
+template <typename E, int DK, bool DROP> static void launch_xattn_dq(const XArgs& a, dim3 grid, hipStream_t stream) {
+    constexpr int lds = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_dq_kb<E, DK>()>::BYTES;
+    static unsigned long long ok = 0;
+    fs2_allow_lds((const void*)xattn_dq_kernel<E, DK, DROP>, lds, &ok);
+    hipLaunchKernelGGL((xattn_dq_kernel<E, DK, DROP>), grid, dim3(256), lds, stream, a);
+}
+template <int DK, bool DROP> static void launch_xattn_dkv(const XArgs& a, dim3 grid, hipStream_t stream) {
+    constexpr int lds = 2 * XTile<XF32, DK, 32>::BYTES + 256;
+    static unsigned long long ok = 0;
+    fs2_allow_lds((const void*)xattn_dkv_kernel<DK, DROP>, lds, &ok);
+    hipLaunchKernelGGL((xattn_dkv_kernel<DK, DROP>), grid, dim3(256), lds, stream, a);
+}
+template <int DK, int KT, bool DROP> static void launch_xattn_dkv32(const XArgs& a, dim3 grid, hipStream_t stream) {
+    constexpr int tiles = 8 * XTile<XB16, DK, 32>::BYTES + 2 * XTile<XB16, DK, 16 * KT>::BYTES, merge = 4 * 16 * KT * (DK + 4) * 4;
+    constexpr int lds = tiles > merge ? tiles : merge;
+    static unsigned long long ok = 0;
+    fs2_allow_lds((const void*)xattn_dkv32_kernel<DK, KT, DROP>, lds, &ok);
+    hipLaunchKernelGGL((xattn_dkv32_kernel<DK, KT, DROP>), grid, dim3(256), lds, stream, a);
+}
+
+template <typename E, int DK>
 static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipStream_t stream) {
-    constexpr int lds_dq = 4 * XTile<T, DK>::BYTES, lds_dkv = lds_dq + 2 * 512;
-    static unsigned long long ok_dq = 0, ok_dkv = 0;
-    fs2_allow_lds((const void*)xattn_dq_kernel<T, DK>, lds_dq, &ok_dq);
-    fs2_allow_lds((const void*)xattn_dkv_kernel<T, DK>, lds_dkv, &ok_dkv);
+    typedef typename E::mem T;
     if (max_q > 0) {
-        const dim3 grid = fs2_pair_order_grid(a.order, (max_q * a.g + 63) / 64, a.KV, B, true);
-        hipLaunchKernelGGL((xattn_dq_kernel<T, DK>), grid, dim3(256), lds_dq, stream, a);
+        XArgs b = a;
+        b.nsplit = 1;
+        const dim3 grid = fs2_x_grid(b, (max_q * a.g + 63) / 64, a.KV, B);
+        if (a.drop.thresh) launch_xattn_dq<E, DK, true>(b, grid, stream);
+        else launch_xattn_dq<E, DK, false>(b, grid, stream);
         FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(dq)");
     }
     if (max_k > 0) {
-        const dim3 grid = fs2_pair_order_grid(a.order, ((max_k + 63) / 64) * a.nsplit, a.KV, B, true);
-        hipLaunchKernelGGL((xattn_dkv_kernel<T, DK>), grid, dim3(256), lds_dkv, stream, a);
+        if constexpr (E::PL == 1) {
+            const dim3 grid = fs2_x_grid(a, (max_k + 31) / 32, a.KV, B);
+            if (a.drop.thresh) launch_xattn_dkv32<DK, 2, true>(a, grid, stream);
+            else launch_xattn_dkv32<DK, 2, false>(a, grid, stream);
+        } else {
+            const dim3 grid = fs2_x_grid(a, (max_k + 63) / 64, a.KV, B);
+            if (a.drop.thresh) launch_xattn_dkv<DK, true>(a, grid, stream);
+            else launch_xattn_dkv<DK, false>(a, grid, stream);
+        }
         FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(dk, dv)");
         if (a.nsplit > 1) {
             const long long n = 2LL * a.Mk * (a.KV * dk / 4);
@@ -368,13 +620,10 @@ static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipSt
     return FS2_OK;
 }
 
-template <typename T, int DK>
+template <typename E, int DK>
 static int launch_xattn_mass(XArgs& a, int B, int max_k, hipStream_t stream) {
-    constexpr int lds = XTile<T, DK, X_MASS_KB>::BYTES;
-    static unsigned long long ok = 0;
-    fs2_allow_lds((const void*)xattn_mass_kernel<T, DK, X_MASS_KB>, lds, &ok);
-    const dim3 grid = fs2_pair_order_grid(a.order, ((max_k + X_MASS_KB - 1) / X_MASS_KB) * a.nsplit, a.H, B, true);
-    hipLaunchKernelGGL((xattn_mass_kernel<T, DK, X_MASS_KB>), grid, dim3(256), lds, stream, a);
+    const dim3 grid = fs2_x_grid(a, (max_k + 31) / 32, a.H, B);
+    hipLaunchKernelGGL((xattn_mass_kernel<E, DK>), grid, dim3(64 * x_mass_waves<E>()), 0, stream, a);
     FS2_CHECK_LAUNCH("fs2_cross_attention_mass");
     if (a.nsplit > 1) {
         const long long n = (long long)a.H * a.Mk;
@@ -393,9 +642,8 @@ static inline long long x_delta_floats(int H, int Mq) { return ((long long)H * M
 
 extern "C" long long fs2_cross_attention_bwd_workspace(int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads,
                                                        int dk, int dtype) {
-    (void)dtype;
     if (B <= 0 || max_q <= 0 || max_k <= 0 || Mq <= 0 || Mk <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return 16;
-    const int n = x_dkv_split(B, max_q, max_k, n_heads, n_kv_heads);
+    const int n = x_dkv_split(B, max_q, max_k, n_heads, n_kv_heads, dtype);
     return (x_delta_floats(n_heads, Mq) + (n > 1 ? 2LL * n * Mk * n_kv_heads * dk : 0)) * (long long)sizeof(float);
 }
 
@@ -412,7 +660,7 @@ extern "C" int fs2_cross_attention_bwd(const void* q, const void* k, const void*
     FS2_CHECK_ARG((Mq == 0 || (ctx && dctx && lse && dq)) && (Mk == 0 || (v && dk_out && dv)), "fs2_cross_attention_bwd: null argument");
     FS2_CHECK_ARG((((uintptr_t)v | (uintptr_t)ctx | (uintptr_t)dctx | (uintptr_t)dq | (uintptr_t)dk_out | (uintptr_t)dv) & 15) == 0,
                   "fs2_cross_attention_bwd: unaligned pointers");
-    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldo >= n_heads * dk && ldv % epv == 0 && ldo % epv == 0,
+    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldv <= (1 << 20) && ldo >= n_heads * dk && ldv % epv == 0 && ldo % epv == 0,
                   "fs2_cross_attention_bwd: bad leading dims ldv=%d ldo=%d", ldv, ldo);
     if (max_q == 0 && max_k == 0) return FS2_OK;
     FS2_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0,
@@ -422,26 +670,26 @@ extern "C" int fs2_cross_attention_bwd(const void* q, const void* k, const void*
     a.drop = fs2_make_dropout(seed, stream_id, rate);
     a.delta = (float*)workspace;
     a.part = (float*)workspace + x_delta_floats(n_heads, Mq);
-    a.nsplit = max_q > 0 && max_k > 0 ? x_dkv_split(B, max_q, max_k, n_heads, n_kv_heads) : 1;
+    a.nsplit = max_q > 0 && max_k > 0 ? x_dkv_split(B, max_q, max_k, n_heads, n_kv_heads, dtype) : 1;
 #define FS2_X(TT, DKK) return launch_xattn_bwd<TT, DKK>(a, B, max_q, max_k, dk, stream)
     if (dtype == 0) {
-        if (dk == 32) FS2_X(float, 32);
-        if (dk == 64) FS2_X(float, 64);
-        if (dk == 96) FS2_X(float, 96);
-        FS2_X(float, 128);
+        if (dk == 32) FS2_X(XF32, 32);
+        if (dk == 64) FS2_X(XF32, 64);
+        if (dk == 96) FS2_X(XF32, 96);
+        FS2_X(XF32, 128);
     }
-    if (dk == 32) FS2_X(bf16_t, 32);
-    if (dk == 64) FS2_X(bf16_t, 64);
-    if (dk == 96) FS2_X(bf16_t, 96);
-    FS2_X(bf16_t, 128);
+    if (dk == 32) FS2_X(XB16, 32);
+    if (dk == 64) FS2_X(XB16, 64);
+    if (dk == 96) FS2_X(XB16, 96);
+    FS2_X(XB16, 128);
 #undef FS2_X
 }
 
 extern "C" long long fs2_cross_attention_mass_workspace(int B, int max_q, int max_k, int Mk, int n_heads, int n_kv_heads, int dk,
                                                         int dtype) {
-    (void)n_kv_heads; (void)dk; (void)dtype;
+    (void)n_kv_heads; (void)dk;
     if (B <= 0 || max_q <= 0 || max_k <= 0 || Mk <= 0 || n_heads <= 0) return 0;
-    const int n = x_mass_split(B, max_q, max_k, n_heads);
+    const int n = x_mass_split(B, max_q, max_k, n_heads, dtype);
     return n > 1 ? (long long)n * n_heads * Mk * (long long)sizeof(float) : 0;
 }
 
@@ -456,19 +704,19 @@ extern "C" int fs2_cross_attention_mass(const void* q, const void* k, const floa
     XArgs a = fs2_x_args(q, k, nullptr, cu_q, cu_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, 0, 0);
     a.lse = (float*)lse;
     a.mass = mass;
-    a.nsplit = max_q > 0 ? x_mass_split(B, max_q, max_k, n_heads) : 1;
+    a.nsplit = max_q > 0 ? x_mass_split(B, max_q, max_k, n_heads, dtype) : 1;
     a.part = (float*)workspace;
     FS2_CHECK_ARG(a.nsplit == 1 || workspace, "fs2_cross_attention_mass: this shape needs fs2_cross_attention_mass_workspace bytes");
 #define FS2_X(TT, DKK) return launch_xattn_mass<TT, DKK>(a, B, max_k, stream)
     if (dtype == 0) {
-        if (dk == 32) FS2_X(float, 32);
-        if (dk == 64) FS2_X(float, 64);
-        if (dk == 96) FS2_X(float, 96);
-        FS2_X(float, 128);
+        if (dk == 32) FS2_X(XF32, 32);
+        if (dk == 64) FS2_X(XF32, 64);
+        if (dk == 96) FS2_X(XF32, 96);
+        FS2_X(XF32, 128);
     }
-    if (dk == 32) FS2_X(bf16_t, 32);
-    if (dk == 64) FS2_X(bf16_t, 64);
-    if (dk == 96) FS2_X(bf16_t, 96);
-    FS2_X(bf16_t, 128);
+    if (dk == 32) FS2_X(XB16, 32);
+    if (dk == 64) FS2_X(XB16, 64);
+    if (dk == 96) FS2_X(XB16, 96);
+    FS2_X(XB16, 128);
 #undef FS2_X
 }
