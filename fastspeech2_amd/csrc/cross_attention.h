@@ -132,6 +132,13 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_load(const typename 
         return x_split8<true>(x_raw(p));
     }
 }
+// element j of an operand
+template <typename E> __device__ __forceinline__ float x_value(const XFrag<E>& f, int j) {
+    float v = to_f32(f.p[E::PL - 1][j]);
+#pragma unroll
+    for (int pl = E::PL - 2; pl >= 0; --pl) v += to_f32(f.p[pl][j]);
+    return v;
+}
 // accumulator pair -> operand (k-slot (g, jj) <-> row 16 (jj / 4) + 4 g + jj % 4 of the 32)
 template <typename E> __device__ __forceinline__ XFrag<E> x_pack(const f32x4& lo, const f32x4& hi) {
     if constexpr (E::PL == 1) {
@@ -254,39 +261,86 @@ template <int DK, int ROWS, int ROT, int NW> struct XFetch<XB16, DK, ROWS, ROT, 
 
 template <int DK, int ROWS, int ROT, int NW> struct XFetch<XF32, DK, ROWS, ROT, NW> {
     typedef XTile<XF32, DK, ROWS> TL;
-    static constexpr int SPR = DK / 8, SLOTS = ROWS * SPR;                 // 8-element slots of a row, of the tile
-    static constexpr int N = (SLOTS + 64 * NW - 1) / (64 * NW);                // of a lane (the last of them may be missing)
-    static __device__ __forceinline__ bool has(int id) { return SLOTS % (64 * NW) == 0 || id < SLOTS; }
-    XRaw r[N];
+    static constexpr int CPR = DK / 4, CHUNKS = ROWS * CPR;                     // 16-byte chunks of a row, of the tile
+    static constexpr int N = (CHUNKS + 64 * NW - 1) / (64 * NW);                // of a lane (the last of them may be missing)
+    static __device__ __forceinline__ bool has(int id) { return CHUNKS % (64 * NW) == 0 || id < CHUNKS; }
+    f32x4 r[N];
     __device__ __forceinline__ XFetch(int, int, int) {}
     __device__ __forceinline__ void fetch(const float* __restrict__ tile, int ld, int left, unsigned char*, int wave, int lane) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int id = n * 64 * NW + wave * 64 + lane, row = id / SPR, s = id - row * SPR;
-            if (has(id)) r[n] = x_raw((const float*)((const unsigned char*)tile + (unsigned)min(row, left - 1) * (unsigned)ld * 4u + (unsigned)s * 32u));
+            const int id = n * 64 * NW + wave * 64 + lane, row = id / CPR, c = id - row * CPR;
+            if (has(id))
+                r[n] = *(const f32x4*)((const unsigned char*)tile + (unsigned)min(row, left - 1) * (unsigned)ld * 4u + (unsigned)c * 16u);
         }
     }
     __device__ __forceinline__ void fetch_rows(const XArgs& a, const float* __restrict__ base, int ld, int first, int nrow, unsigned char*,
                                                int wave, int lane) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int id = n * 64 * NW + wave * 64 + lane, row = id / SPR, s = id - row * SPR;
+            const int id = n * 64 * NW + wave * 64 + lane, row = id / CPR, c = id - row * CPR;
             const int rr = min(first + row, nrow - 1), q = x_query(a, rr);
-            if (has(id)) r[n] = x_raw(base + (size_t)q * ld + (rr - q * a.g) * DK + s * 8);
+            if (has(id)) r[n] = *(const f32x4*)(base + (size_t)q * ld + (rr - q * a.g) * DK + c * 4);
         }
     }
     __device__ __forceinline__ void put(unsigned char* dst, int wave, int lane) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int id = n * 64 * NW + wave * 64 + lane, row = id / SPR, s = id - row * SPR;
+            const int id = n * 64 * NW + wave * 64 + lane, row = id / CPR, c = id - row * CPR;
             if (!has(id)) continue;
-            const XFrag<XF32> f = x_split8<true>(r[n]);
-            unsigned char* at = dst + row * TL::ROWB + ((s + TL::template rot<ROT>(row)) % TL::NS) * 16;
+            uint2 w[3];
+            x_split2<true>(r[n][0], r[n][1], w[0].x, w[1].x, w[2].x);
+            x_split2<true>(r[n][2], r[n][3], w[0].y, w[1].y, w[2].y);
+            unsigned char* at = dst + row * TL::ROWB + (((c >> 1) + TL::template rot<ROT>(row)) % TL::NS) * 16 + (c & 1) * 8;
 #pragma unroll
-            for (int pl = 0; pl < 3; ++pl) *(bf16x8*)(at + pl * TL::PLANE) = f.p[pl];
+            for (int pl = 0; pl < 3; ++pl) *(uint2*)(at + pl * TL::PLANE) = w[pl];
         }
     }
 };
+
+// A wave's own packed rows [first, first + ROWS) of the heads at `base` as operands, through its own LDS (XTile<E, DK, ROWS>::BYTES):
+// a fragment load straight from memory has 16 rows in consecutive lanes, one cache access per lane instead of one per line (64
+// against 8 at dk = 128; the attention mass of 32 x 800 queries spent 9 us of cache accesses that way).  start(), then finish().
+template <typename E, int DK, int ROWS> struct XRows {
+    typedef XTile<E, DK, ROWS> TL;
+    XFetch<E, DK, ROWS, 1, 1> f;
+    __device__ __forceinline__ XRows(int ld, int lane) : f(ld, 0, lane) {}
+    __device__ __forceinline__ void start(const XArgs& a, const typename E::mem* __restrict__ base, int ld, int first, int nrow,
+                                          unsigned char* lds, int lane) {
+        if (a.g == 1)
+            f.fetch(base + (size_t)first * ld, ld, nrow - first, lds, 0, lane);
+        else
+            f.fetch_rows(a, base, ld, first, nrow, lds, 0, lane);
+    }
+    // XB16: what start() began has landed (vmcnt(0) waits for everything the wave has under way)
+    __device__ __forceinline__ void finish(unsigned char* lds, int lane) {
+        f.put(lds, 0, lane);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    }
+};
+
+// Rows of results back to memory: accumulators of 16 packed rows (lane (g, i): row i, columns 16 dt + 4 g ..) through the wave's own
+// LDS (16 x (DK * 4 + 16) bytes at most), then 16 bytes a lane along the rows.
+template <typename T, int DK> constexpr int x_out_bytes() { return 16 * (DK * (int)sizeof(T) + 16); }
+template <typename T, int DK>
+__device__ __forceinline__ void x_store_rows(const XArgs& a, T* __restrict__ dst, int ld, int q0, int kvh, int first, int nrow,
+                                             const f32x4 (&v)[DK / 16], unsigned char* lds, int lane) {
+    constexpr int PITCH = DK * (int)sizeof(T) + 16, CPR = DK * (int)sizeof(T) / 16, N = 16 * CPR / 64;
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int dt = 0; dt < DK / 16; ++dt) store4<T>((T*)(lds + i * PITCH) + dt * 16 + 4 * g, v[dt]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int id = n * 64 + lane, row = id / CPR, c = id - row * CPR, r = first + row;
+        if (r < nrow) {
+            const int q = x_query(a, r);
+            *(vec16*)((unsigned char*)(dst + (size_t)(q0 + q) * ld + (kvh * a.g + r - q * a.g) * DK) + c * 16) =
+                *(const vec16*)(lds + row * PITCH + c * 16);
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next rows overwrite it
+}
 
 }  // namespace fs2
 

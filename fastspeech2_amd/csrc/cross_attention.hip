@@ -51,25 +51,13 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
         x_zero_rows<T, DK>(a, q0, kvh, blk * BQ, min(nrow, blk * BQ + BQ));
         return;
     }
-    int qrow[QT], head[QT];
-    bool live[QT];
-    auto place = [&](int t) __attribute__((always_inline)) {
-        const int r = blk * BQ + (wave * QT + t) * 16 + i;
-        live[t] = r < nrow;
-        const int rc = min(r, nrow - 1), q = x_query(a, rc);
-        qrow[t] = q0 + q;
-        head[t] = kvh * a.g + rc - q * a.g;
-    };
-#pragma unroll
-    for (int t = 0; t < QT; ++t) place(t);
     if (t0 >= t1) {         // this split has no keys: (max, sum) = (-inf, 0)
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-            if (g == 0 && live[t]) {
-                float* ml = a.part + (size_t)a.nsplit * a.Mq * a.H * DK + (((size_t)split * a.H + head[t]) * a.Mq + qrow[t]) * 2;
-                ml[0] = -INFINITY;
-                ml[1] = 0.f;
-            }
+        for (int r = blk * BQ + tid; r < min(nrow, blk * BQ + BQ); r += 256) {
+            const int q = x_query(a, r), head = kvh * a.g + r - q * a.g;
+            float* ml = a.part + (size_t)a.nsplit * a.Mq * a.H * DK + (((size_t)split * a.H + head) * a.Mq + q0 + q) * 2;
+            ml[0] = -INFINITY;
+            ml[1] = 0.f;
+        }
         return;
     }
     const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
@@ -83,12 +71,20 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
     };
     fetch(t0, 0);
 
+    // the queries, through the other stage (bf16) or ahead of the first tile (fp32): every wave has read its own before the barrier
+    // behind which that memory is filled again
     frag_t qf[QT][KS];
+    {
+        typedef XTile<E, DK, 16 * QT> TQ;
+        unsigned char* own = smem + (NST == 2 ? 2 * TL::BYTES : 0) + wave * TQ::BYTES;
+        XRows<E, DK, 16 * QT> rows(a.ldq, lane);
+        rows.start(a, (const T*)a.q + (size_t)q0 * a.ldq + kvh * a.g * DK, a.ldq, min(blk * BQ + wave * 16 * QT, nrow - 1), nrow, own, lane);
+        rows.finish(own, lane);
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+        for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-            qf[t][ks] = x_load<E>((const T*)a.q + (size_t)qrow[t] * a.ldq + head[t] * DK + ks * 32 + g * 8);
+            for (int ks = 0; ks < KS; ++ks) qf[t][ks] = TQ::template row_frag<1>(own, t * 16 + i, ks, g);
+    }
 
     f32x4 o[QT][DT];
     float m_run[QT], l_part[QT];
@@ -106,7 +102,7 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
         if constexpr (E::PL == 1) {
             vm_wait_barrier<0>();         // tile kt has landed; every wave is done with the other stage
         } else {
-            if (kt > t0) __syncthreads();                // every wave is done with the tile before
+            __syncthreads();                             // every wave is done with the tile (or its queries) before
             fk.put(Ks, wave, lane);
             fv.put(Vs, wave, lane);
             __syncthreads();
@@ -178,12 +174,13 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
                 }
             l_part[t] += psum;
             if constexpr (DROP) {      // the sum above is over the undropped probabilities
+                const int row = min(blk * BQ + (wave * QT + t) * 16 + i, nrow - 1), q = x_query(a, row);
                 Dropout dh = a.drop;
-                dh.stream += (uint32_t)head[t];
+                dh.stream += (uint32_t)(kvh * a.g + row - q * a.g);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][nt][r] *= drop_mul(dh, (uint32_t)qrow[t], (uint32_t)(kbase + nt * 16 + r));
+                    for (int r = 0; r < 4; ++r) s[t][nt][r] *= drop_mul(dh, (uint32_t)(q0 + q), (uint32_t)(kbase + nt * 16 + r));
             }
         }
         if constexpr (E::PL == 1) {
@@ -215,25 +212,24 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
             }
         }
     }
-    if constexpr (!DROP) asm volatile("" : "+s"(blk));       // the rows' places are worked out again, not carried through the loop
+    __syncthreads();                                     // the tiles' memory serves the waves' results now
+    unsigned char* own = smem + wave * x_out_bytes<float, DK>();
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const float l = rows_sum(l_part[t]);
-        place(t);
-        if (!live[t]) continue;
+        const int first = blk * BQ + (wave * QT + t) * 16, r = first + i;
+        const int q = x_query(a, min(r, nrow - 1)), head = kvh * a.g + min(r, nrow - 1) - q * a.g;
         if (a.nsplit == 1) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;        // no score above -inf: a zero row
-            if (a.lse && g == 0) a.lse[(size_t)head[t] * a.Mq + qrow[t]] = m_run[t] + __log2f(l);
-            T* dst = (T*)a.ctx + (size_t)qrow[t] * a.ldo + head[t] * DK + 4 * g;
+            if (a.lse && g == 0 && r < nrow) a.lse[(size_t)head * a.Mq + q0 + q] = m_run[t] + __log2f(l);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) store4<T>(dst + dt * 16, o[t][dt] * inv);
+            for (int dt = 0; dt < DT; ++dt) o[t][dt] *= inv;
+            x_store_rows<T, DK>(a, (T*)a.ctx, a.ldo, q0, kvh, first, nrow, o[t], own, lane);
         } else {
-            const size_t d = (size_t)a.H * DK;
-            float* dst = a.part + ((size_t)split * a.Mq + qrow[t]) * d + head[t] * DK + 4 * g;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) *(f32x4*)(dst + dt * 16) = o[t][dt];
-            float* ml = a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)split * a.H + head[t]) * a.Mq + qrow[t]) * 2;
-            if (g == 0) {
+            const int d = a.H * DK;
+            x_store_rows<float, DK>(a, a.part + (size_t)split * a.Mq * d, d, q0, kvh, first, nrow, o[t], own, lane);
+            float* ml = a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)split * a.H + head) * a.Mq + q0 + q) * 2;
+            if (g == 0 && r < nrow) {
                 ml[0] = m_run[t];
                 ml[1] = l;
             }
@@ -271,27 +267,29 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
 
     const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
     const T* __restrict__ vb = (const T*)a.v + (size_t)k0 * a.ldv + kvh * DK;
-    unsigned char* Vs = smem + wave * TL::BYTES;
+    constexpr int KL = E::PL == 1 ? TL::BYTES : 0;          // K goes through LDS too (fp32: three planes of both do not fit)
+    unsigned char* Ks = smem + wave * (TL::BYTES + KL);
+    unsigned char* Vs = Ks + KL;
+    XFetch<E, DK, 32, 1, 1> fk(a.ldk, 0, lane);
     XFetch<E, DK, 32, 2, 1> fv(a.ldv, 0, lane);
     f32x4 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_part = 0.f;
     for (int kt = t0 + wave; kt < t1; kt += 4) {
+        if constexpr (E::PL == 1) fk.fetch(kb + (size_t)kt * 32 * a.ldk, a.ldk, lenk - kt * 32, Ks, 0, lane);
         fv.fetch(vb + (size_t)kt * 32 * a.ldv, a.ldv, lenk - kt * 32, Vs, 0, lane);
         f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        frag_t kf[E::PL == 1 ? KS : 1][2];
+        if constexpr (E::PL == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's tiles have landed (no other wave reads them)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            frag_t (&f)[2] = kf[E::PL == 1 ? ks : 0];
+            frag_t f[2];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-                f[nt] = x_load<E>(kb + (size_t)min(kt * 32 + nt * 16 + i, lenk - 1) * a.ldk + ks * 32 + g * 8);
-            if constexpr (E::PL == 3) x_mma<E, 2>(f, qf[ks], s);
-        }
-        if constexpr (E::PL == 1) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) x_mma<E, 2>(kf[ks], qf[ks], s);
+            for (int nt = 0; nt < 2; ++nt) {
+                if constexpr (E::PL == 1) f[nt] = TL::template row_frag<1>(Ks, nt * 16 + i, ks, g);
+                else f[nt] = x_load<E>(kb + (size_t)min(kt * 32 + nt * 16 + i, lenk - 1) * a.ldk + ks * 32 + g * 8);
+            }
+            x_mma<E, 2>(f, qf[ks], s);
         }
         const int kbase = kt * 32 + 4 * g;
         float m_loc = -INFINITY;
@@ -324,8 +322,10 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
                 for (int r = 0; r < 4; ++r) s[nt][r] *= drop_mul(dh, (uint32_t)qrow, (uint32_t)(kbase + nt * 16 + r));
         }
         const frag_t pf = x_pack<E>(s[0], s[1]);
-        fv.put(Vs, 0, lane);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // this wave's V tile has landed (no other wave reads it)
+        if constexpr (E::PL == 3) {
+            fv.put(Vs, 0, lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
 #pragma unroll
         for (int dt0 = 0; dt0 < DT; dt0 += 2) {
             frag_t v2[2];
@@ -438,7 +438,9 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dk, int dtyp
 }
 
 template <typename E, int DK, int QT, bool DROP> static void launch_xattn_rows(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int lds = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_kb<E, DK>()>::BYTES;
+    constexpr int tiles = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_kb<E, DK>()>::BYTES, out = 4 * x_out_bytes<float, DK>();
+    constexpr int lds = tiles > out ? tiles : out;
+    static_assert(lds >= 4 * XTile<E, DK, 16 * QT>::BYTES + (E::PL == 1 ? 2 * XTile<E, DK, 64>::BYTES : 0), "room for the queries");
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_rows_kernel<E, DK, QT, DROP>, lds, &ok);
     hipLaunchKernelGGL((xattn_rows_kernel<E, DK, QT, DROP>), grid, dim3(256), lds, stream, a);
@@ -448,7 +450,7 @@ template <typename E, int DK>
 static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipStream_t stream) {
     typedef typename E::mem T;
     if (p.few) {
-        constexpr int merge = 4 * 16 * DK * 4 + 512, tiles = 4 * XTile<E, DK, 32>::BYTES;
+        constexpr int merge = 4 * 16 * DK * 4 + 512, tiles = (E::PL == 1 ? 8 : 4) * XTile<E, DK, 32>::BYTES;
         constexpr int lds = merge > tiles ? merge : tiles;
         static unsigned long long ok = 0;
         fs2_allow_lds((const void*)xattn_few_kernel<E, DK>, lds, &ok);

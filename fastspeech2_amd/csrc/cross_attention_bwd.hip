@@ -51,23 +51,37 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     };
     if (lenk > 0) fetch(0, 0);
 
+    // q, dO and ctx rows of the wave: bf16 in the other stage and behind it, all under way together; fp32 one after the other
     frag_t qf[KS], dof[KS];
     float del = 0.f;
+    {
+        typedef XTile<E, DK, 16> TQ;
+        unsigned char* own = smem + (NST == 2 ? 2 * TL::BYTES : 0) + wave * TQ::BYTES;
+        constexpr int NEXT = E::PL == 1 ? 4 * TQ::BYTES : 0;
+        const int first = min(blk * 64 + wave * 16, nrow - 1);
+        const size_t at = (size_t)q0 * a.ldq + kvh * a.g * DK, ato = (size_t)q0 * a.ldo + kvh * a.g * DK;
+        XRows<E, DK, 16> rq(a.ldq, lane), rd(a.ldo, lane), rc(a.ldo, lane);
+        rq.start(a, (const T*)a.q + at, a.ldq, first, nrow, own, lane);
+        rd.start(a, (const T*)a.dctx + ato, a.ldo, first, nrow, own + NEXT, lane);
+        rc.start(a, (const T*)a.ctx + ato, a.ldo, first, nrow, own + 2 * NEXT, lane);
+        rq.finish(own, lane);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const int c = head * DK + ks * 32 + g * 8;
-        const T* od = (const T*)a.dctx + (size_t)qrow * a.ldo + c;
-        const T* oc = (const T*)a.ctx + (size_t)qrow * a.ldo + c;
-        qf[ks] = x_load<E>((const T*)a.q + (size_t)qrow * a.ldq + c);
-        dof[ks] = x_load<E>(od);
-        if constexpr (E::PL == 1) {
-            const bf16x8 of = *(const bf16x8*)oc;
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = TQ::template row_frag<1>(own, i, ks, g);
+        if constexpr (E::PL == 3) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            rd.finish(own, lane);
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) del = fmaf(to_f32(dof[ks].p[0][j]), to_f32(of[j]), del);
-        } else {
-            const XRaw u = x_raw(od), v = x_raw(oc);
+        for (int ks = 0; ks < KS; ++ks) dof[ks] = TQ::template row_frag<1>(own + NEXT, i, ks, g);
+        if constexpr (E::PL == 3) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            rc.finish(own, lane);
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) del = fmaf(u.v[j], v.v[j], del);
+        for (int ks = 0; ks < KS; ++ks) {
+            const frag_t of = TQ::template row_frag<1>(own + 2 * NEXT, i, ks, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) del = fmaf(x_value<E>(dof[ks], j), x_value<E>(of, j), del);
         }
     }
     del = rows_sum(del);
@@ -87,7 +101,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
         if constexpr (E::PL == 1) {
             vm_wait_barrier<0>();      // tile kt has landed; every wave is done with the other stage
         } else {
-            if (kt > 0) __syncthreads();
+            __syncthreads();           // every wave is done with the tile (or its rows) before
             fk.put(Ks, wave, lane);
             fv.put(Vs, wave, lane);
             __syncthreads();
@@ -149,11 +163,10 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
             }
         }
     }
-    if (r < nrow) {
-        T* dst = (T*)a.dq + (size_t)qrow * a.ldq + head * DK + 4 * g;
+    __syncthreads();                   // the tiles' memory serves the waves' results now
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) store4<T>(dst + dt * 16, dq[dt] * a.scale);
-    }
+    for (int dt = 0; dt < DT; ++dt) dq[dt] *= a.scale;
+    x_store_rows<T, DK>(a, (T*)a.dq, a.ldq, q0, kvh, blk * 64 + wave * 16, nrow, dq, smem + wave * x_out_bytes<T, DK>(), lane);
 }
 
 // ---- dk, dv -----------------------------------------------------------------------------------------------------------
@@ -462,79 +475,102 @@ __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int 
         store4<T>((T*)a.dk + (size_t)m * a.ldk + c, sum);
 }
 
-// ---- mass: one workgroup per (utterance, head, 32 keys, range of queries) -----------------------------------------------
-// The 32 keys are operands in the registers of every wave; the waves stream the queries, 16 at a time, straight from memory into
-// registers, the next 16 under way.  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds up its own queries' weights over
-// the whole loop, and the 16 queries of a row of lanes meet only at the end.  16 waves (bf16; 8 in three planes): at 32 x 800
-// queries x 120 keys about one workgroup per CU, whose loads are all in flight together.
-template <typename E> constexpr int x_mass_waves() { return E::PL == 1 ? 16 : 8; }
+// ---- mass: one workgroup per (utterance, head, 16 KT keys, range of queries) --------------------------------------------
+// The keys are operands in the registers of every wave; the waves stream the queries, 16 at a time, through a private LDS ring of two
+// tiles.  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds up its own queries' weights over the whole loop, and the 16
+// queries of a row of lanes meet only at the end.
+#ifndef XNW
+#define XNW 4
+#endif
+#ifndef XMKT
+#define XMKT 4
+#endif
+constexpr int X_MASS_WAVES = XNW;
 
-template <typename E, int DK>
-__global__ __launch_bounds__(64 * x_mass_waves<E>(), E::PL == 1 ? 4 : 2) void xattn_mass_kernel(XArgs a) {
+template <typename E, int DK, int KT>
+__global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs a) {
     typedef typename E::mem T;
-    constexpr int KS = DK / 32, NW = x_mass_waves<E>();
-    __shared__ float red[NW][32];
+    constexpr int KS = DK / 32, NW = X_MASS_WAVES, KB = 16 * KT, NST = E::PL == 1 ? 2 : 1;
+    typedef XTile<E, DK, 16> TQ;
+    typedef XTile<E, DK, KB> TK;
+    constexpr int PER_TILE = TQ::BYTES / 1024 + 1;            // bf16: vector-memory instructions of one tile (its DMA, its lse)
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // keys, then the waves' rings; at the end the sums
     int b, h, blk, split;
     if (!x_decode(a, a.H, b, h, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, q0, lenq);
     x_range(a.cu_k, b, a.Mk, k0, lenk);
-    if (blk * 32 >= lenk) return;
+    if (blk * KB >= lenk) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int kvh = x_query(a, h);                       // h / g
     const int ntiles = (lenq + 15) / 16, per = a.nsplit == 1 ? ntiles : (ntiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * per, t1 = min(t0 + per, ntiles);
-    const T* __restrict__ qb = (const T*)a.q + (size_t)q0 * a.ldq + h * DK + g * 8;
+    const T* __restrict__ qb = (const T*)a.q + (size_t)q0 * a.ldq + h * DK;
     const float* __restrict__ lse = a.lse + (size_t)h * a.Mq + q0;
-    typename std::conditional<E::PL == 1, XFrag<E>, XRaw>::type raw[KS];
-    float l = INFINITY;
-    auto fetch = [&](int qt) __attribute__((always_inline)) {
-        const int q = qt * 16 + i, qc = min(q, lenq - 1);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (E::PL == 1) raw[ks] = x_load<E>(qb + (size_t)qc * a.ldq + ks * 32);
-            else raw[ks] = x_raw(qb + (size_t)qc * a.ldq + ks * 32);
-        }
-        l = lse[qc];
-        if (q >= lenq || !(fabsf(l) < INFINITY)) l = INFINITY;          // no such query: no weight
+    unsigned char* ring = smem + TK::BYTES + wave * NST * TQ::BYTES;
+
+    XFetch<E, DK, KB, 1, NW> fk(a.ldk, wave, lane);
+    fk.fetch((const T*)a.k + (size_t)(k0 + blk * KB) * a.ldk + kvh * DK, a.ldk, lenk - blk * KB, smem, wave, lane);
+    XFetch<E, DK, 16, 1, 1> fq(a.ldq, 0, lane);
+    float l_next = INFINITY;
+    auto fetch = [&](int qt, int st) __attribute__((always_inline)) {
+        fq.fetch(qb + (size_t)qt * 16 * a.ldq, a.ldq, lenq - qt * 16, ring + st * TQ::BYTES, 0, lane);
+        l_next = lse[min(qt * 16 + i, lenq - 1)];
     };
-    if (t0 + wave < t1) fetch(t0 + wave);
-    XFrag<E> kf[KS][2];
+    fk.put(smem, wave, lane);
+    vm_wait_barrier<0>();
+    XFrag<E> kf[KS][KT];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-            kf[ks][kt] = x_load<E>((const T*)a.k + (size_t)(k0 + min(blk * 32 + kt * 16 + i, lenk - 1)) * a.ldk + kvh * DK + ks * 32 + g * 8);
-    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (int kt = 0; kt < KT; ++kt) kf[ks][kt] = TK::template row_frag<1>(smem, kt * 16 + i, ks, g);
+    if (t0 + wave < t1) fetch(t0 + wave, 0);
+    f32x4 acc[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) acc[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    int st = 0;
     for (int qt = t0 + wave; qt < t1; qt += NW) {
-        XFrag<E> qf[KS];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (E::PL == 1) qf[ks] = raw[ks];
-            else qf[ks] = x_split8<true>(raw[ks]);
+        float l = l_next;
+        const unsigned char* Qs = ring + st * TQ::BYTES;
+        if constexpr (E::PL == 1) {
+            if (qt + NW < t1) {
+                fetch(qt + NW, st ^ 1);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER_TILE) : "memory");      // this tile has landed, the next is under way
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            st ^= 1;
+        } else {
+            fq.put(ring, 0, lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (qt + NW < t1) fetch(qt + NW, 0);
         }
-        const float lq = l;
-        if (qt + NW < t1) fetch(qt + NW);
-        f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        if (qt * 16 + i >= lenq || !(fabsf(l) < INFINITY)) l = INFINITY;          // no such query: no weight
+        f32x4 s[KT];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) x_mma<E, 2>(kf[ks], qf[ks], s);
+        for (int kt = 0; kt < KT; ++kt) s[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int ks = 0; ks < KS; ++ks) x_mma<E, KT>(kf[ks], TQ::template row_frag<1>(Qs, i, ks, g), s);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[kt][e] += __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2e, -lq));
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[kt][e] += __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2e, -l));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the tile after next overwrites it
     }
+    __syncthreads();
+    float (*red)[KB] = (float (*)[KB])smem;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float v = row16_sum(acc[kt][e]);
             if (i == 0) red[wave][kt * 16 + 4 * g + e] = v;
         }
     __syncthreads();
-    const int key = blk * 32 + tid;
-    if (tid < 32 && key < lenk) {
+    const int key = blk * KB + tid;
+    if (tid < KB && key < lenk) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += red[w][tid];
@@ -562,15 +598,19 @@ static int x_dkv_split(int B, int max_q, int max_k, int H, int KV, int dtype) {
     const long want = 512 / items, most = dtype == 1 ? tiles / 8 : tiles / 4, n = want < most ? want : most;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
+constexpr int x_mass_kt(int dtype) { return dtype == 1 ? XMKT : 2; }
 static int x_mass_split(int B, int max_q, int max_k, int H, int dtype) {
-    const long items = (long)B * H * ((max_k + 31) / 32), trips = (max_q + 15) / 16 / (dtype == 1 ? 16 : 8);
+    const int kb = 16 * x_mass_kt(dtype);
+    const long items = (long)B * H * ((max_k + kb - 1) / kb), trips = (max_q + 15) / 16 / X_MASS_WAVES;
     if (items >= 192 || trips < 8) return 1;
     const long want = 512 / items, most = trips / 2, n = want < most ? want : most;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
 
 template <typename E, int DK, bool DROP> static void launch_xattn_dq(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int lds = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_dq_kb<E, DK>()>::BYTES;
+    constexpr int tiles = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_dq_kb<E, DK>()>::BYTES + (E::PL == 1 ? 4 * XTile<E, DK, 16>::BYTES : 0);
+    constexpr int out = 4 * x_out_bytes<typename E::mem, DK>(), lds = tiles > out ? tiles : out;
+    static_assert(E::PL == 1 || lds >= 4 * XTile<E, DK, 16>::BYTES, "room for the rows");
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_dq_kernel<E, DK, DROP>, lds, &ok);
     hipLaunchKernelGGL((xattn_dq_kernel<E, DK, DROP>), grid, dim3(256), lds, stream, a);
@@ -622,8 +662,12 @@ static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipSt
 
 template <typename E, int DK>
 static int launch_xattn_mass(XArgs& a, int B, int max_k, hipStream_t stream) {
-    const dim3 grid = fs2_x_grid(a, (max_k + 31) / 32, a.H, B);
-    hipLaunchKernelGGL((xattn_mass_kernel<E, DK>), grid, dim3(64 * x_mass_waves<E>()), 0, stream, a);
+    constexpr int KT = x_mass_kt(E::PL == 1);
+    constexpr int lds = XTile<E, DK, 16 * KT>::BYTES + X_MASS_WAVES * (E::PL == 1 ? 2 : 1) * XTile<E, DK, 16>::BYTES;
+    static unsigned long long ok = 0;
+    fs2_allow_lds((const void*)xattn_mass_kernel<E, DK, KT>, lds, &ok);
+    const dim3 grid = fs2_x_grid(a, (max_k + 16 * KT - 1) / (16 * KT), a.H, B);
+    hipLaunchKernelGGL((xattn_mass_kernel<E, DK, KT>), grid, dim3(64 * X_MASS_WAVES), lds, stream, a);
     FS2_CHECK_LAUNCH("fs2_cross_attention_mass");
     if (a.nsplit > 1) {
         const long long n = (long long)a.H * a.Mk;
