@@ -161,38 +161,41 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_pack(const f32x4& lo
 }
 
 // ---- tiles of ROWS rows x DK in LDS ---------------------------------------------------------------------------------
-// One plane of bf16 rows (three for XF32), unpadded, their 16-byte slots rotated by ROT * (row >> RSH) so that fragment reads of 16
-// rows and transposed reads of 4 rows x 64 bytes spread over the banks; rows narrower than 256 bytes share a rotation where several
-// of them make up one pass over the banks.
-template <typename E, int DK, int ROWS = 64> struct XTile {
+// Fragment reads take one 16-byte slot of 16 rows, transposed reads 32 bytes of 8 rows at a time; both should meet all 64 banks once.
+//   XB16 (filled by LDS-DMA, lane-linear): unpadded rows whose slots are rotated by WAY * (row >> RSH); rows narrower than 256 bytes
+//         share a rotation where several of them make up one pass over the banks.
+//   XF32 (three planes, written by ds_write): rows padded to an odd number of slots (WAY 1, read row-wise) or to 2 more than the
+//         slots (WAY 2, read transposed, or both ways).  dk = 96 rotated like XB16 spent 54 % of its LDS cycles on conflicts.
+template <typename E, int DK, int ROWS, int WAY> struct XTile {
     typedef typename E::mem T;
     typedef XFrag<E> frag_t;
-    static constexpr int ROWB = DK * 2;
-    static constexpr int NS = ROWB / 16;
+    static constexpr int NS = DK / 8;                                                   // slots of a row
+    static constexpr int ROWB = E::PL == 1 ? DK * 2 : (WAY == 1 ? (NS | 1) : NS + 2) * 16;
     static constexpr int PLANE = ROWS * ROWB;
     static constexpr int BYTES = E::PL * PLANE;
     static constexpr int KS = DK / 32;
     static constexpr int DT = DK / 16;
-    static constexpr int RSH = ROWB == 128 ? 1 : (ROWB == 64 ? 2 : 0);
+    static constexpr int RSH = DK == 64 ? 1 : (DK == 32 ? 2 : 0);
 
-    template <int ROT> static __device__ __forceinline__ int rot(int row) { return (ROT * (row >> RSH)) % NS; }
-
+    // byte of logical slot `slot` of row `row`
+    static __device__ __forceinline__ int at(int row, int slot) {
+        if constexpr (E::PL == 1) return row * ROWB + ((slot + WAY * (row >> RSH)) % NS) * 16;
+        return row * ROWB + slot * 16;
+    }
     // row `row`, elements 32 ks + 8 g .. + 7
-    template <int ROT> static __device__ __forceinline__ frag_t row_frag(const unsigned char* img, int row, int ks, int g) {
+    static __device__ __forceinline__ frag_t row_frag(const unsigned char* img, int row, int ks, int g) {
         frag_t f;
-        const unsigned char* at = img + row * ROWB + (((ks * 4 + g) + rot<ROT>(row)) % NS) * 16;
+        const unsigned char* p = img + at(row, ks * 4 + g);
 #pragma unroll
-        for (int pl = 0; pl < E::PL; ++pl) f.p[pl] = *(const bf16x8*)(at + pl * PLANE);
+        for (int pl = 0; pl < E::PL; ++pl) f.p[pl] = *(const bf16x8*)(p + pl * PLANE);
         return f;
     }
     // column 16 dt + i, rows 32 c + {4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3}: the slot map of an accumulator used as operand.
     // Transposed 4 x 16 block reads: lane 4 q + p of a 16-lane group supplies row q, columns 4 p .. 4 p + 3
-    template <int ROT> static __device__ __forceinline__ frag_t col_frag(const unsigned char* img, int c, int dt, int g, int i) {
+    static __device__ __forceinline__ frag_t col_frag(const unsigned char* img, int c, int dt, int g, int i) {
         frag_t f;
-        const int row0 = 32 * c + 4 * g + (i >> 2), row1 = row0 + 16;
-        const int slot = dt * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
-        const unsigned char* p0 = img + row0 * ROWB + ((slot + rot<ROT>(row0)) % NS) * 16 + sub;
-        const unsigned char* p1 = img + row1 * ROWB + ((slot + rot<ROT>(row1)) % NS) * 16 + sub;
+        const int row0 = 32 * c + 4 * g + (i >> 2), slot = dt * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+        const unsigned char *p0 = img + at(row0, slot) + sub, *p1 = img + at(row0 + 16, slot) + sub;
 #pragma unroll
         for (int pl = 0; pl < E::PL; ++pl) {
             const bf16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p0 + pl * PLANE));
@@ -207,32 +210,32 @@ template <typename E, int DK, int ROWS = 64> struct XTile {
     }
 };
 
-// Keys of a tile: 64 where two tiles of K and V (bf16: double-buffered by LDS-DMA) or one in three planes (fp32: loaded ahead into
-// registers, split on the way into LDS) leave room for two workgroups on a CU, else 32.
-template <typename E, int DK> constexpr int x_kb() { return E::PL == 3 && DK == 128 ? 32 : 64; }
+// Keys of a tile: bf16 64, two stages filled by LDS-DMA; fp32 32, one stage in three planes, the next tile loaded ahead into registers
+// and split on the way into LDS (64 would leave room for one workgroup on a CU, and for too few registers).
+template <typename E> constexpr int x_kb() { return E::PL == 3 ? 32 : 64; }
 
 // ---- memory -> tile, by NW waves ---------------------------------------------------------------------------------------
 // fetch() starts the rows [0, left) at `tile` (clamped to the last of them), put() finishes.  Sources are 32-bit byte offsets from the
 // tile's first row, clamped by min() (of offsets in one column: the offset of the smaller row).
 //   XB16: fetch is LDS-DMA (16 bytes a lane, lane-linear on the LDS side: the rotation goes into the source), put nothing; the caller
-//         waits vmcnt(0).  Power-of-two rows: the swizzle repeats every (NS << RSH) / ROT rows, a wave needs one period's offsets.
+//         waits vmcnt(0).  Power-of-two rows: the swizzle repeats every (NS << RSH) / WAY rows, a wave needs one period's offsets.
 //   XF32: fetch loads into registers (32 bytes a lane and 16-byte slot), put splits them and writes the three planes.
 // Packed rows of the g > 1 query heads of a shared head (`rows`): the address is worked out row by row.
-template <typename E, int DK, int ROWS, int ROT, int NW> struct XFetch;
+template <typename E, int DK, int ROWS, int WAY, int NW> struct XFetch;
 
-template <int DK, int ROWS, int ROT, int NW> struct XFetch<XB16, DK, ROWS, ROT, NW> {
-    typedef XTile<XB16, DK, ROWS> TL;
+template <int DK, int ROWS, int WAY, int NW> struct XFetch<XB16, DK, ROWS, WAY, NW> {
+    typedef XTile<XB16, DK, ROWS, WAY> TL;
     static constexpr int PIECES = TL::BYTES / 1024, PP = PIECES / NW, NS = TL::NS, ROWB = TL::ROWB;
     static_assert(PIECES % NW == 0, "the same number of pieces for every wave");
     static constexpr bool POW2 = (NS & (NS - 1)) == 0;
-    static constexpr int STEP = NW * 1024 / ROWB, PERIOD = (NS << TL::RSH) / ROT;          // rows between a wave's pieces
+    static constexpr int STEP = NW * 1024 / ROWB, PERIOD = (NS << TL::RSH) / WAY;          // rows between a wave's pieces
     static constexpr int N = !POW2 ? PP : (PERIOD <= STEP ? 1 : (PERIOD / STEP < PP ? PERIOD / STEP : PP));
     unsigned off[N], col[N];
     __device__ __forceinline__ XFetch(int ld, int wave, int lane) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int o = (wave + NW * n) * 1024 + lane * 16, row = o / ROWB, slot = (o % ROWB) >> 4;
-            col[n] = (unsigned)((slot + NS - TL::template rot<ROT>(row)) % NS) * 16u;       // physical slot `slot` holds this one
+            col[n] = (unsigned)((slot + WAY * NS - (WAY * (row >> TL::RSH)) % NS) % NS) * 16u;       // physical slot `slot` holds this one
             off[n] = (unsigned)row * (unsigned)ld * 2u + col[n];
         }
     }
@@ -251,7 +254,7 @@ template <int DK, int ROWS, int ROT, int NW> struct XFetch<XB16, DK, ROWS, ROT, 
         for (int pp = 0; pp < PP; ++pp) {
             const int p = wave + NW * pp, o = p * 1024 + lane * 16, row = o / ROWB, slot = (o % ROWB) >> 4;
             const int r = min(first + row, nrow - 1), q = x_query(a, r);
-            const int s = (slot + NS - TL::template rot<ROT>(row)) % NS;
+            const int s = (slot + WAY * NS - (WAY * (row >> TL::RSH)) % NS) % NS;
             __builtin_amdgcn_global_load_lds((x_gbl_void*)(base + (size_t)q * ld + (r - q * a.g) * DK + s * 8), (x_lds_void*)(dst + p * 1024),
                                              16, 0, 0);
         }
@@ -259,8 +262,8 @@ template <int DK, int ROWS, int ROT, int NW> struct XFetch<XB16, DK, ROWS, ROT, 
     __device__ __forceinline__ void put(unsigned char*, int, int) {}
 };
 
-template <int DK, int ROWS, int ROT, int NW> struct XFetch<XF32, DK, ROWS, ROT, NW> {
-    typedef XTile<XF32, DK, ROWS> TL;
+template <int DK, int ROWS, int WAY, int NW> struct XFetch<XF32, DK, ROWS, WAY, NW> {
+    typedef XTile<XF32, DK, ROWS, WAY> TL;
     static constexpr int CPR = DK / 4, CHUNKS = ROWS * CPR;                     // 16-byte chunks of a row, of the tile
     static constexpr int N = (CHUNKS + 64 * NW - 1) / (64 * NW);                // of a lane (the last of them may be missing)
     static __device__ __forceinline__ bool has(int id) { return CHUNKS % (64 * NW) == 0 || id < CHUNKS; }
@@ -291,18 +294,18 @@ template <int DK, int ROWS, int ROT, int NW> struct XFetch<XF32, DK, ROWS, ROT, 
             uint2 w[3];
             x_split2<true>(r[n][0], r[n][1], w[0].x, w[1].x, w[2].x);
             x_split2<true>(r[n][2], r[n][3], w[0].y, w[1].y, w[2].y);
-            unsigned char* at = dst + row * TL::ROWB + (((c >> 1) + TL::template rot<ROT>(row)) % TL::NS) * 16 + (c & 1) * 8;
+            unsigned char* at = dst + TL::at(row, c >> 1) + (c & 1) * 8;
 #pragma unroll
             for (int pl = 0; pl < 3; ++pl) *(uint2*)(at + pl * TL::PLANE) = w[pl];
         }
     }
 };
 
-// A wave's own packed rows [first, first + ROWS) of the heads at `base` as operands, through its own LDS (XTile<E, DK, ROWS>::BYTES):
+// A wave's own packed rows [first, first + ROWS) of the heads at `base` as operands, through its own LDS (XTile<E, DK, ROWS, 1>::BYTES):
 // a fragment load straight from memory has 16 rows in consecutive lanes, one cache access per lane instead of one per line (64
 // against 8 at dk = 128; the attention mass of 32 x 800 queries spent 9 us of cache accesses that way).  start(), then finish().
 template <typename E, int DK, int ROWS> struct XRows {
-    typedef XTile<E, DK, ROWS> TL;
+    typedef XTile<E, DK, ROWS, 1> TL;
     XFetch<E, DK, ROWS, 1, 1> f;
     __device__ __forceinline__ XRows(int ld, int lane) : f(ld, 0, lane) {}
     __device__ __forceinline__ void start(const XArgs& a, const typename E::mem* __restrict__ base, int ld, int first, int nrow,

@@ -28,11 +28,12 @@ __device__ __forceinline__ void x_zero_rows(const XArgs& a, int q0, int kvh, int
 template <typename E, int DK, int QT, bool DROP>
 __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
     typedef typename E::mem T;
-    constexpr int KB = x_kb<E, DK>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
-    typedef XTile<E, DK, KB> TL;
-    typedef typename TL::frag_t frag_t;
-    constexpr int KS = TL::KS, DT = TL::DT, BQ = 64 * QT;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile, V tile at s * 2 * BYTES
+    constexpr int KB = x_kb<E>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
+    typedef XTile<E, DK, KB, 1> TK;
+    typedef XTile<E, DK, KB, 2> TV;
+    typedef typename TK::frag_t frag_t;
+    constexpr int KS = TK::KS, DT = TK::DT, BQ = 64 * QT, STAGE = TK::BYTES + TV::BYTES;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile, V tile
 
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
@@ -65,9 +66,9 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
     XFetch<E, DK, KB, 1, 4> fk(a.ldk, wave, lane);
     XFetch<E, DK, KB, 2, 4> fv(a.ldv, wave, lane);
     auto fetch = [&](int kt, int st) __attribute__((always_inline)) {
-        unsigned char* d = smem + st * 2 * TL::BYTES;
+        unsigned char* d = smem + st * STAGE;
         fk.fetch(kb + (size_t)kt * KB * a.ldk, a.ldk, lenk - kt * KB, d, wave, lane);
-        fv.fetch(vb + (size_t)kt * KB * a.ldv, a.ldv, lenk - kt * KB, d + TL::BYTES, wave, lane);
+        fv.fetch(vb + (size_t)kt * KB * a.ldv, a.ldv, lenk - kt * KB, d + TK::BYTES, wave, lane);
     };
     fetch(t0, 0);
 
@@ -75,15 +76,15 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
     // behind which that memory is filled again
     frag_t qf[QT][KS];
     {
-        typedef XTile<E, DK, 16 * QT> TQ;
-        unsigned char* own = smem + (NST == 2 ? 2 * TL::BYTES : 0) + wave * TQ::BYTES;
+        typedef XTile<E, DK, 16 * QT, 1> TQ;
+        unsigned char* own = smem + (NST == 2 ? STAGE : 0) + wave * TQ::BYTES;
         XRows<E, DK, 16 * QT> rows(a.ldq, lane);
         rows.start(a, (const T*)a.q + (size_t)q0 * a.ldq + kvh * a.g * DK, a.ldq, min(blk * BQ + wave * 16 * QT, nrow - 1), nrow, own, lane);
         rows.finish(own, lane);
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) qf[t][ks] = TQ::template row_frag<1>(own, t * 16 + i, ks, g);
+            for (int ks = 0; ks < KS; ++ks) qf[t][ks] = TQ::row_frag(own, t * 16 + i, ks, g);
     }
 
     f32x4 o[QT][DT];
@@ -97,8 +98,8 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
     }
     for (int kt = t0; kt < t1; ++kt) {
         const int st = NST == 2 ? (kt - t0) & 1 : 0;
-        unsigned char* Ks = smem + st * 2 * TL::BYTES;
-        unsigned char* Vs = Ks + TL::BYTES;
+        unsigned char* Ks = smem + st * STAGE;
+        unsigned char* Vs = Ks + TK::BYTES;
         if constexpr (E::PL == 1) {
             vm_wait_barrier<0>();         // tile kt has landed; every wave is done with the other stage
         } else {
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
         for (int ks = 0; ks < KS; ++ks) {
             frag_t kf[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) kf[nt] = TL::template row_frag<1>(Ks, nt * 16 + i, ks, g);
+            for (int nt = 0; nt < NT; ++nt) kf[nt] = TK::row_frag(Ks, nt * 16 + i, ks, g);
 #pragma unroll
             for (int t = 0; t < QT; ++t) x_mma<E, NT>(kf, qf[t][ks], s[t]);
         }
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
         frag_t vf[E::PL == 1 ? NC : 1][DT];
         if constexpr (E::PL == 1) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) vf[0][dt] = TL::template col_frag<2>(Vs, 0, dt, g, i);
+            for (int dt = 0; dt < DT; ++dt) vf[0][dt] = TV::col_frag(Vs, 0, dt, g, i);
             __builtin_amdgcn_sched_barrier(0);
         }
         const int kbase = kt * KB + 4 * g;
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
 #pragma unroll
             for (int c = 1; c < NC; ++c)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) vf[c][dt] = TL::template col_frag<2>(Vs, c, dt, g, i);
+                for (int dt = 0; dt < DT; ++dt) vf[c][dt] = TV::col_frag(Vs, c, dt, g, i);
             if (kt + 1 < t1) fetch(kt + 1, st ^ 1);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
                 for (int dt0 = 0; dt0 < DT; dt0 += 2) {
                     frag_t v2[2];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) v2[u] = TL::template col_frag<2>(Vs, c, dt0 + u, g, i);
+                    for (int u = 0; u < 2; ++u) v2[u] = TV::col_frag(Vs, c, dt0 + u, g, i);
 #pragma unroll
                     for (int t = 0; t < QT; ++t) x_mma<E, 2>(v2, pf[t], &o[t][dt0]);
                 }
@@ -241,9 +242,10 @@ __global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
 template <typename E, int DK>
 __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
     typedef typename E::mem T;
-    typedef XTile<E, DK, 32> TL;
-    typedef typename TL::frag_t frag_t;
-    constexpr int KS = TL::KS, DT = TL::DT;
+    typedef XTile<E, DK, 32, 1> TK;
+    typedef XTile<E, DK, 32, 2> TV;
+    typedef typename TK::frag_t frag_t;
+    constexpr int KS = TK::KS, DT = TK::DT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // wave w: V tile at w * BYTES; then the merge
     const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     int q0, lenq, k0, lenk;
@@ -267,8 +269,8 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
 
     const T* __restrict__ kb = (const T*)a.k + (size_t)k0 * a.ldk + kvh * DK;
     const T* __restrict__ vb = (const T*)a.v + (size_t)k0 * a.ldv + kvh * DK;
-    constexpr int KL = E::PL == 1 ? TL::BYTES : 0;          // K goes through LDS too (fp32: three planes of both do not fit)
-    unsigned char* Ks = smem + wave * (TL::BYTES + KL);
+    constexpr int KL = E::PL == 1 ? TK::BYTES : 0;          // K goes through LDS too (fp32: three planes of both do not fit)
+    unsigned char* Ks = smem + wave * (TV::BYTES + KL);
     unsigned char* Vs = Ks + KL;
     XFetch<E, DK, 32, 1, 1> fk(a.ldk, 0, lane);
     XFetch<E, DK, 32, 2, 1> fv(a.ldv, 0, lane);
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
             frag_t f[2];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
-                if constexpr (E::PL == 1) f[nt] = TL::template row_frag<1>(Ks, nt * 16 + i, ks, g);
+                if constexpr (E::PL == 1) f[nt] = TK::row_frag(Ks, nt * 16 + i, ks, g);
                 else f[nt] = x_load<E>(kb + (size_t)min(kt * 32 + nt * 16 + i, lenk - 1) * a.ldk + ks * 32 + g * 8);
             }
             x_mma<E, 2>(f, qf[ks], s);
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
             frag_t v2[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                v2[u] = TL::template col_frag<2>(Vs, 0, dt0 + u, g, i);
+                v2[u] = TV::col_frag(Vs, 0, dt0 + u, g, i);
                 o[dt0 + u] = o[dt0 + u] * alpha;
             }
             x_mma<E, 2>(v2, pf, &o[dt0]);
@@ -425,10 +427,11 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dk, int dtyp
             p.nsplit = (int)(want < most ? want : most);
         }
     } else {
-        p.qt = dtype == 1 && rows > 64 ? 2 : 1;
-        const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = (max_k + 63) / 64;
-        if (items < 256 && tiles >= 4) {
-            const long want = 512 / items, most = tiles / 2;
+        p.qt = rows > 64 && !(dtype == 0 && dk == 128) ? 2 : 1;        // (two row tiles of dk = 128 in three planes spill 42 registers)
+        const int kb = dtype == 1 ? 64 : 32, fill = dtype == 1 ? 256 : 384;
+        const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = (max_k + kb - 1) / kb;
+        if (items < fill && tiles >= 4) {
+            const long want = 512 / items, most = tiles / (128 / kb);
             p.nsplit = (int)(want < most ? want : most);
         }
     }
@@ -438,9 +441,9 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dk, int dtyp
 }
 
 template <typename E, int DK, int QT, bool DROP> static void launch_xattn_rows(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int tiles = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_kb<E, DK>()>::BYTES, out = 4 * x_out_bytes<float, DK>();
-    constexpr int lds = tiles > out ? tiles : out;
-    static_assert(lds >= 4 * XTile<E, DK, 16 * QT>::BYTES + (E::PL == 1 ? 2 * XTile<E, DK, 64>::BYTES : 0), "room for the queries");
+    constexpr int KB = x_kb<E>(), stage = XTile<E, DK, KB, 1>::BYTES + XTile<E, DK, KB, 2>::BYTES;
+    constexpr int rows = 4 * XTile<E, DK, 16 * QT, 1>::BYTES, out = 4 * x_out_bytes<float, DK>();
+    constexpr int tiles = E::PL == 1 ? stage + (stage > rows ? stage : rows) : (stage > rows ? stage : rows), lds = tiles > out ? tiles : out;
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_rows_kernel<E, DK, QT, DROP>, lds, &ok);
     hipLaunchKernelGGL((xattn_rows_kernel<E, DK, QT, DROP>), grid, dim3(256), lds, stream, a);
@@ -450,7 +453,7 @@ template <typename E, int DK>
 static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipStream_t stream) {
     typedef typename E::mem T;
     if (p.few) {
-        constexpr int merge = 4 * 16 * DK * 4 + 512, tiles = (E::PL == 1 ? 8 : 4) * XTile<E, DK, 32>::BYTES;
+        constexpr int merge = 4 * 16 * DK * 4 + 512, tiles = 4 * (XTile<E, DK, 32, 2>::BYTES + (E::PL == 1 ? XTile<E, DK, 32, 1>::BYTES : 0));
         constexpr int lds = merge > tiles ? merge : tiles;
         static unsigned long long ok = 0;
         fs2_allow_lds((const void*)xattn_few_kernel<E, DK>, lds, &ok);
@@ -459,7 +462,7 @@ static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipS
         const int rows = max_q * a.g, nblk = (rows + 64 * p.qt - 1) / (64 * p.qt);
         const dim3 grid = fs2_x_grid(a, nblk, a.KV, B);
         if (p.qt == 2) {
-            if constexpr (E::PL == 1) {
+            if constexpr (E::PL == 1 || DK < 128) {
                 if (a.drop.thresh) launch_xattn_rows<E, DK, 2, true>(a, grid, stream);
                 else launch_xattn_rows<E, DK, 2, false>(a, grid, stream);
             }

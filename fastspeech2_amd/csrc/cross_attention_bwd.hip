@@ -14,17 +14,15 @@
 namespace fs2 {
 
 // ---- dq and delta: one workgroup per (utterance, shared head, 64 packed rows) -------------------------------------
-// (64-key tiles of dk = 96 in three planes need 37 registers more than there are)
-template <typename E, int DK> constexpr int x_dq_kb() { return E::PL == 3 && DK >= 96 ? 32 : 64; }
-
 template <typename E, int DK, bool DROP>
 __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     typedef typename E::mem T;
-    constexpr int KB = x_dq_kb<E, DK>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
-    typedef XTile<E, DK, KB> TL;
-    typedef typename TL::frag_t frag_t;
-    constexpr int KS = TL::KS, DT = TL::DT;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile (rotation 2), V tile (rotation 1)
+    constexpr int KB = x_kb<E>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
+    typedef XTile<E, DK, KB, 2> TK;
+    typedef XTile<E, DK, KB, 1> TV;
+    typedef typename TK::frag_t frag_t;
+    constexpr int KS = TK::KS, DT = TK::DT, STAGE = TK::BYTES + TV::BYTES;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile (read both ways), V tile
 
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
@@ -45,9 +43,9 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     XFetch<E, DK, KB, 2, 4> fk(a.ldk, wave, lane);
     XFetch<E, DK, KB, 1, 4> fv(a.ldv, wave, lane);
     auto fetch = [&](int kt, int st) __attribute__((always_inline)) {
-        unsigned char* d = smem + st * 2 * TL::BYTES;
+        unsigned char* d = smem + st * STAGE;
         fk.fetch(kb + (size_t)kt * KB * a.ldk, a.ldk, lenk - kt * KB, d, wave, lane);
-        fv.fetch(vb + (size_t)kt * KB * a.ldv, a.ldv, lenk - kt * KB, d + TL::BYTES, wave, lane);
+        fv.fetch(vb + (size_t)kt * KB * a.ldv, a.ldv, lenk - kt * KB, d + TK::BYTES, wave, lane);
     };
     if (lenk > 0) fetch(0, 0);
 
@@ -55,8 +53,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     frag_t qf[KS], dof[KS];
     float del = 0.f;
     {
-        typedef XTile<E, DK, 16> TQ;
-        unsigned char* own = smem + (NST == 2 ? 2 * TL::BYTES : 0) + wave * TQ::BYTES;
+        typedef XTile<E, DK, 16, 1> TQ;
+        unsigned char* own = smem + (NST == 2 ? STAGE : 0) + wave * TQ::BYTES;
         constexpr int NEXT = E::PL == 1 ? 4 * TQ::BYTES : 0;
         const int first = min(blk * 64 + wave * 16, nrow - 1);
         const size_t at = (size_t)q0 * a.ldq + kvh * a.g * DK, ato = (size_t)q0 * a.ldo + kvh * a.g * DK;
@@ -66,20 +64,20 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
         rc.start(a, (const T*)a.ctx + ato, a.ldo, first, nrow, own + 2 * NEXT, lane);
         rq.finish(own, lane);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qf[ks] = TQ::template row_frag<1>(own, i, ks, g);
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = TQ::row_frag(own, i, ks, g);
         if constexpr (E::PL == 3) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             rd.finish(own, lane);
         }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) dof[ks] = TQ::template row_frag<1>(own + NEXT, i, ks, g);
+        for (int ks = 0; ks < KS; ++ks) dof[ks] = TQ::row_frag(own + NEXT, i, ks, g);
         if constexpr (E::PL == 3) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             rc.finish(own, lane);
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const frag_t of = TQ::template row_frag<1>(own + 2 * NEXT, i, ks, g);
+            const frag_t of = TQ::row_frag(own + 2 * NEXT, i, ks, g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) del = fmaf(x_value<E>(dof[ks], j), x_value<E>(of, j), del);
         }
@@ -96,8 +94,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     const int ntiles = (lenk + KB - 1) / KB;
     for (int kt = 0; kt < ntiles; ++kt) {
         const int st = NST == 2 ? kt & 1 : 0;
-        unsigned char* Ks = smem + st * 2 * TL::BYTES;
-        unsigned char* Vs = Ks + TL::BYTES;
+        unsigned char* Ks = smem + st * STAGE;
+        unsigned char* Vs = Ks + TK::BYTES;
         if constexpr (E::PL == 1) {
             vm_wait_barrier<0>();      // tile kt has landed; every wave is done with the other stage
         } else {
@@ -114,10 +112,10 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
         for (int ks = 0; ks < KS; ++ks) {
             frag_t kf[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) kf[nt] = TL::template row_frag<2>(Ks, nt * 16 + i, ks, g);
+            for (int nt = 0; nt < NT; ++nt) kf[nt] = TK::row_frag(Ks, nt * 16 + i, ks, g);
             x_mma<E, NT>(kf, qf[ks], s);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) kf[nt] = TL::template row_frag<1>(Vs, nt * 16 + i, ks, g);
+            for (int nt = 0; nt < NT; ++nt) kf[nt] = TV::row_frag(Vs, nt * 16 + i, ks, g);
             x_mma<E, NT>(kf, dof[ks], dp);
         }
         // bf16: K^T fragments before the next tile's DMA (no transposed LDS read passes one), under the arithmetic
@@ -126,7 +124,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) kc[c][dt] = TL::template col_frag<2>(Ks, c, dt, g, i);
+                for (int dt = 0; dt < DT; ++dt) kc[c][dt] = TK::col_frag(Ks, c, dt, g, i);
             __builtin_amdgcn_sched_barrier(0);
             if (kt + 1 < ntiles) fetch(kt + 1, st ^ 1);
         }
@@ -157,7 +155,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
                 for (int dt0 = 0; dt0 < DT; dt0 += 2) {
                     frag_t k2[2];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) k2[u] = TL::template col_frag<2>(Ks, c, dt0 + u, g, i);
+                    for (int u = 0; u < 2; ++u) k2[u] = TK::col_frag(Ks, c, dt0 + u, g, i);
                     x_mma<E, 2>(k2, dsf, &dq[dt0]);
                 }
             }
@@ -176,10 +174,10 @@ template <int DK, bool DROP>
 __global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs a) {
     typedef XF32 E;
     typedef float T;
-    typedef XTile<E, DK, 32> TL;
+    typedef XTile<E, DK, 32, 2> TL;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // Q tile, dO tile (rotation 2), 32 lse, 32 delta
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // Q tile, dO tile (read both ways), 32 lse, 32 delta
 
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
@@ -231,10 +229,10 @@ __global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs
         for (int ks = 0; ks < KS; ++ks) {
             frag_t f[2];
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) f[rt] = TL::template row_frag<2>(Qs, rt * 16 + i, ks, g);
+            for (int rt = 0; rt < 2; ++rt) f[rt] = TL::row_frag(Qs, rt * 16 + i, ks, g);
             x_mma<E, 2>(f, kf[ks], s);               // rows: packed rows qt 32 + 16 rt + 4 g + e, column: key i
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) f[rt] = TL::template row_frag<2>(Ds, rt * 16 + i, ks, g);
+            for (int rt = 0; rt < 2; ++rt) f[rt] = TL::row_frag(Ds, rt * 16 + i, ks, g);
             x_mma<E, 2>(f, vf[ks], dp);
         }
 #pragma unroll
@@ -261,10 +259,10 @@ __global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs
         for (int dt0 = 0; dt0 < DT; dt0 += 2) {
             frag_t f[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) f[u] = TL::template col_frag<2>(Ds, 0, dt0 + u, g, i);
+            for (int u = 0; u < 2; ++u) f[u] = TL::col_frag(Ds, 0, dt0 + u, g, i);
             x_mma<E, 2>(f, pf, &dv_[dt0]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) f[u] = TL::template col_frag<2>(Qs, 0, dt0 + u, g, i);
+            for (int u = 0; u < 2; ++u) f[u] = TL::col_frag(Qs, 0, dt0 + u, g, i);
             x_mma<E, 2>(f, dsf, &dk_[dt0]);
         }
     }
@@ -297,13 +295,13 @@ template <int DK, int KT, bool DROP>
 __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
     typedef XB16 E;
     typedef bf16_t T;
-    typedef XTile<E, DK, 32> TL;
+    typedef XTile<E, DK, 32, 2> TL;
     constexpr int KB = 16 * KT;
-    typedef XTile<E, DK, KB> TK;
+    typedef XTile<E, DK, KB, 1> TK;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT, NP = TK::BYTES / 1024, NWK = NP % 4 == 0 ? 4 : (NP % 2 == 0 ? 2 : 1);
     constexpr int WAVE = 2 * TL::BYTES;                  // a wave's Q tile, dO tile: 80 KB in all at dk = 128, two workgroups per CU
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // K tile, V tile (rotation 1), then the waves'
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // K tile, V tile, then the waves'
 
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
@@ -362,17 +360,17 @@ __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
         for (int ks = 0; ks < KS; ++ks) {
             frag_t rf[2], kf[KT];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) rf[u] = TL::template row_frag<2>(Qs, u * 16 + i, ks, g);
+            for (int u = 0; u < 2; ++u) rf[u] = TL::row_frag(Qs, u * 16 + i, ks, g);
 #pragma unroll
-            for (int u = 0; u < KT; ++u) kf[u] = TK::template row_frag<1>(Ks, u * 16 + i, ks, g);
+            for (int u = 0; u < KT; ++u) kf[u] = TK::row_frag(Ks, u * 16 + i, ks, g);
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) s[rt][kt] = mma16(rf[rt].p[0], kf[kt].p[0], s[rt][kt]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) rf[u] = TL::template row_frag<2>(Ds, u * 16 + i, ks, g);
+            for (int u = 0; u < 2; ++u) rf[u] = TL::row_frag(Ds, u * 16 + i, ks, g);
 #pragma unroll
-            for (int u = 0; u < KT; ++u) kf[u] = TK::template row_frag<1>(Vs, u * 16 + i, ks, g);
+            for (int u = 0; u < KT; ++u) kf[u] = TK::row_frag(Vs, u * 16 + i, ks, g);
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
@@ -412,13 +410,13 @@ __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            const frag_t dot = TL::template col_frag<2>(Ds, 0, dt, g, i);
+            const frag_t dot = TL::col_frag(Ds, 0, dt, g, i);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) dv_[dt][kt] = mma16(dot.p[0], pf[kt].p[0], dv_[dt][kt]);
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            const frag_t qtr = TL::template col_frag<2>(Qs, 0, dt, g, i);
+            const frag_t qtr = TL::col_frag(Qs, 0, dt, g, i);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) dk_[dt][kt] = mma16(qtr.p[0], dsf[kt].p[0], dk_[dt][kt]);
         }
@@ -491,8 +489,8 @@ template <typename E, int DK, int KT>
 __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs a) {
     typedef typename E::mem T;
     constexpr int KS = DK / 32, NW = X_MASS_WAVES, KB = 16 * KT, NST = E::PL == 1 ? 2 : 1;
-    typedef XTile<E, DK, 16> TQ;
-    typedef XTile<E, DK, KB> TK;
+    typedef XTile<E, DK, 16, 1> TQ;
+    typedef XTile<E, DK, KB, 1> TK;
     constexpr int PER_TILE = TQ::BYTES / 1024 + 1;            // bf16: vector-memory instructions of one tile (its DMA, its lse)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // keys, then the waves' rings; at the end the sums
     int b, h, blk, split;
@@ -525,7 +523,7 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) kf[ks][kt] = TK::template row_frag<1>(smem, kt * 16 + i, ks, g);
+        for (int kt = 0; kt < KT; ++kt) kf[ks][kt] = TK::row_frag(smem, kt * 16 + i, ks, g);
     if (t0 + wave < t1) fetch(t0 + wave, 0);
     f32x4 acc[KT];
 #pragma unroll
@@ -552,7 +550,7 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) s[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) x_mma<E, KT>(kf[ks], TQ::template row_frag<1>(Qs, i, ks, g), s);
+        for (int ks = 0; ks < KS; ++ks) x_mma<E, KT>(kf[ks], TQ::row_frag(Qs, i, ks, g), s);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -608,21 +606,21 @@ static int x_mass_split(int B, int max_q, int max_k, int H, int dtype) {
 }
 
 template <typename E, int DK, bool DROP> static void launch_xattn_dq(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int tiles = (E::PL == 1 ? 4 : 2) * XTile<E, DK, x_dq_kb<E, DK>()>::BYTES + (E::PL == 1 ? 4 * XTile<E, DK, 16>::BYTES : 0);
-    constexpr int out = 4 * x_out_bytes<typename E::mem, DK>(), lds = tiles > out ? tiles : out;
-    static_assert(E::PL == 1 || lds >= 4 * XTile<E, DK, 16>::BYTES, "room for the rows");
+    constexpr int KB = x_kb<E>(), stage = XTile<E, DK, KB, 1>::BYTES + XTile<E, DK, KB, 2>::BYTES;
+    constexpr int rows = (E::PL == 1 ? 12 : 4) * XTile<E, DK, 16, 1>::BYTES, out = 4 * x_out_bytes<typename E::mem, DK>();
+    constexpr int tiles = E::PL == 1 ? stage + (stage > rows ? stage : rows) : (stage > rows ? stage : rows), lds = tiles > out ? tiles : out;
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_dq_kernel<E, DK, DROP>, lds, &ok);
     hipLaunchKernelGGL((xattn_dq_kernel<E, DK, DROP>), grid, dim3(256), lds, stream, a);
 }
 template <int DK, bool DROP> static void launch_xattn_dkv(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int lds = 2 * XTile<XF32, DK, 32>::BYTES + 256;
+    constexpr int lds = 2 * XTile<XF32, DK, 32, 2>::BYTES + 256;
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_dkv_kernel<DK, DROP>, lds, &ok);
     hipLaunchKernelGGL((xattn_dkv_kernel<DK, DROP>), grid, dim3(256), lds, stream, a);
 }
 template <int DK, int KT, bool DROP> static void launch_xattn_dkv32(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int tiles = 8 * XTile<XB16, DK, 32>::BYTES + 2 * XTile<XB16, DK, 16 * KT>::BYTES, merge = 4 * 16 * KT * (DK + 4) * 4;
+    constexpr int tiles = 8 * XTile<XB16, DK, 32, 2>::BYTES + 2 * XTile<XB16, DK, 16 * KT, 1>::BYTES, merge = 4 * 16 * KT * (DK + 4) * 4;
     constexpr int lds = tiles > merge ? tiles : merge;
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_dkv32_kernel<DK, KT, DROP>, lds, &ok);
@@ -663,7 +661,7 @@ static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipSt
 template <typename E, int DK>
 static int launch_xattn_mass(XArgs& a, int B, int max_k, hipStream_t stream) {
     constexpr int KT = x_mass_kt(E::PL == 1);
-    constexpr int lds = XTile<E, DK, 16 * KT>::BYTES + X_MASS_WAVES * (E::PL == 1 ? 2 : 1) * XTile<E, DK, 16>::BYTES;
+    constexpr int lds = XTile<E, DK, 16 * KT, 1>::BYTES + X_MASS_WAVES * (E::PL == 1 ? 2 : 1) * XTile<E, DK, 16, 1>::BYTES;
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_mass_kernel<E, DK, KT>, lds, &ok);
     const dim3 grid = fs2_x_grid(a, (max_k + 16 * KT - 1) / (16 * KT), a.H, B);
