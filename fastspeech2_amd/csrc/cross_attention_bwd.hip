@@ -150,6 +150,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
             const frag_t dsf = x_pack<E>(s[2 * c], s[2 * c + 1]);
             if constexpr (E::PL == 1) {
                 x_mma<E, DT>(kc[c], dsf, dq);
+                x_mma<E, DT>(kc[c], x_pack_rest(s[2 * c], s[2 * c + 1], dsf), dq);
             } else {
 #pragma unroll
                 for (int dt0 = 0; dt0 < DT; dt0 += 2) {
@@ -401,11 +402,12 @@ __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
                 }
             }
         }
-        frag_t pf[KT], dsf[KT];
+        frag_t pf[KT], dsf[KT], dsr[KT];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
             pf[kt] = x_pack<E>(s[0][kt], s[1][kt]);
             dsf[kt] = x_pack<E>(dp[0][kt], dp[1][kt]);
+            dsr[kt] = x_pack_rest(dp[0][kt], dp[1][kt], dsf[kt]);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -418,7 +420,10 @@ __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
         for (int dt = 0; dt < DT; ++dt) {
             const frag_t qtr = TL::col_frag(Qs, 0, dt, g, i);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) dk_[dt][kt] = mma16(qtr.p[0], dsf[kt].p[0], dk_[dt][kt]);
+            for (int kt = 0; kt < KT; ++kt) {
+                dk_[dt][kt] = mma16(qtr.p[0], dsf[kt].p[0], dk_[dt][kt]);
+                dk_[dt][kt] = mma16(qtr.p[0], dsr[kt].p[0], dk_[dt][kt]);
+            }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next tile's DMA overwrites it
         if (qt + 4 < t1) stage(qt + 4);
