@@ -5,7 +5,12 @@
 //   dx = rstd (dh - mean_g(dh) - xhat mean_g(dh xhat));  dgamma = sum dz xhat,  dbeta = sum dz
 // Unlike BatchNorm (batchnorm.hip) no utterance sees another: a batch row equals the utterance alone.
 //
-// Memory-bound: the floor is one read of the inputs and one write of the output.  A workgroup owns a STRIP of whole groups
+// Memory-bound: the floor is one read of the inputs and one write of the output.  Measured, 32 utterances x 800 rows x 256 channels
+// in 16 groups, tanh: forward fp32 -> bf16 13.9 us for 39 MB (2.8 TB/s); backward 20.0 us for 65 MB (3.3 TB/s), 3.9 of it the sums of
+// dgamma and dbeta; 256 x 800 x 80, bf16 backward: 35.8 us for 97 MB (2.7 TB/s).  What is left: all workgroups read, reduce and
+// write at the same time, so the memory waits while they reduce (of the 34 us of the last, 15 are the read at 4.2 TB/s, 4 the sums,
+// 15 the write), and one branch per vector of values and activation (per value: 16.0, 20.5 + 4, 43 + 5 us).
+// A workgroup owns a STRIP of whole groups
 // (at least GN_STRIP_BYTES of a row) of one utterance and holds its rows in REGISTERS: it reads them once, takes the mean, then
 // the centred squares (two passes over registers, no cancellation), and writes.  An utterance too long for the registers is cut
 // into chunks: a first kernel leaves (mean, centred squares) of every chunk, or the backward's channel sums, a second reads the
@@ -18,7 +23,8 @@ namespace fs2 {
 // utterances of 800 rows, backward sums: 50 us with 512 threads, 27 with 256: the small groups overlap each other's phases).
 constexpr int GN_WHOLE_THREADS = 512, GN_CHUNK_THREADS = 256;
 constexpr int GN_CHUNK_ROWS = 8;          // rows per thread of a chunk
-constexpr int GN_STRIP_BYTES = 64;
+constexpr int GN_HOLD = 4;                // rows per thread in registers at a time, in a chunk
+constexpr int GN_STRIP_BYTES = 64;        // 32 x 800 rows x 256 channels, fp32: forward 16.0 us (128: 18.2), one utterance 9.0 (12.8)
 
 struct GnArgs {
     const void* x;           // [M, ldx]
@@ -30,7 +36,7 @@ struct GnArgs {
     const void* dout;        // [M, ldd]
     void* dx;                // [M, ldg]
     float* part;             // forward chunks: [B][nchunk][G][2] mean, M2; backward: [B][nchunk][2][C] sums of dz, dz xhat
-    int M, C, G, cg, ldx, ldo, ldd, ldg, act, nchunk, nstrip;
+    int M, max_len, C, G, cg, ldx, ldo, ldd, ldg, act, nchunk, nstrip;
     int units;               // B * nchunk
     int W, LX, LY;           // channels of a strip, lanes per row, rows per pass of the workgroup
     float inv_lx, inv_cg;    // 1 / LX, 1 / cg
@@ -50,23 +56,42 @@ __device__ __forceinline__ float gn_tanh(float z) {
 __device__ __forceinline__ float gn_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
 }
-__device__ __forceinline__ float gn_act(float z, int act) {
-    if (act == 1) return z > 0.f ? z : (z == z ? 0.f : z);
-    if (act == 2) return gn_tanh(z);
-    if (act == 3) return z == -INFINITY ? 0.f : z * gn_sigmoid(z);
-    return z;
+// act of V values, or act' times u: one (uniform) branch for the vector
+template <int V> __device__ __forceinline__ void gn_act(int act, float (&z)[V]) {
+    if (act == 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = z[j] > 0.f ? z[j] : (z[j] == z[j] ? 0.f : z[j]);
+    } else if (act == 2) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = gn_tanh(z[j]);
+    } else if (act == 3) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = z[j] == -INFINITY ? 0.f : z[j] * gn_sigmoid(z[j]);
+    }
 }
-__device__ __forceinline__ float gn_slope(float z, int act) {
-    if (act == 1) return z > 0.f ? 1.f : 0.f;
-    if (act == 2) {
-        const float t = gn_tanh(z);
-        return fmaf(-t, t, 1.0f);
+template <int V> __device__ __forceinline__ void gn_slope(int act, const float (&z)[V], float (&u)[V]) {
+    if (act == 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] = z[j] > 0.f ? u[j] : u[j] * 0.f;
+    } else if (act == 2) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float t = gn_tanh(z[j]);
+            u[j] *= fmaf(-t, t, 1.0f);
+        }
+    } else if (act == 3) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float s = gn_sigmoid(z[j]);
+            u[j] *= s * fmaf(z[j], 1.0f - s, 1.0f);
+        }
     }
-    if (act == 3) {
-        const float s = gn_sigmoid(z);
-        return s * fmaf(z, 1.0f - s, 1.0f);
+}
+template <int V> __device__ __forceinline__ void gn_drop(const Dropout& drop, int row, int c0, float (&z)[V]) {
+    if (drop.thresh) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] *= drop_mul(drop, (uint32_t)row, (uint32_t)(c0 + j));
     }
-    return 1.0f;
 }
 
 // ---- V consecutive channels of a row: raw registers and their values ---------------------------------------------------
@@ -128,7 +153,7 @@ template <int V, int R> __device__ __forceinline__ GnPlace gn_place(const GnArgs
     p.chunk = unit % a.nchunk;
     p.b = unit / a.nchunk;
     const int c0 = min(max(a.cu[p.b], 0), a.M), c1 = min(max(a.cu[p.b + 1], c0), a.M);
-    total = c1 - c0;
+    total = min(c1 - c0, a.max_len);
     const int rows = a.LY * R, first = min(p.chunk * rows, total);
     p.r0 = c0 + first;
     p.len = min(total - first, rows);
@@ -249,11 +274,9 @@ __device__ __forceinline__ void gn_write_row(const GnArgs& a, int row, int c0, c
                                              const float (&rg)[V], const float (&be)[V]) {
     float o[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        float z = gn_act(fmaf(x.get(j) - mean[j], rg[j], be[j]), a.act);
-        if (a.drop.thresh) z *= drop_mul(a.drop, (uint32_t)row, (uint32_t)(c0 + j));
-        o[j] = z;
-    }
+    for (int j = 0; j < V; ++j) o[j] = fmaf(x.get(j) - mean[j], rg[j], be[j]);
+    gn_act<V>(a.act, o);
+    gn_drop<V>(a.drop, row, c0, o);
     gn_store<TO, V>((TO*)a.out + (size_t)row * a.ldo + c0, o);
 }
 
@@ -343,8 +366,8 @@ __global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_apply_kernel(GnArgs a) {
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
     if (p.b < 0 || (p.len == 0 && p.chunk > 0)) return;
-    const int g0 = p.strip * (a.W / a.cg), ng = a.W / a.cg, rows = a.LY * R, nch = min((total + rows - 1) / rows, a.nchunk);
-    const float n_all = (float)min(total, a.nchunk * rows) * (float)a.cg;
+    const int g0 = p.strip * (a.W / a.cg), ng = a.W / a.cg, rows = a.LY * R, nch = (total + rows - 1) / rows;
+    const float n_all = (float)total * (float)a.cg;
     for (int t = threadIdx.x; t < ng; t += NT) {
         const float* src = a.part + ((size_t)p.b * a.nchunk * a.G + g0 + t) * 2;
         const size_t step = (size_t)a.G * 2;
@@ -385,12 +408,14 @@ __global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_apply_kernel(GnArgs a) {
 template <typename TD, int V>
 __device__ __forceinline__ void gn_dz(const GnArgs& a, int row, int c0, const GnVec<TD, V>& d, const float (&xh)[V],
                                       const float (&ga)[V], const float (&be)[V], float (&dz)[V]) {
+    float z[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float u = d.get(j);
-        if (a.drop.thresh) u *= drop_mul(a.drop, (uint32_t)row, (uint32_t)(c0 + j));
-        dz[j] = a.act ? u * gn_slope(fmaf(xh[j], ga[j], be[j]), a.act) : u;
+        dz[j] = d.get(j);
+        z[j] = fmaf(xh[j], ga[j], be[j]);
     }
+    gn_drop<V>(a.drop, row, c0, dz);
+    gn_slope<V>(a.act, z, dz);
 }
 
 // mean, rstd, gamma, beta of a lane's channels
@@ -418,10 +443,11 @@ __global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void g
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
     if (p.b < 0) return;
-    constexpr int HOLD = WHOLE ? R : 4;                     // rows in registers at a time
+    constexpr int HOLD = WHOLE ? R : GN_HOLD;                   // rows in registers at a time
     GnVec<TX, V> x[HOLD];
     GnVec<TD, V> d[HOLD];
-    float dz[WHOLE ? R : 1][V];
+    constexpr bool KEEP = WHOLE && (R <= 8 || sizeof(TX) == 4);
+    float dz[KEEP ? R : 1][V];
     const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
     const TD* sd = (const TD*)a.dout + (size_t)p.r0 * a.ldd + p.c0;
     float mean[V], rs[V], ga[V], be[V];
@@ -447,11 +473,11 @@ __global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void g
                 float xh[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) xh[j] = (x[k].get(j) - mean[j]) * rs[j];
-                gn_dz<TD, V>(a, p.r0 + row, p.c0, d[k], xh, ga, be, dz[WHOLE ? k : 0]);
+                gn_dz<TD, V>(a, p.r0 + row, p.c0, d[k], xh, ga, be, dz[KEEP ? k : 0]);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    s0[j] += dz[WHOLE ? k : 0][j];
-                    s1[j] = fmaf(dz[WHOLE ? k : 0][j], xh[j], s1[j]);
+                    s0[j] += dz[KEEP ? k : 0][j];
+                    s1[j] = fmaf(dz[KEEP ? k : 0][j], xh[j], s1[j]);
                 }
             }
         }
@@ -485,17 +511,20 @@ __global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void g
         m2[j] = grp2[gi] * inv_n;
     }
 #pragma unroll
-    for (int k = 0; k < R; ++k) x[k].keep_raw();
+    for (int k = 0; k < R; ++k) {
+        x[k].keep_raw();
+        if (!KEEP) d[k].keep_raw();
+    }
 #pragma unroll
     for (int k = 0; k < R; ++k) {
         const int row = p.y + k * a.LY;
         if (row < p.len) {
-            float o[V];
+            float o[V], xh[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float xh = (x[k].get(j) - mean[j]) * rs[j];
-                o[j] = rs[j] * (fmaf(ga[j], dz[k][j], -m1[j]) - xh * m2[j]);
-            }
+            for (int j = 0; j < V; ++j) xh[j] = (x[k].get(j) - mean[j]) * rs[j];
+            if (!KEEP) gn_dz<TD, V>(a, p.r0 + row, p.c0, d[k], xh, ga, be, dz[0]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = rs[j] * (fmaf(ga[j], dz[KEEP ? k : 0][j], -m1[j]) - xh[j] * m2[j]);
             gn_store<TG, V>((TG*)a.dx + (size_t)(p.r0 + row) * a.ldg + p.c0, o);
         }
     }
@@ -511,7 +540,7 @@ __global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_bwd_apply_kernel(GnArgs a
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
     if (p.b < 0 || p.len == 0) return;
-    const int rows = a.LY * R, nch = min((total + rows - 1) / rows, a.nchunk), ng = a.W / a.cg;
+    const int rows = a.LY * R, nch = (total + rows - 1) / rows, ng = a.W / a.cg;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float* part = a.part + (size_t)p.b * a.nchunk * 2 * a.C + p.strip * a.W;
     for (int gi = wave; gi < ng; gi += NT / 64) {
@@ -535,7 +564,7 @@ __global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_bwd_apply_kernel(GnArgs a
     }
     __syncthreads();
     if (!p.on) return;
-    const float inv_n = 1.0f / ((float)min(total, a.nchunk * rows) * (float)a.cg);
+    const float inv_n = 1.0f / ((float)total * (float)a.cg);
     float mean[V], rs[V], ga[V], be[V], m1[V], m2[V];
     gn_lane_params<V>(a, p, mean, rs, ga, be);
 #pragma unroll
@@ -575,25 +604,34 @@ __global__ __launch_bounds__(1024) void gn_param_kernel(const float* __restrict_
     }
     red[y][x] = t;
     __syncthreads();
-    if (y == 0 && c < 2 * C) {
+    if (threadIdx.x < 64) {                      // y < 4: a quarter of the row lanes each
         double sum = 0.0;
-#pragma unroll 8
-        for (int k = 0; k < 64; ++k) sum += (double)red[k][x];
-        if (c < C)
-            dbeta[c] = (float)sum;
-        else
-            dgamma[c - C] = (float)sum;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum += (double)red[y * 16 + k][x];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (y == 0 && c < 2 * C) {
+            if (c < C)
+                dbeta[c] = (float)sum;
+            else
+                dgamma[c - C] = (float)sum;
+        }
     }
 }
 
 // ---- geometry ------------------------------------------------------------------------------------------------------
-// Strip: the narrowest run of whole groups and whole vectors that is at least GN_STRIP_BYTES wide and divides C.  R: rows
-// per thread, the smallest compiled one that holds the utterance; none does: chunks of the largest.
+// Strip: the narrowest run of whole groups and whole vectors that is at least GN_STRIP_BYTES wide and divides C.  R: rows per thread,
+// the smallest compiled one that holds the utterance; none does: chunks of GN_CHUNK_ROWS.
+// More than 8 rows per thread of a bf16 backward (128 registers of data): only for bf16 dout (the thread recomputes dz instead of
+// keeping it; 32 x 1600 rows x 256 channels with fp32 dout: 51 us against 48 in chunks), and only where the workgroups fill the chip
+// (512 of them, 256 x 800 x 80: 35 us against 41 in chunks; 256: 34 against 38; 64: 29 against 21).  All others hold 16 rows
+// (32 x 1600 x 256 fp32: forward 23 us against 35 in chunks, backward 43 against 63; one utterance 10.7 against 11.6, 11.7 against 14.5).
 struct GnPlan { int W, LX, LY, R, nchunk; bool whole; };
 
 static int gn_gcd(int a, int b) { return b ? gn_gcd(b, a % b) : a; }
 
-static GnPlan gn_plan(int max_len, int C, int G, int x_dtype, bool backward) {
+// dout_dtype: of a backward, -1 for the forward
+static GnPlan gn_plan(int B, int max_len, int C, int G, int x_dtype, int dout_dtype) {
     GnPlan p;
     const int V = x_dtype == 0 ? 4 : 8, es = x_dtype == 0 ? 4 : 2, cg = C / G;
     const int unit = cg / gn_gcd(cg, V) * V, units = C / unit;
@@ -601,11 +639,11 @@ static GnPlan gn_plan(int max_len, int C, int G, int x_dtype, bool backward) {
     while (m < units && (m * unit * es < GN_STRIP_BYTES || units % m)) ++m;
     p.W = m * unit;
     p.LX = p.W / V;
-    const int most = !backward || x_dtype == 0 ? 16 : 8;
+    const bool fewer = x_dtype == 1 && dout_dtype >= 0 && (dout_dtype == 0 || (long long)B * (C / p.W) < 256);
     for (int nt = GN_WHOLE_THREADS;; nt = GN_CHUNK_THREADS) {
         p.LY = p.LX <= 64 ? nt / 64 * (64 / p.LX) : nt / p.LX;
         const int need = (max_len + p.LY - 1) / p.LY;
-        p.whole = nt == GN_WHOLE_THREADS && need <= most;
+        p.whole = nt == GN_WHOLE_THREADS && need <= (fewer ? 8 : 16);
         p.R = !p.whole ? GN_CHUNK_ROWS : (need <= 4 ? 4 : (need <= 8 ? 8 : 16));
         p.nchunk = p.whole ? 1 : (max_len + p.LY * p.R - 1) / (p.LY * p.R);
         if (p.whole || nt == GN_CHUNK_THREADS) break;
@@ -647,7 +685,7 @@ static void gn_launch_bwd(const GnArgs& a, const GnPlan& p, hipStream_t s) {
 template <typename TX, typename TD, typename TG> static void gn_launch_bwd_r(const GnArgs& a, const GnPlan& p, hipStream_t s) {
     if (p.R == 4) gn_launch_bwd<TX, TD, TG, 4>(a, p, s);
     else if (p.R == 8) gn_launch_bwd<TX, TD, TG, 8>(a, p, s);
-    else if constexpr (sizeof(TX) == 4) gn_launch_bwd<TX, TD, TG, 16>(a, p, s);
+    else if constexpr (sizeof(TX) == 4 || sizeof(TD) == 2) gn_launch_bwd<TX, TD, TG, 16>(a, p, s);
 }
 
 static int gn_check(const char* who, const void* x, const int* cu, const float* gamma, const float* beta, const float* stats, int B,
@@ -665,11 +703,11 @@ static int gn_check(const char* who, const void* x, const int* cu, const float* 
     return FS2_OK;
 }
 
-static GnArgs gn_args(int B, const void* x, const int* cu, const float* gamma, const float* beta, float* stats, void* workspace, int M, int C,
+static GnArgs gn_args(int B, const void* x, const int* cu, const float* gamma, const float* beta, float* stats, void* workspace, int max_len, int M, int C,
                       int groups, int ldx, int act, const GnPlan& p, Dropout drop) {
     GnArgs a = {};
     a.x = x; a.cu = cu; a.gamma = gamma; a.beta = beta; a.stats = stats; a.part = (float*)workspace;
-    a.M = M; a.C = C; a.G = groups; a.cg = C / groups; a.ldx = ldx; a.act = act;
+    a.M = M; a.max_len = max_len; a.C = C; a.G = groups; a.cg = C / groups; a.ldx = ldx; a.act = act;
     a.nchunk = p.nchunk; a.nstrip = C / p.W; a.W = p.W; a.LX = p.LX; a.LY = p.LY;
     a.units = B * p.nchunk; a.inv_lx = 1.0f / (float)p.LX; a.inv_cg = 1.0f / (float)a.cg;
     a.drop = drop;
@@ -684,7 +722,7 @@ extern "C" long long fs2_group_norm_workspace(int B, int max_len, int C, int gro
     if (B <= 0 || C <= 0 || groups <= 0 || C % groups || C % 4) return 0;
     long long most = 0;
     for (int t = 0; t < (C % 8 ? 1 : 2); ++t) {
-        const GnPlan p = gn_plan(max_len, C, groups, t, false);
+        const GnPlan p = gn_plan(B, max_len, C, groups, t, -1);
         const long long n = p.whole ? 0 : (long long)B * p.nchunk * groups * 2 * (long long)sizeof(float);
         most = n > most ? n : most;
     }
@@ -699,10 +737,10 @@ extern "C" int fs2_group_norm(const void* x, const int* cu, const float* gamma, 
     FS2_CHECK_ARG((out_dtype == 0 || out_dtype == 1) && (out || M == 0) && ldo >= C && ldo % 4 == 0 && ((uintptr_t)out & 15) == 0,
                   "fs2_group_norm: out_dtype=%d, ldo=%d (a multiple of 4), or out null or unaligned", out_dtype, ldo);
     FS2_CHECK_ARG(eps > 0.f, "fs2_group_norm: eps must be positive");
-    const GnPlan p = gn_plan(max_len, C, groups, x_dtype, false);
+    const GnPlan p = gn_plan(B, max_len, C, groups, x_dtype, -1);
     FS2_CHECK_ARG(p.whole || workspace, "fs2_group_norm: this shape needs fs2_group_norm_workspace bytes");
     FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 30), "fs2_group_norm: too many workgroups (B=%d)", B);
-    GnArgs a = gn_args(B, x, cu, gamma, beta, stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
+    GnArgs a = gn_args(B, x, cu, gamma, beta, stats, workspace, max_len, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
     a.out = out; a.ldo = ldo; a.eps = eps;
     if (x_dtype == 0 && out_dtype == 0) gn_launch_fwd_r<float, float>(a, p, stream);
     else if (x_dtype == 0) gn_launch_fwd_r<float, bf16_t>(a, p, stream);
@@ -715,8 +753,8 @@ extern "C" int fs2_group_norm(const void* x, const int* cu, const float* gamma, 
 extern "C" long long fs2_group_norm_bwd_workspace(int B, int max_len, int C, int groups) {
     if (B <= 0 || C <= 0 || groups <= 0 || C % groups || C % 4) return 16;
     long long most = 0;
-    for (int t = 0; t < (C % 8 ? 1 : 2); ++t) {
-        const GnPlan p = gn_plan(max_len, C, groups, t, true);
+    for (int t = 0; t < (C % 8 ? 2 : 4); ++t) {
+        const GnPlan p = gn_plan(B, max_len, C, groups, t >> 1, t & 1);
         const long long n = (long long)B * p.nchunk * 2 * C * (long long)sizeof(float);
         most = n > most ? n : most;
     }
@@ -736,9 +774,9 @@ extern "C" int fs2_group_norm_bwd(const void* x, const float* stats, const int* 
                       (((uintptr_t)dout | (uintptr_t)dx) & 15) == 0,
                   "fs2_group_norm_bwd: ldd=%d (a multiple of %d), ldg=%d (of 4), or dout or dx unaligned", ldd, x_dtype == 0 ? 4 : 8,
                   ldg);
-    const GnPlan p = gn_plan(max_len, C, groups, x_dtype, true);
+    const GnPlan p = gn_plan(B, max_len, C, groups, x_dtype, dout_dtype);
     FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 30), "fs2_group_norm_bwd: too many workgroups (B=%d)", B);
-    GnArgs a = gn_args(B, x, cu, gamma, beta, (float*)stats, workspace, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
+    GnArgs a = gn_args(B, x, cu, gamma, beta, (float*)stats, workspace, max_len, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
     a.dout = dout; a.dx = dx; a.ldd = ldd; a.ldg = ldg;
 #define FS2_GN(TX, TD)                                              \
     if (dx_dtype == 0) gn_launch_bwd_r<TX, TD, float>(a, p, stream); \

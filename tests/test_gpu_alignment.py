@@ -438,6 +438,7 @@ NORMS = [
     ([9000, 3], 40, 8, "silu"),                          # chunks both ways
     ([40, 3], 1024, 2, "none"),
     ([70], 1024, 1024, "tanh"),
+    ([180, 0] + [3] * 254, 256, 1, "tanh"),              # 256 workgroups of up to 16 rows a thread, both ways and types
 ]
 
 
