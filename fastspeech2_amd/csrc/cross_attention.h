@@ -89,28 +89,24 @@ template <typename E, int N> __device__ __forceinline__ void x_mma(const XFrag<E
     }
 }
 
-// the three planes of two values, packed in pairs.  CHECK: an infinity stays one (its rest is not a number otherwise)
-template <bool CHECK> __device__ __forceinline__ void x_split2(float a, float b, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
+// the three planes of two values, packed in pairs (an infinity becomes a NaN: infinity - infinity is its rest)
+__device__ __forceinline__ void x_split2(float a, float b, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
     const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
     w0 = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
     const float a0 = __builtin_bit_cast(float, ua & 0xffff0000u), b0 = __builtin_bit_cast(float, ub & 0xffff0000u);
-    float ra = a - a0, rb = b - b0;
-    if (CHECK) {
-        ra = a == a0 ? 0.f : ra;
-        rb = b == b0 ? 0.f : rb;
-    }
+    const float ra = a - a0, rb = b - b0;
     const uint32_t va = __builtin_bit_cast(uint32_t, ra), vb = __builtin_bit_cast(uint32_t, rb);
     w1 = __builtin_amdgcn_perm(vb, va, 0x07060302u);
     const float sa = ra - __builtin_bit_cast(float, va & 0xffff0000u), sb = rb - __builtin_bit_cast(float, vb & 0xffff0000u);
     w2 = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, sb), __builtin_bit_cast(uint32_t, sa), 0x07060302u);
 }
 struct XRaw { float v[8]; };          // eight consecutive fp32 values on their way to a fragment
-template <bool CHECK> __device__ __forceinline__ XFrag<XF32> x_split8(const XRaw& x) {
+__device__ __forceinline__ XFrag<XF32> x_split8(const XRaw& x) {
     uint4 w[3];
-    x_split2<CHECK>(x.v[0], x.v[1], w[0].x, w[1].x, w[2].x);
-    x_split2<CHECK>(x.v[2], x.v[3], w[0].y, w[1].y, w[2].y);
-    x_split2<CHECK>(x.v[4], x.v[5], w[0].z, w[1].z, w[2].z);
-    x_split2<CHECK>(x.v[6], x.v[7], w[0].w, w[1].w, w[2].w);
+    x_split2(x.v[0], x.v[1], w[0].x, w[1].x, w[2].x);
+    x_split2(x.v[2], x.v[3], w[0].y, w[1].y, w[2].y);
+    x_split2(x.v[4], x.v[5], w[0].z, w[1].z, w[2].z);
+    x_split2(x.v[6], x.v[7], w[0].w, w[1].w, w[2].w);
     XFrag<XF32> f;
 #pragma unroll
     for (int pl = 0; pl < 3; ++pl) f.p[pl] = __builtin_bit_cast(bf16x8, w[pl]);
@@ -129,7 +125,7 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_load(const typename 
         f.p[0] = *(const bf16x8*)p;
         return f;
     } else {
-        return x_split8<true>(x_raw(p));
+        return x_split8(x_raw(p));
     }
 }
 // element j of an operand
@@ -156,7 +152,7 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_pack(const f32x4& lo
             x.v[r] = lo[r];
             x.v[4 + r] = hi[r];
         }
-        return x_split8<false>(x);
+        return x_split8(x);
     }
 }
 
@@ -281,8 +277,21 @@ template <int DK, int ROWS, int WAY, int NW> struct XFetch<XF32, DK, ROWS, WAY, 
     static constexpr int N = (CHUNKS + 64 * NW - 1) / (64 * NW);                // of a lane (the last of them may be missing)
     static __device__ __forceinline__ bool has(int id) { return CHUNKS % (64 * NW) == 0 || id < CHUNKS; }
     f32x4 r[N];
-    __device__ __forceinline__ XFetch(int, int, int) {}
+    unsigned off[N];
+    __device__ __forceinline__ XFetch(int ld, int wave, int lane) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int id = n * 64 * NW + wave * 64 + lane, row = id / CPR, c = id - row * CPR;
+            off[n] = (unsigned)row * (unsigned)ld * 4u + (unsigned)c * 16u;
+        }
+    }
     __device__ __forceinline__ void fetch(const float* __restrict__ tile, int ld, int left, unsigned char*, int wave, int lane) {
+        if (left >= ROWS) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (has(n * 64 * NW + wave * 64 + lane)) r[n] = *(const f32x4*)((const unsigned char*)tile + off[n]);
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int id = n * 64 * NW + wave * 64 + lane, row = id / CPR, c = id - row * CPR;
@@ -305,8 +314,8 @@ template <int DK, int ROWS, int WAY, int NW> struct XFetch<XF32, DK, ROWS, WAY, 
             const int id = n * 64 * NW + wave * 64 + lane, row = id / CPR, c = id - row * CPR;
             if (!has(id)) continue;
             uint2 w[3];
-            x_split2<true>(r[n][0], r[n][1], w[0].x, w[1].x, w[2].x);
-            x_split2<true>(r[n][2], r[n][3], w[0].y, w[1].y, w[2].y);
+            x_split2(r[n][0], r[n][1], w[0].x, w[1].x, w[2].x);
+            x_split2(r[n][2], r[n][3], w[0].y, w[1].y, w[2].y);
             unsigned char* at = dst + TL::at(row, c >> 1) + (c & 1) * 8;
 #pragma unroll
             for (int pl = 0; pl < 3; ++pl) *(uint2*)(at + pl * TL::PLANE) = w[pl];

@@ -26,7 +26,7 @@ __device__ __forceinline__ void x_zero_rows(const XArgs& a, int q0, int kvh, int
 }
 
 template <typename E, int DK, int QT, bool DROP>
-__global__ __launch_bounds__(256, 2) void xattn_rows_kernel(XArgs a) {
+__global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_rows_kernel(XArgs a) {
     typedef typename E::mem T;
     constexpr int KB = x_kb<E>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
     typedef XTile<E, DK, KB, 1> TK;
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int 
 
 struct XPlan { bool few; int qt, nsplit; };
 
-static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dk, int dtype) {
+static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
     XPlan p = {};
     const int g = H / KV;
     const long rows = (long)max_q * g, pairs = (long)B * KV;
@@ -427,11 +427,14 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dk, int dtyp
             p.nsplit = (int)(want < most ? want : most);
         }
     } else {
-        p.qt = rows > 64 && !(dtype == 0 && dk == 128) ? 2 : 1;        // (two row tiles of dk = 128 in three planes spill 42 registers)
-        const int kb = dtype == 1 ? 64 : 32, fill = dtype == 1 ? 256 : 384;
+        // two row tiles to a wave: bf16, whose tiles cost nothing but their reads.  fp32: with one, three workgroups share a CU and
+        // hide each other's LDS reads and splits (32 x 240 rows x 810 keys, dk = 96: 59 us against 62; 32 x 120 x 800, dk = 32: 25
+        // against 31), though each splits its keys for half the rows
+        p.qt = rows > 64 && dtype == 1 ? 2 : 1;
+        const int kb = dtype == 1 ? 64 : 32, full = dtype == 1 ? 512 : 768;          // workgroups that the chip holds at a time
         const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = (max_k + kb - 1) / kb;
-        if (items < fill && tiles >= 4) {
-            const long want = 512 / items, most = tiles / (128 / kb);
+        if (items < (dtype == 1 ? full / 2 : full) && tiles >= 4) {
+            const long want = full / items, most = tiles / (128 / kb);
             p.nsplit = (int)(want < most ? want : most);
         }
     }
@@ -462,7 +465,7 @@ static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipS
         const int rows = max_q * a.g, nblk = (rows + 64 * p.qt - 1) / (64 * p.qt);
         const dim3 grid = fs2_x_grid(a, nblk, a.KV, B);
         if (p.qt == 2) {
-            if constexpr (E::PL == 1 || DK < 128) {
+            if constexpr (E::PL == 1) {
                 if (a.drop.thresh) launch_xattn_rows<E, DK, 2, true>(a, grid, stream);
                 else launch_xattn_rows<E, DK, 2, false>(a, grid, stream);
             }
@@ -487,7 +490,7 @@ using namespace fs2;
 extern "C" long long fs2_cross_attention_workspace(int B, int max_q, int max_k, int Mq, int n_heads, int n_kv_heads, int dk,
                                                    int dtype) {
     if (B <= 0 || max_q <= 0 || max_k <= 0 || Mq <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return 0;
-    const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dk, dtype);
+    const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dtype);
     return p.nsplit == 1 ? 0 : (long long)p.nsplit * Mq * n_heads * (dk + 2) * (long long)sizeof(float);
 }
 
@@ -509,7 +512,7 @@ extern "C" int fs2_cross_attention(const void* q, const void* k, const void* v, 
     a.ctx = ctx;
     a.lse = lse;
     a.drop = fs2_make_dropout(seed, stream_id, rate);
-    const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dk, dtype);
+    const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dtype);
     a.nsplit = p.nsplit;
     a.part = (float*)workspace;
     FS2_CHECK_ARG(p.nsplit == 1 || (workspace && ((uintptr_t)workspace & 15) == 0),
