@@ -383,33 +383,76 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
     }
 }
 
-// merge of the key ranges; one lane per (row, four channels).  Rows behind the last utterance, and rows of utterances longer
-// than max_q, were computed by nobody: cu_q[B] bounds the first, the second are the caller's breach of max_q.
+// Merge of the key ranges, many rows: one lane per (row, four channels), the few ranges in a loop.  Rows [cu_q[0], cu_q[B]) only: the
+// others were computed by nobody.  A range without keys wrote no partial context (its sum is 0): read, not used.
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int dk) {
     const int d = a.H * dk, dv = d >> 2;
     const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int rows = min(max(a.cu_q[B], 0), a.Mq);
-    if (idx >= (long long)rows * dv) return;
-    const int m = (int)(idx / dv), c = (int)(idx % dv) * 4, h = c / dk;
+    const int r0 = min(max(a.cu_q[0], 0), a.Mq), r1 = min(max(a.cu_q[B], 0), a.Mq);
+    if (idx >= (long long)(r1 - r0) * dv) return;
+    const int m = r0 + (int)(idx / dv), c = (int)(idx % dv) * 4, h = c / dk;
     const float* ml = a.part + (size_t)a.nsplit * a.Mq * d + ((size_t)h * a.Mq + m) * 2;
     const size_t step = (size_t)a.H * a.Mq * 2;
     float mx = -INFINITY;
+#pragma unroll 4
     for (int s = 0; s < a.nsplit; ++s) mx = fmaxf(mx, ml[s * step]);
     const float mu = mx == -INFINITY ? 0.f : mx;
     float L = 0.f;
     bool any = false;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < a.nsplit; ++s) {
-        const float l = ml[s * step + 1];
-        if (l == 0.f) continue;                  // a range without keys wrote no partial context
-        any = true;
-        const float f = __builtin_amdgcn_exp2f(ml[s * step] - mu);
-        L = fmaf(l, f, L);
-        acc += *(const f32x4*)(a.part + ((size_t)s * a.Mq + m) * d + c) * f;
+        const float l = ml[s * step + 1], f = __builtin_amdgcn_exp2f(ml[s * step] - mu);
+        const f32x4 o = *(const f32x4*)(a.part + ((size_t)s * a.Mq + m) * d + c);
+        if (l != 0.f) {
+            any = true;
+            L = fmaf(l, f, L);
+            acc += o * f;
+        }
     }
     store4<T>((T*)a.ctx + (size_t)m * a.ldo + c, any ? acc * (1.0f / L) : acc);
     if (a.lse && c % dk == 0) a.lse[(size_t)h * a.Mq + m] = any ? mx + __log2f(L) : -INFINITY;
+}
+
+// Few rows, up to X_MAX_SPLIT ranges: one workgroup per (row, head), 1024 / dk lanes to every four channels, each takes every
+// (1024 / dk)th range.  One lane for all ranges waited for 32 loads in a row (15 us of the 21 us of one frame over 65000 keys).
+constexpr int X_MAX_SPLIT = 256;
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void xattn_combine_few_kernel(XArgs a, int B) {
+    constexpr int SL = DK / 4, NL = 256 / SL;
+    __shared__ float ms[X_MAX_SPLIT], ls[X_MAX_SPLIT];
+    __shared__ __attribute__((aligned(16))) float red[NL][DK];
+    const int h = blockIdx.x, m = blockIdx.y + min(max(a.cu_q[0], 0), a.Mq), tid = threadIdx.x;
+    if (m >= min(max(a.cu_q[B], 0), a.Mq)) return;
+    const size_t d = (size_t)a.H * DK;
+    if (tid < a.nsplit) {
+        const float2 t = *(const float2*)(a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)tid * a.H + h) * a.Mq + m) * 2);
+        ms[tid] = t.x;
+        ls[tid] = t.y;
+    }
+    __syncthreads();
+    float mx = -INFINITY;
+    for (int s = tid & 63; s < a.nsplit; s += 64) mx = fmaxf(mx, ms[s]);
+    mx = wave_max(mx);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float L = 0.f;
+    for (int s = tid & 63; s < a.nsplit; s += 64) L += ls[s] == 0.f ? 0.f : ls[s] * __builtin_amdgcn_exp2f(ms[s] - mu);
+    L = wave_sum(L);
+    const int c = tid % SL * 4, lane_s = tid / SL;            // (dk = 96: 16 lanes are left over)
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = lane_s; s < a.nsplit; s += NL) {
+        const f32x4 o = *(const f32x4*)(a.part + ((size_t)s * a.Mq + m) * d + h * DK + c);
+        if (ls[s] != 0.f) acc += o * __builtin_amdgcn_exp2f(ms[s] - mu);
+    }
+    if (lane_s < NL) *(f32x4*)(red[lane_s] + c) = acc;
+    __syncthreads();
+    if (tid >= SL) return;
+#pragma unroll
+    for (int k = 1; k < NL; ++k) acc += *(const f32x4*)(red[k] + c);
+    store4<T>((T*)a.ctx + (size_t)m * a.ldo + h * DK + c, acc * (L == 0.f ? 0.f : 1.0f / L));
+    if (a.lse && c == 0) a.lse[(size_t)h * a.Mq + m] = L == 0.f ? -INFINITY : mx + __log2f(L);
 }
 
 struct XPlan { bool few; int qt, nsplit; };
@@ -423,7 +466,9 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
     if (p.few) {
         const long tiles = (max_k + 31) / 32;
         if (tiles > 8 && pairs < 256) {
-            const long want = 512 / pairs, most = tiles / 4;
+            // a tile to every wave up to 32 ranges, four tiles to a wave beyond (one frame over 65000 keys, dk = 128: 127 ranges
+            // 14.5 + 7.4 us, 253 ranges 14.4 + 13.0 us, 32 ranges 26.6 + 4.5 us)
+            const long want = 512 / pairs, some = tiles / 4 < 32 ? tiles / 4 : 32, most = tiles / 16 > some ? tiles / 16 : some;
             p.nsplit = (int)(want < most ? want : most);
         }
     } else {
@@ -438,7 +483,8 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
             p.nsplit = (int)(want < most ? want : most);
         }
     }
-    if (p.nsplit > 32) p.nsplit = 32;
+    const int cap = p.few ? X_MAX_SPLIT : 32;
+    if (p.nsplit > cap) p.nsplit = cap;
     if (p.nsplit < 1) p.nsplit = 1;
     return p;
 }
@@ -476,8 +522,11 @@ static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipS
     }
     FS2_CHECK_LAUNCH("fs2_cross_attention");
     if (a.nsplit > 1) {
-        const long long n = (long long)a.Mq * (a.H * dk / 4);
-        hipLaunchKernelGGL(xattn_combine_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B, dk);
+        const long long most = (long long)B * max_q, rows = most < a.Mq ? most : a.Mq, n = rows * (a.H * dk / 4);
+        if (p.few)
+            hipLaunchKernelGGL((xattn_combine_few_kernel<T, DK>), dim3(a.H, (unsigned)rows), dim3(256), 0, stream, a, B);
+        else
+            hipLaunchKernelGGL(xattn_combine_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B, dk);
         FS2_CHECK_LAUNCH("fs2_cross_attention(merge)");
     }
     return FS2_OK;
