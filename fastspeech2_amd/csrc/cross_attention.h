@@ -18,7 +18,7 @@ struct XArgs {
     float* lse;          // [H][Mq] log2-domain log-sum-exp (or null)
     const int* cu_q;     // [B + 1]
     const int* cu_k;     // [B + 1]
-    int Mq, Mk, ldq, ldk, ldv, ldo, H, KV;
+    int Mq, Mk, max_q, max_k, ldq, ldk, ldv, ldo, H, KV;
     int g;               // H / KV
     unsigned magic;      // floor(2^32 / g) + 1 (g > 1): r / g = umulhi(r, magic) for r < 2^24, g <= 128
     float scale_log2e;   // log2(e) / sqrt(dk)
@@ -38,11 +38,17 @@ struct XArgs {
 typedef __attribute__((address_space(3))) void x_lds_void;
 typedef const __attribute__((address_space(1))) void x_gbl_void;
 
-// rows [r0, r0 + len) of utterance b.  The offsets come from device memory: whatever they hold, no access leaves [0, M)
-__device__ __forceinline__ void x_range(const int* cu, int b, int M, int& r0, int& len) {
+// rows [r0, r0 + len) of utterance b.  The offsets come from device memory: whatever they hold, no access leaves [0, M), and
+// an utterance ends after `longest` rows, which the grids and the 32-bit row arithmetic count on
+__device__ __forceinline__ void x_range(const int* cu, int b, int M, int longest, int& r0, int& len) {
     const int c0 = min(max(cu[b], 0), M), c1 = min(max(cu[b + 1], c0), M);
     r0 = c0;
-    len = c1 - c0;
+    len = min(c1 - c0, longest);
+}
+// rows that some utterance owns, [first, end)
+__device__ __forceinline__ void x_owned(const int* cu, int B, int M, int& first, int& end) {
+    first = min(max(cu[0], 0), M);
+    end = min(max(cu[B], first), M);
 }
 // packed row -> query index inside the utterance; head in group = r - q * g
 __device__ __forceinline__ int x_query(const XArgs& a, int r) { return a.g == 1 ? r : (int)__umulhi((unsigned)r, a.magic); }
@@ -399,11 +405,11 @@ static inline dim3 fs2_x_grid(fs2::XArgs& a, int nblk, int heads, int B) {
     return a.pairs >= 8 ? dim3(8 * nblk, (a.pairs + 7) / 8, a.nsplit) : dim3(nblk, a.pairs, a.nsplit);
 }
 
-static inline fs2::XArgs fs2_x_args(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, int Mq, int Mk, int H,
-                                    int KV, int dk, int ldq, int ldk, int ldv, int ldo) {
+static inline fs2::XArgs fs2_x_args(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, int max_q, int max_k,
+                                    int Mq, int Mk, int H, int KV, int dk, int ldq, int ldk, int ldv, int ldo) {
     fs2::XArgs a = {};
     a.q = q; a.k = k; a.v = v; a.cu_q = cu_q; a.cu_k = cu_k;
-    a.Mq = Mq; a.Mk = Mk; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
+    a.Mq = Mq; a.Mk = Mk; a.max_q = max_q; a.max_k = max_k; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
     a.H = H; a.KV = KV; a.g = H / KV;
     a.magic = a.g > 1 ? (unsigned)((1ull << 32) / a.g + 1) : 0u;
     a.scale = 1.0f / sqrtf((float)dk);

@@ -6,10 +6,20 @@
 //
 // Orientation as in attention.hip: S^T = K Q^T and O^T = V^T P^T, so that a lane owns one query row and every softmax statistic
 // is lane-local; the accumulator layout of P^T is used as the next operand, V is read transposed from LDS with the same map.
-//   rows kernel: 4 waves x 16 QT packed rows, K / V tiles of 64 keys double-buffered in LDS for all four.
+//   rows kernel: 4 waves x 16 QT packed rows; K / V tiles for all four in LDS: bf16 64 keys, two stages; fp32 32 keys in three bf16
+//                planes, one stage, the next tile on its way in registers.
 //   few kernel:  at most 16 packed rows per pair (one frame at a time): the four waves share the rows and split the KEYS,
-//                each with its own 32-key tiles; K goes straight into registers, V through wave-private LDS; one merge.
+//                each with its own 32-key tiles in wave-private LDS (fp32: K straight into registers); one merge.
 // Where the pairs alone do not fill the chip, ranges of keys go to `nsplit` workgroups and a second kernel merges.
+//
+// Measured (floor: bytes at 5.2 TB/s, or products at 1198 TFLOP/s bf16, 154 fp32):
+//   one frame of 256 sentences, 8 heads on 2 of 64, 160 keys, bf16: 7.5 us for 21 MB (2.8 TB/s; floor 4.1); one sentence 5.8 us, of
+//     which the launch is 3.8.
+//   32 x 800 frames over 120 phones, 2 heads of 128, bf16: 14.2 us for 31 MB (2.2 TB/s; floor 6.0).  Two key tiles leave nothing to
+//     overlap: a workgroup waits for its queries and first keys, multiplies, and writes.
+//   32 x 120 phones over 810 frames, 4 heads on 2 of 96, fp32: 55 us, 4.8 GFLOP = 87 TFLOP/s (floor 31), 6 of it the merge.  Each
+//     tile costs a SIMD 1150 cycles of MFMA (six bf16 products for one of fp32), 1400 of splitting and softmax and the CU 1700 of LDS;
+//     three workgroups on a CU overlap them to about 3000.
 #include "cross_attention.h"
 
 namespace fs2 {
@@ -38,8 +48,8 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
-    x_range(a.cu_q, b, a.Mq, q0, lenq);
-    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
     const int nrow = lenq * a.g;
     if (blk * BQ >= nrow) return;
 
@@ -249,8 +259,8 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // wave w: V tile at w * BYTES; then the merge
     const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     int q0, lenq, k0, lenk;
-    x_range(a.cu_q, b, a.Mq, q0, lenq);
-    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
     const int nrow = min(lenq * a.g, 16);
     if (nrow == 0) return;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -389,7 +399,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int dk) {
     const int d = a.H * dk, dv = d >> 2;
     const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int r0 = min(max(a.cu_q[0], 0), a.Mq), r1 = min(max(a.cu_q[B], 0), a.Mq);
+    int r0, r1;
+    x_owned(a.cu_q, B, a.Mq, r0, r1);
     if (idx >= (long long)(r1 - r0) * dv) return;
     const int m = r0 + (int)(idx / dv), c = (int)(idx % dv) * 4, h = c / dk;
     const float* ml = a.part + (size_t)a.nsplit * a.Mq * d + ((size_t)h * a.Mq + m) * 2;
@@ -423,8 +434,10 @@ __global__ __launch_bounds__(256) void xattn_combine_few_kernel(XArgs a, int B) 
     constexpr int SL = DK / 4, NL = 256 / SL;
     __shared__ float ms[X_MAX_SPLIT], ls[X_MAX_SPLIT];
     __shared__ __attribute__((aligned(16))) float red[NL][DK];
-    const int h = blockIdx.x, m = blockIdx.y + min(max(a.cu_q[0], 0), a.Mq), tid = threadIdx.x;
-    if (m >= min(max(a.cu_q[B], 0), a.Mq)) return;
+    int r0, r1;
+    x_owned(a.cu_q, B, a.Mq, r0, r1);
+    const int h = blockIdx.x, m = r0 + blockIdx.y, tid = threadIdx.x;
+    if (m >= r1) return;
     const size_t d = (size_t)a.H * DK;
     if (tid < a.nsplit) {
         const float2 t = *(const float2*)(a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)tid * a.H + h) * a.Mq + m) * 2);
@@ -554,10 +567,10 @@ extern "C" int fs2_cross_attention(const void* q, const void* k, const void* v, 
     FS2_CHECK_ARG(rate >= 0.f && rate < 1.f, "fs2_cross_attention: dropout rate must be in [0, 1)");
     FS2_CHECK_ARG((v || Mk == 0) && (ctx || Mq == 0) && ((uintptr_t)v & 15) == 0 && ((uintptr_t)ctx & 15) == 0,
                   "fs2_cross_attention: null or unaligned v or ctx");
-    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldv <= (1 << 20) && ldo >= n_heads * dk && ldv % epv == 0 && ldo % epv == 0,
+    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldv <= (1 << 20) && ldo >= n_heads * dk && ldo <= (1 << 20) && ldv % epv == 0 && ldo % epv == 0,
                   "fs2_cross_attention: bad leading dims ldv=%d ldo=%d", ldv, ldo);
     if (max_q == 0) return FS2_OK;
-    XArgs a = fs2_x_args(q, k, v, cu_q, cu_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, ldv, ldo);
+    XArgs a = fs2_x_args(q, k, v, cu_q, cu_k, max_q, max_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, ldv, ldo);
     a.ctx = ctx;
     a.lse = lse;
     a.drop = fs2_make_dropout(seed, stream_id, rate);

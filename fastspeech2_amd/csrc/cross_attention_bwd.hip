@@ -9,11 +9,15 @@
 // The packed rows of a shared head are its g query heads, so the sum over the group that dk and dv need is part of the loop.
 // Every output element has one writer and every sum a fixed order: no atomics, the same bits every time.
 #include "cross_attention.h"
-#include <type_traits>
 
 namespace fs2 {
 
+// Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16 (floor of the whole step 11.8 us): dq 22 us,
+// dk and dv 28 us; and of 3 x 1601 frames over 301 phones, 4 heads on 2 of 96, fp32 (floor 47.7): 43 and 46 + 6.5 us.
+
 // ---- dq and delta: one workgroup per (utterance, shared head, 64 packed rows) -------------------------------------
+// 832 workgroups of four waves, two to a CU (registers, and 80 KB of LDS at dk = 128): a second round that half fills the chip, and in
+// each two key tiles behind a wait for the rows.  dS as two numbers is 2 of the 22 us.
 template <typename E, int DK, bool DROP>
 __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     typedef typename E::mem T;
@@ -27,8 +31,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
-    x_range(a.cu_q, b, a.Mq, q0, lenq);
-    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
     const int nrow = lenq * a.g;
     if (blk * 64 >= nrow) return;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -170,7 +174,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
 
 // ---- dk, dv -----------------------------------------------------------------------------------------------------------
 // fp32: one workgroup per (utterance, shared head, 64 keys, range of packed rows), a wave to 16 keys, its K and V operands in
-// registers; row tiles of 32 in LDS for all four.
+// registers; row tiles of 32 in LDS for all four, split into planes once for all (a wave with a tile of its own, as in bf16, would
+// split each for itself).  Bound by what a tile costs a SIMD in turn: MFMA, splits, LDS.
 template <int DK, bool DROP>
 __global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs a) {
     typedef XF32 E;
@@ -183,8 +188,8 @@ __global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
-    x_range(a.cu_q, b, a.Mq, q0, lenq);
-    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
     if (blk * 64 >= lenk) return;
     const int nrow = lenq * a.g;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -290,14 +295,16 @@ __global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs
 // bf16: one workgroup of four waves per (utterance, shared head, 32 keys, range of packed rows).  The 32 keys stay in LDS; each wave
 // streams its OWN tiles of 32 rows through a private LDS buffer (read row-wise for S and dP, transposed for dV and dK) and keeps a
 // dK, dV of its own, so the loop has no barrier; the four are added through LDS at the end.  64 keys to a workgroup and one row tile
-// for all four waves (the fp32 form above) left half the chip without a workgroup at 32 x 120 phones unless the rows were split,
-// and wrote four times the gradients as partial sums: 27 + 5 us against 
-template <int DK, int KT, bool DROP>
+// for all four waves (the fp32 form above) leave half the chip without a workgroup at 32 x 120 phones unless the rows are split, which
+// writes the gradients several times over as partial sums (27 + 5 us, before dS became two numbers; this form then 25.6).  A second
+// buffer for each wave would overlap its tiles' DMA and products, but leaves one workgroup to a CU where there are slightly more
+// workgroups than CUs: 41 us against 28.
+template <int DK, bool DROP>
 __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
     typedef XB16 E;
     typedef bf16_t T;
     typedef XTile<E, DK, 32, 2> TL;
-    constexpr int KB = 16 * KT;
+    constexpr int KT = 2, KB = 16 * KT;
     typedef XTile<E, DK, KB, 1> TK;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT, NP = TK::BYTES / 1024, NWK = NP % 4 == 0 ? 4 : (NP % 2 == 0 ? 2 : 1);
@@ -307,8 +314,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
     int b, kvh, blk, split;
     if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
-    x_range(a.cu_q, b, a.Mq, q0, lenq);
-    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
     if (blk * KB >= lenk) return;
     const int nrow = lenq * a.g;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -462,12 +469,13 @@ template <typename T>
 __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int dk) {
     const int w = a.KV * dk, wv = w >> 2;
     const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int rows = min(max(a.cu_k[B], 0), a.Mk);
-    const long long n = (long long)rows * wv;
+    int r0, r1;
+    x_owned(a.cu_k, B, a.Mk, r0, r1);
+    const long long n = (long long)(r1 - r0) * wv;
     if (idx >= 2 * n) return;
     const bool is_v = idx >= n;
     const long long e = is_v ? idx - n : idx;
-    const int m = (int)(e / wv), c = (int)(e % wv) * 4;
+    const int m = r0 + (int)(e / wv), c = (int)(e % wv) * 4;
     const size_t half = (size_t)a.Mk * w;
     const float* src = a.part + (is_v ? half : 0) + (size_t)m * w + c;
     f32x4 sum = *(const f32x4*)src;
@@ -481,14 +489,10 @@ __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int 
 // ---- mass: one workgroup per (utterance, head, 16 KT keys, range of queries) --------------------------------------------
 // The keys are operands in the registers of every wave; the waves stream the queries, 16 at a time, through a private LDS ring of two
 // tiles.  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds up its own queries' weights over the whole loop, and the 16
-// queries of a row of lanes meet only at the end.
-#ifndef XNW
-#define XNW 4
-#endif
-#ifndef XMKT
-#define XMKT 4
-#endif
-constexpr int X_MASS_WAVES = XNW;
+// queries of a row of lanes meet only at the end.  32 x 800 queries, 120 keys, 2 heads of 128, bf16: 11.6 us for 16 MB (1.3 TB/s; floor
+// 3.0), the keys' wait and the first queries' behind it, then 13 tiles to a wave.  3100 queries, 512 keys, 4 heads of 64, fp32: 12.3 us
+// with the sum over nine query ranges (floor 3.9).  64 keys to a workgroup in bf16; 32 in fp32, whose keys take three times the registers.
+constexpr int X_MASS_WAVES = 4;
 
 template <typename E, int DK, int KT>
 __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs a) {
@@ -501,8 +505,8 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
     int b, h, blk, split;
     if (!x_decode(a, a.H, b, h, blk, split)) return;
     int q0, lenq, k0, lenk;
-    x_range(a.cu_q, b, a.Mq, q0, lenq);
-    x_range(a.cu_k, b, a.Mk, k0, lenk);
+    x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
+    x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
     if (blk * KB >= lenk) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -550,7 +554,7 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (qt + NW < t1) fetch(qt + NW, 0);
         }
-        if (qt * 16 + i >= lenq || !(fabsf(l) < INFINITY)) l = INFINITY;          // no such query: no weight
+        if (qt * 16 + i >= lenq || l == -INFINITY) l = INFINITY;      // no such query, or one without keys: no weight
         f32x4 s[KT];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) s[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -584,9 +588,11 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
 
 __global__ __launch_bounds__(256) void xattn_mass_sum_kernel(XArgs a, int B) {
     const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int rows = min(max(a.cu_k[B], 0), a.Mk);
+    int r0, r1;
+    x_owned(a.cu_k, B, a.Mk, r0, r1);
+    const int rows = r1 - r0;
     if (idx >= (long long)a.H * rows) return;
-    const size_t at = (size_t)(idx / rows) * a.Mk + idx % rows, step = (size_t)a.H * a.Mk;
+    const size_t at = (size_t)(idx / rows) * a.Mk + r0 + idx % rows, step = (size_t)a.H * a.Mk;
     float sum = a.part[at];
     for (int s = 1; s < a.nsplit; ++s) sum += a.part[s * step + at];
     a.mass[at] = sum;
@@ -601,7 +607,7 @@ static int x_dkv_split(int B, int max_q, int max_k, int H, int KV, int dtype) {
     const long want = 512 / items, most = dtype == 1 ? tiles / 8 : tiles / 4, n = want < most ? want : most;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
-constexpr int x_mass_kt(int dtype) { return dtype == 1 ? XMKT : 2; }
+constexpr int x_mass_kt(int dtype) { return dtype == 1 ? 4 : 2; }
 static int x_mass_split(int B, int max_q, int max_k, int H, int dtype) {
     const int kb = 16 * x_mass_kt(dtype);
     const long items = (long)B * H * ((max_k + kb - 1) / kb), trips = (max_q + 15) / 16 / X_MASS_WAVES;
@@ -624,12 +630,12 @@ template <int DK, bool DROP> static void launch_xattn_dkv(const XArgs& a, dim3 g
     fs2_allow_lds((const void*)xattn_dkv_kernel<DK, DROP>, lds, &ok);
     hipLaunchKernelGGL((xattn_dkv_kernel<DK, DROP>), grid, dim3(256), lds, stream, a);
 }
-template <int DK, int KT, bool DROP> static void launch_xattn_dkv32(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int tiles = 8 * XTile<XB16, DK, 32, 2>::BYTES + 2 * XTile<XB16, DK, 16 * KT, 1>::BYTES, merge = 4 * 16 * KT * (DK + 4) * 4;
+template <int DK, bool DROP> static void launch_xattn_dkv32(const XArgs& a, dim3 grid, hipStream_t stream) {
+    constexpr int tiles = 8 * XTile<XB16, DK, 32, 2>::BYTES + 2 * XTile<XB16, DK, 32, 1>::BYTES, merge = 4 * 32 * (DK + 4) * 4;
     constexpr int lds = tiles > merge ? tiles : merge;
     static unsigned long long ok = 0;
-    fs2_allow_lds((const void*)xattn_dkv32_kernel<DK, KT, DROP>, lds, &ok);
-    hipLaunchKernelGGL((xattn_dkv32_kernel<DK, KT, DROP>), grid, dim3(256), lds, stream, a);
+    fs2_allow_lds((const void*)xattn_dkv32_kernel<DK, DROP>, lds, &ok);
+    hipLaunchKernelGGL((xattn_dkv32_kernel<DK, DROP>), grid, dim3(256), lds, stream, a);
 }
 
 template <typename E, int DK>
@@ -646,8 +652,8 @@ static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipSt
     if (max_k > 0) {
         if constexpr (E::PL == 1) {
             const dim3 grid = fs2_x_grid(a, (max_k + 31) / 32, a.KV, B);
-            if (a.drop.thresh) launch_xattn_dkv32<DK, 2, true>(a, grid, stream);
-            else launch_xattn_dkv32<DK, 2, false>(a, grid, stream);
+            if (a.drop.thresh) launch_xattn_dkv32<DK, true>(a, grid, stream);
+            else launch_xattn_dkv32<DK, false>(a, grid, stream);
         } else {
             const dim3 grid = fs2_x_grid(a, (max_k + 63) / 64, a.KV, B);
             if (a.drop.thresh) launch_xattn_dkv<DK, true>(a, grid, stream);
@@ -655,7 +661,7 @@ static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipSt
         }
         FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(dk, dv)");
         if (a.nsplit > 1) {
-            const long long n = 2LL * a.Mk * (a.KV * dk / 4);
+            const long long most = (long long)B * max_k, n = 2 * (most < a.Mk ? most : a.Mk) * (a.KV * dk / 4);
             hipLaunchKernelGGL(xattn_dkv_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B, dk);
             FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(sum)");
         }
@@ -673,7 +679,7 @@ static int launch_xattn_mass(XArgs& a, int B, int max_k, hipStream_t stream) {
     hipLaunchKernelGGL((xattn_mass_kernel<E, DK, KT>), grid, dim3(64 * X_MASS_WAVES), lds, stream, a);
     FS2_CHECK_LAUNCH("fs2_cross_attention_mass");
     if (a.nsplit > 1) {
-        const long long n = (long long)a.H * a.Mk;
+        const long long most = (long long)B * max_k, n = a.H * (most < a.Mk ? most : a.Mk);
         hipLaunchKernelGGL(xattn_mass_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B);
         FS2_CHECK_LAUNCH("fs2_cross_attention_mass(sum)");
     }
@@ -707,12 +713,12 @@ extern "C" int fs2_cross_attention_bwd(const void* q, const void* k, const void*
     FS2_CHECK_ARG((Mq == 0 || (ctx && dctx && lse && dq)) && (Mk == 0 || (v && dk_out && dv)), "fs2_cross_attention_bwd: null argument");
     FS2_CHECK_ARG((((uintptr_t)v | (uintptr_t)ctx | (uintptr_t)dctx | (uintptr_t)dq | (uintptr_t)dk_out | (uintptr_t)dv) & 15) == 0,
                   "fs2_cross_attention_bwd: unaligned pointers");
-    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldv <= (1 << 20) && ldo >= n_heads * dk && ldv % epv == 0 && ldo % epv == 0,
+    FS2_CHECK_ARG(ldv >= n_kv_heads * dk && ldv <= (1 << 20) && ldo >= n_heads * dk && ldo <= (1 << 20) && ldv % epv == 0 && ldo % epv == 0,
                   "fs2_cross_attention_bwd: bad leading dims ldv=%d ldo=%d", ldv, ldo);
     if (max_q == 0 && max_k == 0) return FS2_OK;
     FS2_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0,
                   "fs2_cross_attention_bwd: fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, are needed");
-    XArgs a = fs2_x_args(q, k, v, cu_q, cu_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, ldv, ldo);
+    XArgs a = fs2_x_args(q, k, v, cu_q, cu_k, max_q, max_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, ldv, ldo);
     a.ctx = (void*)ctx; a.dctx = dctx; a.lse = (float*)lse; a.dq = dq; a.dk = dk_out; a.dv = dv;
     a.drop = fs2_make_dropout(seed, stream_id, rate);
     a.delta = (float*)workspace;
@@ -748,7 +754,7 @@ extern "C" int fs2_cross_attention_mass(const void* q, const void* k, const floa
     if (rc != FS2_OK) return rc;
     FS2_CHECK_ARG((lse || Mq == 0) && (mass || Mk == 0), "fs2_cross_attention_mass: null lse or mass");
     if (max_k == 0) return FS2_OK;
-    XArgs a = fs2_x_args(q, k, nullptr, cu_q, cu_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, 0, 0);
+    XArgs a = fs2_x_args(q, k, nullptr, cu_q, cu_k, max_q, max_k, Mq, Mk, n_heads, n_kv_heads, dk, ldq, ldk, 0, 0);
     a.lse = (float*)lse;
     a.mass = mass;
     a.nsplit = max_q > 0 ? x_mass_split(B, max_q, max_k, n_heads, dtype) : 1;

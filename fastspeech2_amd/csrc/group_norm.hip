@@ -739,7 +739,7 @@ extern "C" int fs2_group_norm(const void* x, const int* cu, const float* gamma, 
     FS2_CHECK_ARG(eps > 0.f, "fs2_group_norm: eps must be positive");
     const GnPlan p = gn_plan(B, max_len, C, groups, x_dtype, -1);
     FS2_CHECK_ARG(p.whole || workspace, "fs2_group_norm: this shape needs fs2_group_norm_workspace bytes");
-    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 30), "fs2_group_norm: too many workgroups (B=%d)", B);
+    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 22), "fs2_group_norm: too many workgroups (B=%d)", B);
     GnArgs a = gn_args(B, x, cu, gamma, beta, stats, workspace, max_len, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
     a.out = out; a.ldo = ldo; a.eps = eps;
     if (x_dtype == 0 && out_dtype == 0) gn_launch_fwd_r<float, float>(a, p, stream);
@@ -775,7 +775,7 @@ extern "C" int fs2_group_norm_bwd(const void* x, const float* stats, const int* 
                   "fs2_group_norm_bwd: ldd=%d (a multiple of %d), ldg=%d (of 4), or dout or dx unaligned", ldd, x_dtype == 0 ? 4 : 8,
                   ldg);
     const GnPlan p = gn_plan(B, max_len, C, groups, x_dtype, dout_dtype);
-    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 30), "fs2_group_norm_bwd: too many workgroups (B=%d)", B);
+    FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 22), "fs2_group_norm_bwd: too many workgroups (B=%d)", B);
     GnArgs a = gn_args(B, x, cu, gamma, beta, (float*)stats, workspace, max_len, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
     a.dout = dout; a.dx = dx; a.ldd = ldd; a.ldg = ldg;
 #define FS2_GN(TX, TD)                                              \

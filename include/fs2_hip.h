@@ -419,13 +419,14 @@ int fs2_bn_bwd(const float* y, const float* stats, const float* gamma, const flo
  * values, rows cu_k[b] .. cu_k[b+1] of k [Mk, ldk] and v [Mk, ldv].  n_heads query heads over n_kv_heads key / value heads
  * (n_kv_heads divides n_heads, at most 128 to one; head h reads shared head h / (n_heads / n_kv_heads)); head h sits at
  * columns h * dk of q and ctx, a shared head j at columns j * dk of k and v (a fused k | v projection: v = k + n_kv_heads * dk,
- * ldk = ldv).  dk in {32, 64, 96, 128}; T = fp32 or bf16; leading dims multiples of 16 bytes.
+ * ldk = ldv).  dk in {32, 64, 96, 128}; T = fp32 or bf16; leading dims multiples of 16 bytes, at most 2^20.
  *   ctx = dropout(softmax(q k^T / sqrt(dk))) v  [Mq, ldo] T;   lse [n_heads][Mq] (may be NULL): log2-domain log-sum-exp
- * An utterance without keys gets ctx = 0, lse = -inf; rows behind cu_q[B] are left as they were.  max_q / max_k: at least the
- * longest utterance of either side, at most Mq / Mk (queries beyond max_q of an utterance are not computed).  Serves one
+ * An utterance without keys gets ctx = 0, lse = -inf; rows in front of cu_q[0] and behind cu_q[B] are left as they were.
+ * max_q / max_k: at least the longest utterance of either side, at most Mq / Mk.  (A longer one is cut there, the results of its
+ * rows behind are undefined; offsets outside the matrices are clamped to them.)  Outputs overlap no input.  Serves one
  * query per utterance (autoregressive decoding against fixed encoder states) to whole batches; the kernel and a split of the
  * keys over workgroups follow from the shape.  Softmax statistics and sums are fp32; bf16 rounds the probabilities and the
- * result.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row = packed query row, col =
+ * result; fp32 products are exact to 2^-23, an infinite element of fp32 q, k or v counts as NaN.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row = packed query row, col =
  * key index inside the utterance; rate 0 = none).
  * workspace: fs2_cross_attention_workspace bytes, 16-byte aligned (0: NULL is fine).  It is written by every call: two calls
  * that may overlap (streams, captured graphs) need one each. */
@@ -436,7 +437,7 @@ int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, 
 
 /* Its backward, from ctx and lse as fs2_cross_attention left them and dctx [Mq, ldo] T: dq [Mq, ldq], dk_out [Mk, ldk],
  * dv [Mk, ldv] T (the leading dims of q, k, v; written, not added to; gradients of a shared head sum over its query heads).
- * Probabilities are recomputed; every element has one writer and every sum a fixed order.  workspace:
+ * Probabilities are recomputed; every element has one writer and every sum a fixed order (the same bits every time).  workspace:
  * fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, never NULL; one per call that may overlap. */
 long long fs2_cross_attention_bwd_workspace(int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk,
                                             int dtype);
@@ -461,7 +462,8 @@ int fs2_cross_attention_mass(const void* q, const void* k, const float* lse, flo
  * act 0 none, 1 ReLU, 2 tanh, 3 SiLU; dropout element (site, row, col) as in the other training kernels.  stats
  * [B][groups][2] = mean, 1 / sqrt(var + eps) (0, 1 / sqrt(eps) for an utterance without rows).  Dtypes 0 fp32, 1 bf16, each on
  * its own; C % 4 == 0 (fp32 x) or 8 (bf16 x), C <= 1024, any group size; ldo % 4 == 0.  The per-utterance counterpart of
- * fs2_bn_stats + fs2_bn_apply: a batch row equals the utterance alone.  Statistics in fp32 from centred squares.
+ * fs2_bn_stats + fs2_bn_apply: a batch row equals the utterance alone.  Statistics in fp32 from centred squares.  Rows that no
+ * utterance owns are left as they were, one longer than max_len is cut there; at most 2^22 utterances (less where they are long).
  * workspace: fs2_group_norm_workspace bytes (0: NULL is fine). */
 long long fs2_group_norm_workspace(int B, int max_len, int C, int groups);
 int fs2_group_norm(const void* x, const int* cu, const float* gamma, const float* beta, void* out, float* stats, void* workspace,

@@ -56,7 +56,7 @@ def _back(change):
 
 @pytest.mark.parametrize("change,text", [
     (dict(v=None), "null or unaligned v"), (dict(ctx=P + 4), "null or unaligned v or ctx"), (dict(ldv=120), "ldv=120"),
-    (dict(ldo=252), "ldo=252"), (dict(rate=1.0), "dropout rate"), (dict(rate=-0.1), "dropout rate"),
+    (dict(ldo=252), "ldo=252"), (dict(ldo=(1 << 20) + 8), "ldo=1048584"), (dict(rate=1.0), "dropout rate"), (dict(rate=-0.1), "dropout rate"),
     (dict(B=1, max_q=1, Mq=1, max_k=4000, Mk=4000, ws=None), "fs2_cross_attention_workspace bytes"),
     (dict(B=1, max_q=1, Mq=1, max_k=4000, Mk=4000, ws=P + 8), "fs2_cross_attention_workspace bytes"),
 ])
@@ -67,7 +67,7 @@ def test_cross_attention_forward_refuses(change, text):
 
 @pytest.mark.parametrize("change,text", [
     (dict(ctx=None), "null argument"), (dict(lse=None), "null argument"), (dict(v=None), "null argument"),
-    (dict(ctx=P + 4), "unaligned"), (dict(ldv=120), "ldv=120"), (dict(rate=1.5), "dropout rate"), (dict(ws=None), "workspace bytes"),
+    (dict(ctx=P + 4), "unaligned"), (dict(ldv=120), "ldv=120"), (dict(ldo=1 << 28), "ldo=268435456"), (dict(rate=1.5), "dropout rate"), (dict(ws=None), "workspace bytes"),
     (dict(ws=P + 4), "workspace bytes"),
 ])
 def test_cross_attention_backward_refuses(change, text):
@@ -101,6 +101,7 @@ NORM_REFUSED = [
     (dict(x=None), "bad args"), (dict(B=0), "bad args"), (dict(max_len=17), "max_len=17"), (dict(x_dtype=2), "x_dtype=2"),
     (dict(C=82, G=2), "C=82"), (dict(C=84, G=2, x_dtype=1), "C=84"), (dict(C=1040, ldx=1040, ldo=1040), "C=1040"), (dict(G=3), "80 channels in 3"),
     (dict(ldx=76), "ldx=76"), (dict(ldx=82), "ldx=82"), (dict(x=P + 8), "unaligned"), (dict(act=4), "act=4"), (dict(rate=1.0), "dropout"),
+    (dict(B=1 << 23), "too many workgroups"),
 ]
 
 

@@ -186,6 +186,7 @@ SHAPES = [
     ([40], [900], 2, 2, 64, 0),                                    # few rows, long keys: split and merged
     ([17, 30, 0], [0, 1030, 5], 4, 4, 128, 0),
     ([700], [301], 2, 1, 128, 8),
+    ([2, 1], [20000, 17], 2, 1, 96, 0),                            # more than 32 key ranges for a few rows
 ]
 
 
@@ -210,7 +211,8 @@ def test_cross_attention(lq, lk, H, KV, dk, pad, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
-@pytest.mark.parametrize("lq,lk,H,KV,dk", [([90, 33], [70, 40], 4, 2, 64), ([1, 1], [40, 100], 4, 1, 128), ([30], [700], 2, 2, 96)])
+@pytest.mark.parametrize("lq,lk,H,KV,dk", [([90, 33], [70, 40], 4, 2, 64), ([1, 1], [40, 100], 4, 1, 128), ([30], [700], 2, 2, 96),
+                                           ([400, 3], [301, 9], 4, 2, 128), ([1, 2], [1500, 40], 4, 2, 32)])
 def test_cross_attention_dropout(lq, lk, H, KV, dk, dtype):
     drop = (12345, 9, 0.25)
     p = Problem(lq, lk, H, KV, dk, dtype, seed=4)
@@ -322,6 +324,54 @@ def test_offsets_outside_the_matrices_touch_nothing():
     dkv = torch.full((p.Mk + 64, p.ldk), 7.0, dtype=torch.bfloat16, device=DEV)
     p.backward(ctx, lse, dkv=dkv)
     assert (dkv[p.Mk:] == 7.0).all()
+
+
+@pytest.mark.parametrize("lq,lk", [([70, 20], [50, 33]), ([1, 1], [3000, 40]), ([30, 50], [900, 700])])
+def test_rows_in_front_of_the_first_utterance(lq, lk):
+    """offsets that begin behind row 0: the rows in front of them keep their values, the others the results of a batch without them"""
+    p = Problem(lq, lk, 2, 2, 64, "bf16", seed=3)
+    lead = Problem([5] + lq, [7] + lk, 2, 2, 64, "bf16", seed=3)
+    for name, n in (("q", 5), ("kv", 7), ("dctx", 5)):
+        lead.d[name][n:] = p.d[name]
+        lead.d[name][:n] = math.nan
+    lead.cu_q, lead.cu_k, lead.B, lead.max_q, lead.max_k = lead.cu_q[1:].clone(), lead.cu_k[1:].clone(), 2, max(lq), max(lk)
+    ctx, lse = p.forward()
+    got, glse = lead.forward()
+    assert torch.equal(got[5:], ctx) and torch.equal(glse[:, 5:], lse) and (got[:5] == 7.0).all() and (glse[:, :5] == 7.0).all()
+    dq, dkv = p.backward(ctx, lse)
+    gq, gkv = lead.backward(got, glse)
+    assert torch.equal(gq[5:], dq) and torch.equal(gkv[7:], dkv) and (gq[:5] == 7.0).all() and (gkv[:7] == 7.0).all()
+    m, gm = p.mass(lse), lead.mass(glse)
+    assert torch.equal(gm[:, 7:], m) and (gm[:, :7] == 7.0).all()
+
+
+def test_utterances_longer_than_announced_are_cut():
+    """max_q, max_k below the longest: what is computed is that of the cut utterances, no other row is touched"""
+    full = Problem([100, 60], [80, 30], 4, 2, 64, "bf16", seed=5)
+    full.max_q, full.max_k = 60, 30
+    cut = Problem([60, 60], [30, 30], 4, 2, 64, "bf16", seed=5)
+    for name, c, n in (("q", full.cq, 60), ("kv", full.ck, 30), ("dctx", full.cq, 60)):
+        for b in range(2):
+            cut.d[name][b * n:(b + 1) * n] = full.d[name][c[b]:c[b] + n]
+    ctx, lse = cut.forward()
+    dq, dkv = cut.backward(ctx, lse)
+    got, glse = full.forward()
+    gq, gkv = full.backward(got, glse)
+    m, gm = cut.mass(lse), full.mass(glse)
+    for b in range(2):
+        rq, sq = slice(b * 60, b * 60 + 60), slice(full.cq[b], full.cq[b] + 60)
+        rk, sk = slice(b * 30, b * 30 + 30), slice(full.ck[b], full.ck[b] + 30)
+        assert torch.equal(got[sq], ctx[rq]) and torch.equal(glse[:, sq], lse[:, rq]) and torch.equal(gq[sq], dq[rq])
+        assert torch.equal(gkv[sk], dkv[rk]) and torch.equal(gm[:, sk], m[:, rk])
+    assert (got[60:100] == 7.0).all() and (gq[60:100] == 7.0).all() and (gkv[30:80] == 7.0).all() and (gm[:, 30:80] == 7.0).all()
+
+
+def test_mass_of_a_broken_query_is_nan():
+    p = Problem([20, 9], [30, 12], 2, 2, 64, "fp32", seed=4)
+    clean = p.mass(p.forward()[1])
+    p.d["q"][3] = math.nan
+    m = p.mass(p.forward()[1])
+    assert torch.isnan(m[:, :30]).all() and torch.equal(m[:, 30:42], clean[:, 30:42])
 
 
 # ---------------------------------------------------------------------------------------------------------- group norm
@@ -541,6 +591,50 @@ def test_other_stream_and_two_graphs():
             p.forward()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(outs, w))
+
+
+@pytest.mark.parametrize("lens", [[70, 0, 33], [9000, 20]])
+def test_group_norm_in_a_graph(lens):
+    """the forms that hold an utterance and that cut it into chunks: captured, replayed with eager calls between; rows in front of the
+    first utterance and behind an announced length keep their values"""
+    p = Norm(lens, 64, 4, "silu", "bf16", seed=2)
+    p.dout = p.dout.to(DEV)                      # (no copy from the host while capturing)
+    drop = (5, 6, 0.1)
+    y, st = p.forward("bf16", drop)
+    want = [y, st, *p.backward(st, "bf16", "bf16", drop)]
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y, st = p.forward("bf16", drop)
+        out = [y, st, *p.backward(st, "bf16", "bf16", drop)]
+    for _ in range(3):
+        for o in out:
+            o.fill_(3.0)
+        gr.replay()
+        p.forward("bf16")
+        torch.cuda.synchronize()
+        for got, w in zip(out, want):
+            assert torch.equal(got[:sum(lens)], w[:sum(lens)]) if got.shape[0] == p.M else torch.equal(got, w)
+
+
+def test_group_norm_rows_of_nobody():
+    """offsets that begin behind row 0 and an utterance longer than announced"""
+    p = Norm([50, 40], 96, 4, "tanh", "fp32", seed=1)
+    cut = Norm([40, 40], 96, 4, "tanh", "fp32", seed=1)
+    p.xd = torch.cat([torch.full((4, p.ld), math.nan, device=DEV), p.xd])
+    p.dout = torch.cat([torch.full((4, p.ld), math.nan), p.dout])
+    cut.gd, cut.bd = p.gd, p.bd
+    cut.xd[:40], cut.xd[40:80] = p.xd[4:44], p.xd[54:94]
+    cut.dout[:40], cut.dout[40:80] = p.dout[4:44], p.dout[54:94]
+    p.cu, p.M, p.lens = p.cu + 4, p.M + 4, [40, 40]
+    y, st = p.forward("fp32")
+    w, wst = cut.forward("fp32")
+    assert torch.equal(st, wst) and torch.equal(y[4:44], w[:40]) and torch.equal(y[54:94], w[40:80])
+    dx, dg, db = p.backward(st, "fp32", "fp32")
+    wx, wg, wb = cut.backward(wst, "fp32", "fp32")
+    assert torch.equal(dg, wg) and torch.equal(db, wb) and torch.equal(dx[4:44], wx[:40]) and torch.equal(dx[54:94], wx[40:80])
+    for t in (y, dx):
+        assert (t[:4] == 7.0).all() and (t[44:54] == 7.0).all() and (t[94:] == 7.0).all()
 
 
 def test_aligner_step_end_to_end():
