@@ -24,6 +24,8 @@ struct XArgs {
     float scale_log2e;   // log2(e) / sqrt(dk)
     float scale;         // 1 / sqrt(dk)
     int nblk, pairs;     // blocks of a pair, (utterance, head) pairs: see x_decode
+    int nblk_q;          // backward: row blocks of a pair, and the workgroups in front of the row blocks'
+    unsigned key_groups;
     unsigned kv_magic;   // 1 / heads-per-utterance of the pair index
     Dropout drop;        // dropout of the probabilities: site drop.stream + head, row = packed query row, col = key index
     int nsplit;          // ranges of the summed axis over workgroups (1: none), partial results to `part`
@@ -45,10 +47,13 @@ __device__ __forceinline__ void x_range(const int* cu, int b, int M, int longest
     r0 = c0;
     len = min(c1 - c0, longest);
 }
-// rows that some utterance owns, [first, end)
-__device__ __forceinline__ void x_owned(const int* cu, int B, int M, int& first, int& end) {
-    first = min(max(cu[0], 0), M);
-    end = min(max(cu[B], first), M);
+// row `slot % longest` of utterance `slot / longest`, -1 if it has none: the rows that the launches behind a split work on
+__device__ __forceinline__ int x_row_of(const int* cu, int M, int longest, unsigned slot) {
+    const unsigned b = slot / (unsigned)longest;
+    int r0, len;
+    x_range(cu, (int)b, M, longest, r0, len);
+    const int i = (int)(slot - b * (unsigned)longest);
+    return i < len ? r0 + i : -1;
 }
 // packed row -> query index inside the utterance; head in group = r - q * g
 __device__ __forceinline__ int x_query(const XArgs& a, int r) { return a.g == 1 ? r : (int)__umulhi((unsigned)r, a.magic); }
@@ -69,6 +74,19 @@ __device__ __forceinline__ bool x_decode(const XArgs& a, int heads, int& b, int&
     if (pair >= a.pairs) return false;
     b = heads == 1 ? pair : (int)__umulhi((unsigned)pair, a.kv_magic);       // pair < 2^24, heads <= 4096: exact
     h = pair - b * heads;
+    return true;
+}
+
+// the same order from the id in a one-dimensional grid of `nblk` blocks to a pair
+__device__ __forceinline__ bool x_decode_line(const XArgs& a, unsigned id, unsigned nblk, int& b, int& h, int& blk, int& split) {
+    const unsigned ny = a.pairs >= 8 ? (unsigned)(a.pairs + 7) >> 3 : (unsigned)a.pairs, t = a.pairs >= 8 ? id >> 3 : id;
+    const unsigned u = t / nblk;
+    blk = (int)(t - u * nblk);
+    split = (int)(u / ny);
+    const int y = (int)u - split * (int)ny, pair = a.pairs >= 8 ? y * 8 + (int)(id & 7) : y;
+    if (pair >= a.pairs) return false;
+    b = a.KV == 1 ? pair : (int)__umulhi((unsigned)pair, a.kv_magic);
+    h = pair - b * a.KV;
     return true;
 }
 

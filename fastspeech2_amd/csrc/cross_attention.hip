@@ -393,16 +393,15 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
     }
 }
 
-// Merge of the key ranges, many rows: one lane per (row, four channels), the few ranges in a loop.  Rows [cu_q[0], cu_q[B]) only: the
-// others were computed by nobody.  A range without keys wrote no partial context (its sum is 0): read, not used.
+// Merge of the key ranges, many rows: one lane per (row, four channels), the few ranges in a loop.  A range without keys wrote no
+// partial context (its sum is 0): read, not used.
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int dk) {
     const int d = a.H * dk, dv = d >> 2;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    int r0, r1;
-    x_owned(a.cu_q, B, a.Mq, r0, r1);
-    if (idx >= (long long)(r1 - r0) * dv) return;
-    const int m = r0 + (int)(idx / dv), c = (int)(idx % dv) * 4, h = c / dk;
+    const unsigned idx = blockIdx.x * 256 + threadIdx.x, slot = idx / (unsigned)dv;
+    if (slot >= (unsigned)B * (unsigned)a.max_q) return;
+    const int m = x_row_of(a.cu_q, a.Mq, a.max_q, slot), c = (int)(idx - slot * (unsigned)dv) * 4, h = c / dk;
+    if (m < 0) return;
     const float* ml = a.part + (size_t)a.nsplit * a.Mq * d + ((size_t)h * a.Mq + m) * 2;
     const size_t step = (size_t)a.H * a.Mq * 2;
     float mx = -INFINITY;
@@ -430,14 +429,12 @@ __global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int 
 // (1024 / dk)th range.  One lane for all ranges waited for 32 loads in a row (15 us of the 21 us of one frame over 65000 keys).
 constexpr int X_MAX_SPLIT = 256;
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void xattn_combine_few_kernel(XArgs a, int B) {
+__global__ __launch_bounds__(256) void xattn_combine_few_kernel(XArgs a) {
     constexpr int SL = DK / 4, NL = 256 / SL;
     __shared__ float ms[X_MAX_SPLIT], ls[X_MAX_SPLIT];
     __shared__ __attribute__((aligned(16))) float red[NL][DK];
-    int r0, r1;
-    x_owned(a.cu_q, B, a.Mq, r0, r1);
-    const int h = blockIdx.x, m = r0 + blockIdx.y, tid = threadIdx.x;
-    if (m >= r1) return;
+    const int h = blockIdx.x, m = x_row_of(a.cu_q, a.Mq, a.max_q, blockIdx.y), tid = threadIdx.x;
+    if (m < 0) return;
     const size_t d = (size_t)a.H * DK;
     if (tid < a.nsplit) {
         const float2 t = *(const float2*)(a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)tid * a.H + h) * a.Mq + m) * 2);
@@ -535,9 +532,9 @@ static int launch_xattn(XArgs& a, const XPlan& p, int B, int max_q, int dk, hipS
     }
     FS2_CHECK_LAUNCH("fs2_cross_attention");
     if (a.nsplit > 1) {
-        const long long most = (long long)B * max_q, rows = most < a.Mq ? most : a.Mq, n = rows * (a.H * dk / 4);
+        const long long rows = (long long)B * max_q, n = rows * (a.H * dk / 4);         // (both small where keys are split)
         if (p.few)
-            hipLaunchKernelGGL((xattn_combine_few_kernel<T, DK>), dim3(a.H, (unsigned)rows), dim3(256), 0, stream, a, B);
+            hipLaunchKernelGGL((xattn_combine_few_kernel<T, DK>), dim3(a.H, (unsigned)rows), dim3(256), 0, stream, a);
         else
             hipLaunchKernelGGL(xattn_combine_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B, dk);
         FS2_CHECK_LAUNCH("fs2_cross_attention(merge)");

@@ -1,10 +1,10 @@
 // Backward of cross attention (cross_attention.hip) and the attention mass of every key; the probabilities are recomputed tile
 // by tile from q, k and the saved log-sum-exp, never stored.  With S = q k^T / sqrt(dk), P = exp2(S log2 e - lse), D the
 // dropout multiplier, O = (P o D) v and upstream dO:
-//   delta = sum_dv dO o O
-//   dP = dO v^T o D,  dS = P o (dP - delta)
-//   dq = dS k / sqrt(dk)                                          xattn_dq_kernel: one wave per 16 packed rows
-//   dk = dS^T q / sqrt(dk),  dv = (P o D)^T dO                    xattn_dkv32_kernel (bf16), xattn_dkv_kernel (fp32)
+//   delta = sum_dv dO o O                                         xattn_delta_kernel
+//   dP = dO v^T o D,  dS = P o (dP - delta)                       xattn_bwd_kernel, two kinds of workgroups:
+//   dq = dS k / sqrt(dk)                                            x_dq_block: one wave per 16 packed rows
+//   dk = dS^T q / sqrt(dk),  dv = (P o D)^T dO                      x_dkv32_block (bf16), x_dkv_block (fp32)
 //   mass[h][key] = sum_q P                                        xattn_mass_kernel
 // The packed rows of a shared head are its g query heads, so the sum over the group that dk and dv need is part of the loop.
 // Every output element has one writer and every sum a fixed order: no atomics, the same bits every time.
@@ -12,24 +12,29 @@
 
 namespace fs2 {
 
-// Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16 (floor of the whole step 11.8 us): dq 22 us,
-// dk and dv 28 us; and of 3 x 1601 frames over 301 phones, 4 heads on 2 of 96, fp32 (floor 47.7): 43 and 46 + 6.5 us.
+// Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16: delta 6.4 us for 27 MB (4.2 TB/s), the rest 37 us
+// (floor of the whole step, forward included, 11.8 us); 3 x 1601 frames over 301 phones, 4 heads on 2 of 96, fp32: 5 + 78 + 5.5 us for
+// 4.9 GFLOP (floor 47.7 with the forward).
 
-// ---- dq and delta: one workgroup per (utterance, shared head, 64 packed rows) -------------------------------------
-// 832 workgroups of four waves, two to a CU (registers, and 80 KB of LDS at dk = 128): a second round that half fills the chip, and in
-// each two key tiles behind a wait for the rows.  dS as two numbers is 2 of the 22 us.
-template <typename E, int DK, bool DROP>
-__global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
+template <typename T> __device__ __forceinline__ f32x4 x_load4(const T* p) {
+    if constexpr (sizeof(T) == 4) return *(const f32x4*)p;
+    const bf16x4 v = *(const bf16x4*)p;
+    return (f32x4){(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+
+// ---- dq: one workgroup per (utterance, shared head, 64 packed rows) -------------------------------------
+// Two key tiles behind a wait for the rows, in each of 832 workgroups (32 x 800 rows, 2 heads): latency.  dS as two numbers is 2 of the 22
+// us that these took in a launch of their own.
+template <typename E, int DK, bool DROP> __device__ __forceinline__ void x_dq_block(const XArgs& a, unsigned id, unsigned char* smem) {
     typedef typename E::mem T;
     constexpr int KB = x_kb<E>(), NT = KB / 16, NC = KB / 32, NST = E::PL == 1 ? 2 : 1;
     typedef XTile<E, DK, KB, 2> TK;
     typedef XTile<E, DK, KB, 1> TV;
     typedef typename TK::frag_t frag_t;
     constexpr int KS = TK::KS, DT = TK::DT, STAGE = TK::BYTES + TV::BYTES;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // stage s: K tile (read both ways), V tile
-
+    // smem: stage s: K tile (read both ways), V tile
     int b, kvh, blk, split;
-    if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
+    if (!x_decode_line(a, id, a.nblk_q, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
     x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
@@ -53,19 +58,16 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
     };
     if (lenk > 0) fetch(0, 0);
 
-    // q, dO and ctx rows of the wave: bf16 in the other stage and behind it, all under way together; fp32 one after the other
+    // q and dO rows of the wave: bf16 in the other stage, both under way together; fp32 one after the other
     frag_t qf[KS], dof[KS];
-    float del = 0.f;
     {
         typedef XTile<E, DK, 16, 1> TQ;
         unsigned char* own = smem + (NST == 2 ? STAGE : 0) + wave * TQ::BYTES;
         constexpr int NEXT = E::PL == 1 ? 4 * TQ::BYTES : 0;
         const int first = min(blk * 64 + wave * 16, nrow - 1);
-        const size_t at = (size_t)q0 * a.ldq + kvh * a.g * DK, ato = (size_t)q0 * a.ldo + kvh * a.g * DK;
-        XRows<E, DK, 16> rq(a.ldq, lane), rd(a.ldo, lane), rc(a.ldo, lane);
-        rq.start(a, (const T*)a.q + at, a.ldq, first, nrow, own, lane);
-        rd.start(a, (const T*)a.dctx + ato, a.ldo, first, nrow, own + NEXT, lane);
-        rc.start(a, (const T*)a.ctx + ato, a.ldo, first, nrow, own + 2 * NEXT, lane);
+        XRows<E, DK, 16> rq(a.ldq, lane), rd(a.ldo, lane);
+        rq.start(a, (const T*)a.q + (size_t)q0 * a.ldq + kvh * a.g * DK, a.ldq, first, nrow, own, lane);
+        rd.start(a, (const T*)a.dctx + (size_t)q0 * a.ldo + kvh * a.g * DK, a.ldo, first, nrow, own + NEXT, lane);
         rq.finish(own, lane);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qf[ks] = TQ::row_frag(own, i, ks, g);
@@ -75,19 +77,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) dof[ks] = TQ::row_frag(own + NEXT, i, ks, g);
-        if constexpr (E::PL == 3) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            rc.finish(own, lane);
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const frag_t of = TQ::row_frag(own + 2 * NEXT, i, ks, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) del = fmaf(x_value<E>(dof[ks], j), x_value<E>(of, j), del);
-        }
     }
-    del = rows_sum(del);
-    if (g == 0 && r < nrow) a.delta[(size_t)head * a.Mq + qrow] = del;
+    const float del = a.delta[(size_t)head * a.Mq + qrow];
     const float lse_q = a.lse[(size_t)head * a.Mq + qrow];
 
     f32x4 dq[DT];
@@ -176,17 +167,15 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XArgs a) {
 // fp32: one workgroup per (utterance, shared head, 64 keys, range of packed rows), a wave to 16 keys, its K and V operands in
 // registers; row tiles of 32 in LDS for all four, split into planes once for all (a wave with a tile of its own, as in bf16, would
 // split each for itself).  Bound by what a tile costs a SIMD in turn: MFMA, splits, LDS.
-template <int DK, bool DROP>
-__global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs a) {
+template <int DK, bool DROP> __device__ __forceinline__ void x_dkv_block(const XArgs& a, unsigned id, unsigned char* smem) {
     typedef XF32 E;
     typedef float T;
     typedef XTile<E, DK, 32, 2> TL;
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // Q tile, dO tile (read both ways), 32 lse, 32 delta
-
+    // smem: Q tile, dO tile (read both ways), 32 lse, 32 delta
     int b, kvh, blk, split;
-    if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
+    if (!x_decode_line(a, id, a.nblk, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
     x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
@@ -299,8 +288,7 @@ __global__ __launch_bounds__(256, DK == 128 ? 1 : 2) void xattn_dkv_kernel(XArgs
 // writes the gradients several times over as partial sums (27 + 5 us, before dS became two numbers; this form then 25.6).  A second
 // buffer for each wave would overlap its tiles' DMA and products, but leaves one workgroup to a CU where there are slightly more
 // workgroups than CUs: 41 us against 28.
-template <int DK, bool DROP>
-__global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
+template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const XArgs& a, unsigned id, unsigned char* smem) {
     typedef XB16 E;
     typedef bf16_t T;
     typedef XTile<E, DK, 32, 2> TL;
@@ -309,10 +297,9 @@ __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
     typedef typename TL::frag_t frag_t;
     constexpr int KS = TL::KS, DT = TL::DT, NP = TK::BYTES / 1024, NWK = NP % 4 == 0 ? 4 : (NP % 2 == 0 ? 2 : 1);
     constexpr int WAVE = 2 * TL::BYTES;                  // a wave's Q tile, dO tile: 80 KB in all at dk = 128, two workgroups per CU
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // K tile, V tile, then the waves'
-
+    // smem: K tile, V tile, then the waves'
     int b, kvh, blk, split;
-    if (!x_decode(a, a.KV, b, kvh, blk, split)) return;
+    if (!x_decode_line(a, id, a.nblk, b, kvh, blk, split)) return;
     int q0, lenq, k0, lenk;
     x_range(a.cu_q, b, a.Mq, a.max_q, q0, lenq);
     x_range(a.cu_k, b, a.Mk, a.max_k, k0, lenk);
@@ -465,17 +452,58 @@ __global__ __launch_bounds__(256, 2) void xattn_dkv32_kernel(XArgs a) {
     }
 }
 
+// Both in one launch, the longer key workgroups first: alone, the row workgroups ended in a half-filled second round and the key
+// workgroups, hardly more than CUs, left half of every CU.  32 x 800 over 120, 2 heads of 128, bf16: 37 + 6.4 us (delta, which both
+// need, has become a launch) against 22 + 28; 8 x 3100 over 512: 89 + 6 against 45 + 81; 3 x 1601 over 301, fp32, dk = 96: 78 + 5
+// against 46 + 47.
+template <typename E, int DK, bool DROP>
+__global__ __launch_bounds__(256, E::PL == 3 && DK == 128 ? 1 : 2) void xattn_bwd_kernel(XArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    if (blockIdx.x >= a.key_groups) x_dq_block<E, DK, DROP>(a, blockIdx.x - a.key_groups, smem);
+    else if constexpr (E::PL == 1) x_dkv32_block<DK, DROP>(a, blockIdx.x, smem);
+    else x_dkv_block<DK, DROP>(a, blockIdx.x, smem);
+}
+
+// delta: 16 lanes to a row and up to X_DELTA_HEADS of its heads, four elements at a time
+constexpr int X_DELTA_HEADS = 2;
+template <typename T, int DK> __global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a, int B) {
+    const unsigned per = (unsigned)(a.H + X_DELTA_HEADS - 1) / X_DELTA_HEADS;
+    const unsigned id = blockIdx.x * 16 + (threadIdx.x >> 4), slot = id / per;
+    if (slot >= (unsigned)B * (unsigned)a.max_q) return;
+    const int m = x_row_of(a.cu_q, a.Mq, a.max_q, slot), lane = threadIdx.x & 15, h0 = (int)(id - slot * per) * X_DELTA_HEADS;
+    if (m < 0) return;
+    float s[X_DELTA_HEADS];
+#pragma unroll
+    for (int u = 0; u < X_DELTA_HEADS; ++u) {                 // (the last head again where there are fewer: no branch between the loads)
+        const size_t at = (size_t)m * a.ldo + min(h0 + u, a.H - 1) * DK;
+        s[u] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DK; c += 64) {
+            const int e = c + lane * 4;
+            if (DK % 64 == 0 || e < DK) {
+                const f32x4 o = x_load4((const T*)a.ctx + at + e), d = x_load4((const T*)a.dctx + at + e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[u] = fmaf(o[j], d[j], s[u]);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < X_DELTA_HEADS; ++u) {
+        s[u] = row16_sum(s[u]);
+        if (lane == 0 && h0 + u < a.H) a.delta[(size_t)(h0 + u) * a.Mq + m] = s[u];
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int dk) {
-    const int w = a.KV * dk, wv = w >> 2;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    int r0, r1;
-    x_owned(a.cu_k, B, a.Mk, r0, r1);
-    const long long n = (long long)(r1 - r0) * wv;
-    if (idx >= 2 * n) return;
-    const bool is_v = idx >= n;
-    const long long e = is_v ? idx - n : idx;
-    const int m = r0 + (int)(e / wv), c = (int)(e % wv) * 4;
+    const int w = a.KV * dk;
+    const unsigned wv = (unsigned)w >> 2, idx = blockIdx.x * 256 + threadIdx.x, slot = idx / (2 * wv);
+    if (slot >= (unsigned)B * (unsigned)a.max_k) return;
+    const int m = x_row_of(a.cu_k, a.Mk, a.max_k, slot);
+    if (m < 0) return;
+    const unsigned e = idx - slot * 2 * wv;
+    const bool is_v = e >= wv;
+    const int c = (int)(is_v ? e - wv : e) * 4;
     const size_t half = (size_t)a.Mk * w;
     const float* src = a.part + (is_v ? half : 0) + (size_t)m * w + c;
     f32x4 sum = *(const f32x4*)src;
@@ -587,24 +615,24 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
 }
 
 __global__ __launch_bounds__(256) void xattn_mass_sum_kernel(XArgs a, int B) {
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    int r0, r1;
-    x_owned(a.cu_k, B, a.Mk, r0, r1);
-    const int rows = r1 - r0;
-    if (idx >= (long long)a.H * rows) return;
-    const size_t at = (size_t)(idx / rows) * a.Mk + r0 + idx % rows, step = (size_t)a.H * a.Mk;
+    const unsigned idx = blockIdx.x * 256 + threadIdx.x, n = (unsigned)B * (unsigned)a.max_k, h = idx / n;
+    if (h >= (unsigned)a.H) return;
+    const int m = x_row_of(a.cu_k, a.Mk, a.max_k, idx - h * n);
+    if (m < 0) return;
+    const size_t at = (size_t)h * a.Mk + m, step = (size_t)a.H * a.Mk;
     float sum = a.part[at];
     for (int s = 1; s < a.nsplit; ++s) sum += a.part[s * step + at];
     a.mass[at] = sum;
 }
 
-// Row ranges of the key kernels, chosen from the shape: a workgroup for every CU where the keys alone do not give one, and at least
-// four row tiles to a wave (bf16) or to the workgroup (fp32).  More would only add partial sums.
+// Row ranges of the key workgroups, chosen from the shape: one workgroup for every CU where the keys alone do not give one (the row
+// workgroups fill the rest: 8 x 800 over 120, fp32, dk = 128: 47 us against 54 with two to a CU), and at least two row tiles to a wave
+// (bf16) or four to the workgroup (fp32).  More would only add partial sums.
 static int x_dkv_split(int B, int max_q, int max_k, int H, int KV, int dtype) {
     const int kb = dtype == 1 ? 32 : 64;
     const long items = (long)B * KV * ((max_k + kb - 1) / kb), tiles = ((long)max_q * (H / KV) + 31) / 32;
-    if (items >= 192 || tiles < 8) return 1;
-    const long want = 512 / items, most = dtype == 1 ? tiles / 8 : tiles / 4, n = want < most ? want : most;
+    if (items >= 128 || tiles < 8) return 1;
+    const long want = 256 / items, most = dtype == 1 ? tiles / 8 : tiles / 4, n = want < most ? want : most;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
 constexpr int x_mass_kt(int dtype) { return dtype == 1 ? 4 : 2; }
@@ -616,55 +644,41 @@ static int x_mass_split(int B, int max_q, int max_k, int H, int dtype) {
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
 }
 
-template <typename E, int DK, bool DROP> static void launch_xattn_dq(const XArgs& a, dim3 grid, hipStream_t stream) {
+template <typename E, int DK, bool DROP> static void launch_xattn_bwd_kernel(const XArgs& a, unsigned grid, hipStream_t stream) {
     constexpr int KB = x_kb<E>(), stage = XTile<E, DK, KB, 1>::BYTES + XTile<E, DK, KB, 2>::BYTES;
-    constexpr int rows = (E::PL == 1 ? 12 : 4) * XTile<E, DK, 16, 1>::BYTES, out = 4 * x_out_bytes<typename E::mem, DK>();
-    constexpr int tiles = E::PL == 1 ? stage + (stage > rows ? stage : rows) : (stage > rows ? stage : rows), lds = tiles > out ? tiles : out;
+    constexpr int rows = (E::PL == 1 ? 8 : 4) * XTile<E, DK, 16, 1>::BYTES, out = 4 * x_out_bytes<typename E::mem, DK>();
+    constexpr int tiles = E::PL == 1 ? stage + (stage > rows ? stage : rows) : (stage > rows ? stage : rows), dq = tiles > out ? tiles : out;
+    constexpr int key_tiles = E::PL == 1 ? 8 * XTile<E, DK, 32, 2>::BYTES + 2 * XTile<E, DK, 32, 1>::BYTES : 2 * XTile<E, DK, 32, 2>::BYTES + 256;
+    constexpr int merge = E::PL == 1 ? 4 * 32 * (DK + 4) * 4 : 0, dkv = key_tiles > merge ? key_tiles : merge, lds = dq > dkv ? dq : dkv;
     static unsigned long long ok = 0;
-    fs2_allow_lds((const void*)xattn_dq_kernel<E, DK, DROP>, lds, &ok);
-    hipLaunchKernelGGL((xattn_dq_kernel<E, DK, DROP>), grid, dim3(256), lds, stream, a);
-}
-template <int DK, bool DROP> static void launch_xattn_dkv(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int lds = 2 * XTile<XF32, DK, 32, 2>::BYTES + 256;
-    static unsigned long long ok = 0;
-    fs2_allow_lds((const void*)xattn_dkv_kernel<DK, DROP>, lds, &ok);
-    hipLaunchKernelGGL((xattn_dkv_kernel<DK, DROP>), grid, dim3(256), lds, stream, a);
-}
-template <int DK, bool DROP> static void launch_xattn_dkv32(const XArgs& a, dim3 grid, hipStream_t stream) {
-    constexpr int tiles = 8 * XTile<XB16, DK, 32, 2>::BYTES + 2 * XTile<XB16, DK, 32, 1>::BYTES, merge = 4 * 32 * (DK + 4) * 4;
-    constexpr int lds = tiles > merge ? tiles : merge;
-    static unsigned long long ok = 0;
-    fs2_allow_lds((const void*)xattn_dkv32_kernel<DK, DROP>, lds, &ok);
-    hipLaunchKernelGGL((xattn_dkv32_kernel<DK, DROP>), grid, dim3(256), lds, stream, a);
+    fs2_allow_lds((const void*)xattn_bwd_kernel<E, DK, DROP>, lds, &ok);
+    hipLaunchKernelGGL((xattn_bwd_kernel<E, DK, DROP>), dim3(grid), dim3(256), lds, stream, a);
 }
 
 template <typename E, int DK>
 static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipStream_t stream) {
     typedef typename E::mem T;
-    if (max_q > 0) {
-        XArgs b = a;
-        b.nsplit = 1;
-        const dim3 grid = fs2_x_grid(b, (max_q * a.g + 63) / 64, a.KV, B);
-        if (a.drop.thresh) launch_xattn_dq<E, DK, true>(b, grid, stream);
-        else launch_xattn_dq<E, DK, false>(b, grid, stream);
-        FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(dq)");
+    constexpr int KEYS = E::PL == 1 ? 32 : 64;
+    const long long nq = ((long long)max_q * a.g + 63) / 64, nk = (max_k + KEYS - 1) / KEYS;
+    fs2_x_grid(a, (int)nk, a.KV, B);
+    const long long line = a.pairs >= 8 ? (a.pairs + 7) / 8 * 8 : a.pairs;
+    const long long rows = (long long)B * max_q * a.H, delta = (long long)B * max_q * ((a.H + X_DELTA_HEADS - 1) / X_DELTA_HEADS);
+    FS2_CHECK_ARG(rows <= (1 << 28) && line * (nk * a.nsplit + nq) < (1 << 24),
+                  "fs2_cross_attention_bwd: B=%d x %d heads x max_q=%d or max_k=%d in one launch", B, a.H, max_q, max_k);
+    if (rows > 0 && max_k > 0) {
+        hipLaunchKernelGGL((xattn_delta_kernel<T, DK>), dim3((unsigned)((delta + 15) / 16)), dim3(256), 0, stream, a, B);
+        FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(delta)");
     }
-    if (max_k > 0) {
-        if constexpr (E::PL == 1) {
-            const dim3 grid = fs2_x_grid(a, (max_k + 31) / 32, a.KV, B);
-            if (a.drop.thresh) launch_xattn_dkv32<DK, true>(a, grid, stream);
-            else launch_xattn_dkv32<DK, false>(a, grid, stream);
-        } else {
-            const dim3 grid = fs2_x_grid(a, (max_k + 63) / 64, a.KV, B);
-            if (a.drop.thresh) launch_xattn_dkv<DK, true>(a, grid, stream);
-            else launch_xattn_dkv<DK, false>(a, grid, stream);
-        }
-        FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(dk, dv)");
-        if (a.nsplit > 1) {
-            const long long most = (long long)B * max_k, n = 2 * (most < a.Mk ? most : a.Mk) * (a.KV * dk / 4);
-            hipLaunchKernelGGL(xattn_dkv_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B, dk);
-            FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(sum)");
-        }
+    a.nblk_q = (int)nq;
+    a.key_groups = (unsigned)(line * nk * a.nsplit);
+    const unsigned grid = a.key_groups + (unsigned)(line * nq);
+    if (a.drop.thresh) launch_xattn_bwd_kernel<E, DK, true>(a, grid, stream);
+    else launch_xattn_bwd_kernel<E, DK, false>(a, grid, stream);
+    FS2_CHECK_LAUNCH("fs2_cross_attention_bwd");
+    if (a.nsplit > 1) {
+        const long long n = 2LL * B * max_k * (a.KV * dk / 4);         // (small where rows are split)
+        hipLaunchKernelGGL(xattn_dkv_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B, dk);
+        FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(sum)");
     }
     return FS2_OK;
 }
@@ -679,7 +693,7 @@ static int launch_xattn_mass(XArgs& a, int B, int max_k, hipStream_t stream) {
     hipLaunchKernelGGL((xattn_mass_kernel<E, DK, KT>), grid, dim3(64 * X_MASS_WAVES), lds, stream, a);
     FS2_CHECK_LAUNCH("fs2_cross_attention_mass");
     if (a.nsplit > 1) {
-        const long long most = (long long)B * max_k, n = a.H * (most < a.Mk ? most : a.Mk);
+        const long long n = (long long)B * max_k * a.H;
         hipLaunchKernelGGL(xattn_mass_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a, B);
         FS2_CHECK_LAUNCH("fs2_cross_attention_mass(sum)");
     }

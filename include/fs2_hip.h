@@ -422,8 +422,8 @@ int fs2_bn_bwd(const float* y, const float* stats, const float* gamma, const flo
  * ldk = ldv).  dk in {32, 64, 96, 128}; T = fp32 or bf16; leading dims multiples of 16 bytes, at most 2^20.
  *   ctx = dropout(softmax(q k^T / sqrt(dk))) v  [Mq, ldo] T;   lse [n_heads][Mq] (may be NULL): log2-domain log-sum-exp
  * An utterance without keys gets ctx = 0, lse = -inf; rows in front of cu_q[0] and behind cu_q[B] are left as they were.
- * max_q / max_k: at least the longest utterance of either side, at most Mq / Mk.  (A longer one is cut there, the results of its
- * rows behind are undefined; offsets outside the matrices are clamped to them.)  Outputs overlap no input.  Serves one
+ * max_q / max_k: at least the longest utterance of either side, at most Mq / Mk.  (A longer one is cut there, its rows behind
+ * are left as they were; offsets outside the matrices are clamped to them.)  Outputs overlap no input.  Serves one
  * query per utterance (autoregressive decoding against fixed encoder states) to whole batches; the kernel and a split of the
  * keys over workgroups follow from the shape.  Softmax statistics and sums are fp32; bf16 rounds the probabilities and the
  * result; fp32 products are exact to 2^-23, an infinite element of fp32 q, k or v counts as NaN.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row = packed query row, col =

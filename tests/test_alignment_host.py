@@ -68,7 +68,7 @@ def test_cross_attention_forward_refuses(change, text):
 @pytest.mark.parametrize("change,text", [
     (dict(ctx=None), "null argument"), (dict(lse=None), "null argument"), (dict(v=None), "null argument"),
     (dict(ctx=P + 4), "unaligned"), (dict(ldv=120), "ldv=120"), (dict(ldo=1 << 28), "ldo=268435456"), (dict(rate=1.5), "dropout rate"), (dict(ws=None), "workspace bytes"),
-    (dict(ws=P + 4), "workspace bytes"),
+    (dict(ws=P + 4), "workspace bytes"), (dict(B=32768, max_q=4096, Mq=1 << 20), "32768 x 4 heads x max_q=4096"),
 ])
 def test_cross_attention_backward_refuses(change, text):
     with pytest.raises(hip.HipError, match=text):

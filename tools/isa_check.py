@@ -38,7 +38,7 @@ MAGIC = b"__CLANG_OFFLOAD_BUNDLE__"
 NO_SCRATCH = ("attention32_kernel", "attention_split_kernel", "proj_ln_kernel", "gemm_regw_kernel", "conv_gemm256_kernel", "conv_wgrad_kernelIDF16b", "attn_bwd_dq_kernelIDF16b",
               "attn_bwd_dkv_kernelIDF16b")
 # kernels whose LDS-DMA buffers are private to a wave (no other wave reads them): the vmcnt wait alone orders a DMA's bytes
-WAVE_PRIVATE = ("xattn_few_kernel", "xattn_dkv32_kernel", "xattn_mass_kernel")
+WAVE_PRIVATE = ("xattn_few_kernel", "xattn_bwd_kernel", "xattn_mass_kernel")
 READLANE_WINDOW = 8
 
 
