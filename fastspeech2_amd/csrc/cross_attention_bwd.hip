@@ -517,10 +517,10 @@ __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int 
 // ---- mass: one workgroup per (utterance, head, 16 KT keys, range of queries) --------------------------------------------
 // The keys are operands in the registers of every wave; the waves stream the queries, 16 at a time, through a private LDS ring of two
 // tiles.  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds up its own queries' weights over the whole loop, and the 16
-// queries of a row of lanes meet only at the end.  32 x 800 queries, 120 keys, 2 heads of 128, bf16: 11.6 us for 16 MB (1.3 TB/s; floor
-// 3.0), the keys' wait and the first queries' behind it, then 13 tiles to a wave.  3100 queries, 512 keys, 4 heads of 64, fp32: 12.3 us
+// queries of a row of lanes meet only at the end.  32 x 800 queries, 120 keys, 2 heads of 128, bf16: 9.4 us for 16 MB (1.7 TB/s; floor
+// 3.0; 11.6 with four waves): the keys' wait and the first queries' behind it, then seven tiles to a wave, in workgroups fewer than CUs.  3100 queries, 512 keys, 4 heads of 64, fp32: 12.3 us
 // with the sum over nine query ranges (floor 3.9).  64 keys to a workgroup in bf16; 32 in fp32, whose keys take three times the registers.
-constexpr int X_MASS_WAVES = 4;
+constexpr int X_MASS_WAVES = 8;
 
 template <typename E, int DK, int KT>
 __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs a) {
@@ -546,14 +546,17 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
     const float* __restrict__ lse = a.lse + (size_t)h * a.Mq + q0;
     unsigned char* ring = smem + TK::BYTES + wave * NST * TQ::BYTES;
 
-    XFetch<E, DK, KB, 1, NW> fk(a.ldk, wave, lane);
-    fk.fetch((const T*)a.k + (size_t)(k0 + blk * KB) * a.ldk + kvh * DK, a.ldk, lenk - blk * KB, smem, wave, lane);
+    constexpr int NP = TK::BYTES / 1024, NWK = E::PL == 3 || NP % NW == 0 ? NW : 4;          // waves that fetch the keys
+    XFetch<E, DK, KB, 1, NWK> fk(a.ldk, wave, lane);
+    if (NWK == NW || wave < NWK)
+        fk.fetch((const T*)a.k + (size_t)(k0 + blk * KB) * a.ldk + kvh * DK, a.ldk, lenk - blk * KB, smem, wave, lane);
     XFetch<E, DK, 16, 1, 1> fq(a.ldq, 0, lane);
     float l_next = INFINITY;
     auto fetch = [&](int qt, int st) __attribute__((always_inline)) {
         fq.fetch(qb + (size_t)qt * 16 * a.ldq, a.ldq, lenq - qt * 16, ring + st * TQ::BYTES, 0, lane);
         l_next = lse[min(qt * 16 + i, lenq - 1)];
     };
+    if (t0 + wave < t1) fetch(t0 + wave, 0);                   // under the keys' wait
     fk.put(smem, wave, lane);
     vm_wait_barrier<0>();
     XFrag<E> kf[KS][KT];
@@ -561,7 +564,6 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) kf[ks][kt] = TK::row_frag(smem, kt * 16 + i, ks, g);
-    if (t0 + wave < t1) fetch(t0 + wave, 0);
     f32x4 acc[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) acc[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
