@@ -249,6 +249,8 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
 }
 
 // At most 16 packed rows per (utterance, shared head).  grid (nsplit, KV, B); wave w takes the 32-key tiles t0 + w, + 4, ..
+// 256 sentences x 2000 keys, 2 heads of 128, bf16: 98 us for 524 MB (5.3 TB/s, a large copy's rate); short key lists are a chain of dependent
+// reads (one sentence of 120 keys: 4.8 us in the kernel, eight waves instead of four 5.7).
 template <typename E, int DK>
 __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
     typedef typename E::mem T;
@@ -482,9 +484,9 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
             p.nsplit = (int)(want < most ? want : most);
         }
     } else {
-        // two row tiles to a wave: bf16, whose tiles cost nothing but their reads.  fp32: with one, three workgroups share a CU and
-        // hide each other's LDS reads and splits (32 x 240 rows x 810 keys, dk = 96: 59 us against 62; 32 x 120 x 800, dk = 32: 25
-        // against 31), though each splits its keys for half the rows
+        // two row tiles to a wave: bf16, whose tiles cost nothing but their reads (32 x 800 rows over 120 keys: 15.2 us, one: 17.0).
+        // fp32: with one, three workgroups share a CU and hide each other's LDS reads and splits (32 x 240 rows x 810 keys, dk = 96: 59 us
+        // against 62; 32 x 120 x 800, dk = 32: 25 against 31), though each splits its keys for half the rows
         p.qt = rows > 64 && dtype == 1 ? 2 : 1;
         const int kb = dtype == 1 ? 64 : 32, full = dtype == 1 ? 512 : 768;          // workgroups that the chip holds at a time
         const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = (max_k + kb - 1) / kb;

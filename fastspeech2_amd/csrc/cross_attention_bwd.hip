@@ -518,8 +518,9 @@ __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int 
 // The keys are operands in the registers of every wave; the waves stream the queries, 16 at a time, through a private LDS ring of two
 // tiles.  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds up its own queries' weights over the whole loop, and the 16
 // queries of a row of lanes meet only at the end.  32 x 800 queries, 120 keys, 2 heads of 128, bf16: 9.4 us for 16 MB (1.7 TB/s; floor
-// 3.0; 11.6 with four waves): the keys' wait and the first queries' behind it, then seven tiles to a wave, in workgroups fewer than CUs.  3100 queries, 512 keys, 4 heads of 64, fp32: 12.3 us
-// with the sum over nine query ranges (floor 3.9).  64 keys to a workgroup in bf16; 32 in fp32, whose keys take three times the registers.
+// 3.0; 11.6 with four waves): the keys' wait and the first queries' behind it, then seven tiles to a wave, in workgroups fewer than CUs.
+// 3100 queries, 512 keys, 4 heads of 64, fp32: 12.9 us with the sum over nine query ranges (floor 3.9).  64 keys to a workgroup in bf16;
+// 32 in fp32, whose keys take three times the registers.
 constexpr int X_MASS_WAVES = 8;
 
 template <typename E, int DK, int KT>

@@ -5,22 +5,24 @@
 //   dx = rstd (dh - mean_g(dh) - xhat mean_g(dh xhat));  dgamma = sum dz xhat,  dbeta = sum dz
 // Unlike BatchNorm (batchnorm.hip) no utterance sees another: a batch row equals the utterance alone.
 //
-// Memory-bound: the floor is one read of the inputs and one write of the output.  Measured, 32 utterances x 800 rows x 256 channels
-// in 16 groups, tanh: forward fp32 -> bf16 13.9 us for 39 MB (2.8 TB/s); backward 20.0 us for 65 MB (3.3 TB/s), 3.9 of it the sums of
-// dgamma and dbeta; 256 x 800 x 80, bf16 backward: 35.8 us for 97 MB (2.7 TB/s).  What is left: all workgroups read, reduce and
-// write at the same time, so the memory waits while they reduce (of the 34 us of the last, 15 are the read at 4.2 TB/s, 4 the sums,
-// 15 the write), and one branch per vector of values and activation (per value: 16.0, 20.5 + 4, 43 + 5 us).
-// A workgroup owns a STRIP of whole groups
-// (at least GN_STRIP_BYTES of a row) of one utterance and holds its rows in REGISTERS: it reads them once, takes the mean, then
-// the centred squares (two passes over registers, no cancellation), and writes.  An utterance too long for the registers is cut
-// into chunks: a first kernel leaves (mean, centred squares) of every chunk, or the backward's channel sums, a second reads the
-// rows again and applies.  Chunks merge by M2 = sum M2_i + n_i (mean_i - mean)^2 in a fixed order; no atomics.
+// Memory-bound: the floor is one read of the inputs and one write of the output.  A workgroup owns a STRIP of whole groups (at least
+// GN_STRIP_BYTES of a row) of one utterance and holds its rows in REGISTERS: it reads them once, takes the mean, then the centred
+// squares (two passes over registers, no cancellation), and writes.  An utterance too long for the registers is cut into chunks: a first
+// kernel leaves (mean, centred squares) of every chunk, or the backward's channel sums, a second reads the rows again and applies.
+// Chunks merge by M2 = sum M2_i + n_i (mean_i - mean)^2 in a fixed order; no atomics.
+//
+// Measured, 32 utterances x 800 rows x 256 channels in 16 groups, tanh: forward fp32 -> bf16 13.9 us for 39 MB (2.8 TB/s); backward
+// 20.0 us for 65 MB (3.3 TB/s), 3.9 of it the sums of dgamma and dbeta; 256 x 800 x 80, bf16 backward: 35.5 us for 97 MB (2.7 TB/s).
+// What is left: all workgroups read, reduce and write at the same time, so the memory waits while they reduce (of the 34 us of the
+// last, 15 are the read at 4.2 TB/s, 4 the sums, 15 the write).  Activation and dropout are chosen by the vector of values: by the
+// value, with its branches, the three took 15.4, 22.5 and 47.4 us.
 #include "common.h"
 
 namespace fs2 {
 
-// Threads of a workgroup: 512 where it holds a whole utterance's strip, 256 where it streams a chunk (80 channels, 256
-// utterances of 800 rows, backward sums: 50 us with 512 threads, 27 with 256: the small groups overlap each other's phases).
+// Threads of a workgroup: 512 where it holds a whole utterance's strip, 256 where it streams a chunk: small groups overlap each other's
+// phases (64 x 6000 rows x 80 channels, bf16 backward: sums 35 us with 256 and 44 with 512 threads, gradient 52 and 40; 32 x 6000 x 256
+// fp32 forward 48 + 83 and 53 + 91; one utterance of 6000: 9.8 + 10.3 and 11.6 + 10.1).
 constexpr int GN_WHOLE_THREADS = 512, GN_CHUNK_THREADS = 256;
 constexpr int GN_CHUNK_ROWS = 8;          // rows per thread of a chunk
 constexpr int GN_HOLD = 4;                // rows per thread in registers at a time, in a chunk
