@@ -404,6 +404,7 @@ static inline int fs2_x_check(const char* who, const void* q, const void* k, con
     FS2_CHECK_ARG(B <= 65535 && max_q <= Mq && max_k <= Mk, "%s: B=%d (<= 65535), max_q=%d > Mq=%d or max_k=%d > Mk=%d", who, B,
                   max_q, Mq, max_k, Mk);
     FS2_CHECK_ARG((long long)max_q * (H / KV) <= (1 << 24), "%s: max_q=%d with %d heads to a key head", who, max_q, H / KV);
+    FS2_CHECK_ARG(max_k <= (1 << 30), "%s: max_k=%d beyond 2^30", who, max_k);
     const long long longest = (long long)max_q * (H / KV) > max_k ? (long long)max_q * (H / KV) : max_k;
     FS2_CHECK_ARG((long long)B * H <= (1 << 19) && (long long)B * H * ((longest + 31) / 32) < (1ll << 30),
                   "%s: B=%d x %d heads x %lld rows in one launch", who, B, H, longest);

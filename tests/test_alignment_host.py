@@ -32,7 +32,7 @@ ATTEND_REFUSED = [
     (dict(B=65536), "B=65536"), (dict(max_q=17), "max_q=17 > Mq=16"), (dict(max_k=19), "max_k=19 > Mk=18"),
     (dict(ldq=255), "ldq=255"), (dict(ldq=248), "ldq=248"), (dict(ldk=130), "ldk=130"), (dict(q=P + 8), "unaligned q or k"),
     (dict(k=P + 2), "unaligned q or k"),
-    (dict(max_q=1 << 25, Mq=1 << 25), "max_q=33554432"),
+    (dict(max_q=1 << 25, Mq=1 << 25), "max_q=33554432"), (dict(max_k=(1 << 30) + 1, Mk=(1 << 31) - 1), "max_k=1073741825"),
     (dict(B=60000, max_q=1 << 22, Mq=1 << 24, H=4), "in one launch"),
 ]
 

@@ -366,6 +366,39 @@ def test_utterances_longer_than_announced_are_cut():
     assert (got[60:100] == 7.0).all() and (gq[60:100] == 7.0).all() and (gkv[30:80] == 7.0).all() and (gm[:, 30:80] == 7.0).all()
 
 
+@pytest.mark.parametrize("H,nq,nk", [(8, 1, 3), (1, 17, 2)])
+def test_as_many_utterances_as_one_call_takes(H, nq, nk):
+    """65535 utterances: the last one's results, and a sum over all, against float64 on the device"""
+    B, dk = 65535, 32
+    g = torch.Generator(device=DEV).manual_seed(H)
+    q, do = (torch.randn(B * nq, H * dk, generator=g, device=DEV) for _ in range(2))
+    k, v = (torch.randn(B * nk, H * dk, generator=g, device=DEV) for _ in range(2))
+    cu_q = torch.arange(B + 1, device=DEV, dtype=torch.int32) * nq
+    cu_k = torch.arange(B + 1, device=DEV, dtype=torch.int32) * nk
+    ctx, dq, dk_, dv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    lse, mass = torch.empty(H, B * nq, device=DEV), torch.empty(H, B * nk, device=DEV)
+    ld = H * dk
+    n = (B, nq, nk, B * nq, B * nk)
+    ws = _bytes("fs2_cross_attention_workspace", *n[:4], H, H, dk, 0)
+    call("fs2_cross_attention", ptr(q), ptr(k), ptr(v), ptr(ctx), ptr(lse), ptr(cu_q), ptr(cu_k), ptr(ws), *n, H, H, dk, ld, ld, ld, ld, 0,
+         0, 0, 0.0, stream())
+    ws = _bytes("fs2_cross_attention_bwd_workspace", *n, H, H, dk, 0)
+    call("fs2_cross_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(ctx), ptr(do), ptr(lse), ptr(dq), ptr(dk_), ptr(dv), ptr(cu_q), ptr(cu_k),
+         ptr(ws), *n, H, H, dk, ld, ld, ld, ld, 0, 0, 0, 0.0, stream())
+    ws = _bytes("fs2_cross_attention_mass_workspace", *n[:3], B * nk, H, H, dk, 0)
+    call("fs2_cross_attention_mass", ptr(q), ptr(k), ptr(lse), ptr(mass), ptr(cu_q), ptr(cu_k), ptr(ws), *n, H, H, dk, ld, ld, 0, stream())
+    Q, D = (t.double().view(B, nq, 1, H, dk) for t in (q, do))
+    K, V = (t.double().view(B, 1, nk, H, dk) for t in (k, v))
+    P = torch.softmax((Q * K).sum(-1) * dk ** -0.5, 2)
+    O = (P[..., None] * V).sum(2)
+    dS = P * ((D * V).sum(-1) - (D[:, :, 0] * O).sum(-1)[:, :, None]) * dk ** -0.5
+    for got, want in ((ctx, O), (dq, (dS[..., None] * K).sum(2)), (dk_, (dS[..., None] * Q).sum(1)), (dv, (P[..., None] * D).sum(1)),
+                      (mass.t(), P.sum(1))):
+        got, want = got.double().reshape(B, -1), want.reshape(B, -1)
+        # 2 dk fp32 operations behind an element of size ~10, at most
+        assert (got - want).abs().max() <= 64 * U * 10 * 4 and (got[-1] - want[-1]).abs().max() <= 64 * U * 10 * 4
+
+
 def test_mass_of_a_broken_query_is_nan():
     p = Problem([20, 9], [30, 12], 2, 2, 64, "fp32", seed=4)
     clean = p.mass(p.forward()[1])
