@@ -345,6 +345,68 @@ def test_rows_in_front_of_the_first_utterance(lq, lk):
     assert torch.equal(gm[:, 7:], m) and (gm[:, :7] == 7.0).all()
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lq,lk,H,KV,dk", [([70, 33], [50, 90], 4, 2, 64), ([2, 1], [300, 5], 2, 1, 96)])
+def test_every_matrix_has_its_own_leading_dim(lq, lk, H, KV, dk, dtype):
+    """q, k, v and ctx as views of wider matrices, each of another width: the bits of the packed call"""
+    p = Problem(lq, lk, H, KV, dk, dtype, seed=11)
+    ctx, lse = p.forward()
+    dq, dkv = p.backward(ctx, lse)
+    m = p.mass(lse)
+    t, nk, nv = TDT[dtype], KV * dk, 2 * KV * dk
+
+    def wide(x, extra, left):
+        w = torch.full((x.shape[0], x.shape[1] + extra), 7.0, dtype=t, device=DEV)
+        v = w[:, left:left + x.shape[1]]
+        v.copy_(x)
+        return w, v
+    bufs = [wide(x, e, l) for x, e, l in ((p.d["q"], 40, 16), (p.d["kv"][:, :nk], 8, 8), (p.d["kv"][:, nk:nv], 24, 0),
+                                          (torch.full_like(ctx, 7.0), 56, 32), (p.d["dctx"], 56, 32))]
+    grads = [wide(torch.full_like(b[1], 7.0), b[0].shape[1] - b[1].shape[1], l) for b, l in zip(bufs[:3], (16, 8, 0))]
+    ldq, ldk, ldv, ldo = (b[0].shape[1] for b in bufs[:4])
+    q, k, v, o, do = (b[1].data_ptr() for b in bufs)
+    gq, gk, gv = (b[1].data_ptr() for b in grads)
+    n = (p.B, p.max_q, p.max_k, p.Mq, p.Mk)
+    l2 = torch.full_like(lse, 7.0)
+    m2 = torch.full_like(m, 7.0)
+    ws = _bytes("fs2_cross_attention_workspace", *n[:4], H, KV, dk, CODE[dtype])
+    call("fs2_cross_attention", q, k, v, o, ptr(l2), ptr(p.cu_q), ptr(p.cu_k), ptr(ws), *n, H, KV, dk, ldq, ldk, ldv, ldo, CODE[dtype], 0, 0,
+         0.0, stream())
+    ws = _bytes("fs2_cross_attention_bwd_workspace", *n, H, KV, dk, CODE[dtype])
+    call("fs2_cross_attention_bwd", q, k, v, o, do, ptr(l2), gq, gk, gv, ptr(p.cu_q), ptr(p.cu_k), ptr(ws), *n, H, KV, dk, ldq, ldk, ldv, ldo,
+         CODE[dtype], 0, 0, 0.0, stream())
+    ws = _bytes("fs2_cross_attention_mass_workspace", *n[:3], p.Mk, H, KV, dk, CODE[dtype])
+    call("fs2_cross_attention_mass", q, k, ptr(l2), ptr(m2), ptr(p.cu_q), ptr(p.cu_k), ptr(ws), *n, H, KV, dk, ldq, ldk, CODE[dtype], stream())
+    assert torch.equal(bufs[3][1], ctx) and torch.equal(l2, lse) and torch.equal(m2, m)
+    assert torch.equal(grads[0][1], dq) and torch.equal(grads[1][1], dkv[:, :nk]) and torch.equal(grads[2][1], dkv[:, nk:nv])
+    for (w, v_), left in zip([bufs[3]] + grads, (32, 16, 8, 0)):
+        assert (w[:, :left] == 7.0).all() and (w[:, left + v_.shape[1]:] == 7.0).all()
+
+
+def test_two_calls_at_once():
+    """two streams, a workspace each, many calls under way together: the bits of the calls alone"""
+    probs = [Problem([1, 1], [5000, 700], 2, 2, 64, "bf16", seed=1), Problem([700], [301], 4, 2, 96, "fp32", seed=2)]
+    norm = Norm([300, 120], 256, 16, "tanh", "fp32", seed=3)
+    want = []
+    for p in probs:
+        c, l = p.forward()
+        want.append([c, l, *p.backward(c, l), p.mass(l)])
+    ny, nst = norm.forward("bf16")
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for p, st in zip(probs, streams):
+            with torch.cuda.stream(st):
+                c, l = p.forward()
+                got.append([c, l, *p.backward(c, l), p.mass(l), *norm.forward("bf16")])
+    for st in streams:
+        st.synchronize()
+    for k, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[k % 2] + [ny, nst]))
+
+
 def test_utterances_longer_than_announced_are_cut():
     """max_q, max_k below the longest: what is computed is that of the cut utterances, no other row is touched"""
     full = Problem([100, 60], [80, 30], 4, 2, 64, "bf16", seed=5)
