@@ -705,8 +705,8 @@ static int gn_check(const char* who, const void* x, const int* cu, const float* 
     return FS2_OK;
 }
 
-static GnArgs gn_args(int B, const void* x, const int* cu, const float* gamma, const float* beta, float* stats, void* workspace, int max_len, int M, int C,
-                      int groups, int ldx, int act, const GnPlan& p, Dropout drop) {
+static GnArgs gn_args(int B, const void* x, const int* cu, const float* gamma, const float* beta, float* stats, void* workspace,
+                      int max_len, int M, int C, int groups, int ldx, int act, const GnPlan& p, Dropout drop) {
     GnArgs a = {};
     a.x = x; a.cu = cu; a.gamma = gamma; a.beta = beta; a.stats = stats; a.part = (float*)workspace;
     a.M = M; a.max_len = max_len; a.C = C; a.G = groups; a.cg = C / groups; a.ldx = ldx; a.act = act;
