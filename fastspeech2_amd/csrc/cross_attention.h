@@ -182,7 +182,7 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_pack(const f32x4& lo
 
 // what x_pack<XB16> rounded away, as another operand.  dS goes into its products as two bf16 numbers: dP - delta already carries the
 // rounding of ctx (delta is summed from it), and with dS rounded too dq and dk were 1.4 .. 1.55 times as far off as one rounding
-// of the result is; so they are at most 1.3 times, for one more product beside dq's three and dk's two.
+// of the result is; so they are at most 1.4 times, for one more product beside dq's three and dk's two.
 __device__ __forceinline__ XFrag<XB16> x_pack_rest(const f32x4& lo, const f32x4& hi, const XFrag<XB16>& f) {
     XFrag<XB16> r;
 #pragma unroll
