@@ -180,9 +180,9 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_pack(const f32x4& lo
     }
 }
 
-// what x_pack<XB16> rounded away, as another operand.  dS goes into its products as two bf16 numbers: dP - delta already carries the
-// rounding of ctx (delta is summed from it), and with dS rounded too dq and dk were 1.4 .. 1.55 times as far off as one rounding
-// of the result is; so they are at most 1.4 times, for one more product beside dq's three and dk's two.
+// bf16: a value goes into a product as two numbers, or the sum over keys (or rows) carries its rounding: with P as one number ctx and
+// dv were 1.2 .. 1.4 times as far off as rounding the result alone, with dS as one dq and dk 1.4 .. 1.55 times.
+// What x_pack<XB16> rounded away, as another operand (dS).
 __device__ __forceinline__ XFrag<XB16> x_pack_rest(const f32x4& lo, const f32x4& hi, const XFrag<XB16>& f) {
     XFrag<XB16> r;
 #pragma unroll
@@ -191,6 +191,25 @@ __device__ __forceinline__ XFrag<XB16> x_pack_rest(const f32x4& lo, const f32x4&
         r.p[0][4 + e] = (bf16_t)(hi[e] - (float)f.p[0][4 + e]);
     }
     return r;
+}
+// Weights >= 0 (P) as f + r, both > 0 where the weight is: f is cut below the weight (the next smaller number's upper half), r is what is
+// left, below 2^-7 of it, rounded to half a step: together off by 2^-15.  A remainder of either sign, or of zero, would make NaN of
+// an infinite value's weight times infinity.  (A weight without bits, 0, stays 0.)
+__device__ __forceinline__ void x_pack_weights(const f32x4& lo, const f32x4& hi, XFrag<XB16>& f, XFrag<XB16>& r) {
+    uint4 w;
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const float a = e < 4 ? lo[e] : hi[e - 4], b = e < 4 ? lo[e + 1] : hi[e - 3];
+        const uint32_t ua = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, a), 1u);
+        const uint32_t ub = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, b), 1u);
+        ((uint32_t*)&w)[e >> 1] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+        rest[e] = a - __builtin_bit_cast(float, ua & 0xffff0000u);
+        rest[e + 1] = b - __builtin_bit_cast(float, ub & 0xffff0000u);
+    }
+    f.p[0] = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.p[0][e] = (bf16_t)rest[e];
 }
 
 // ---- tiles of ROWS rows x DK in LDS ---------------------------------------------------------------------------------

@@ -1,8 +1,8 @@
 // Cross attention over packed ragged batches: queries [Mq] of one matrix, keys / values [Mk] of another, utterance b of the
 // first against utterance b of the second (cu_q, cu_k), g = H / KV query heads to a key / value head.
 //   S = q k^T / sqrt(dk);  P = softmax over the utterance's keys;  ctx = dropout(P) v;  lse = log2 sum exp2(S log2 e)
-// An utterance without keys has ctx = 0 and lse = -inf.  Running maximum and sum in fp32; bf16 rounds P (to half a step of
-// bf16, like the operands it meets on the matrix pipe) and the result, nothing else.
+// An utterance without keys has ctx = 0 and lse = -inf.  Running maximum and sum in fp32; bf16 rounds the result alone (P goes into its
+// product as two bf16 numbers).
 //
 // Orientation as in attention.hip: S^T = K Q^T and O^T = V^T P^T, so that a lane owns one query row and every softmax statistic
 // is lane-local; the accumulator layout of P^T is used as the next operand, V is read transposed from LDS with the same map.
@@ -206,12 +206,17 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             frag_t pf[QT];
-#pragma unroll
-            for (int t = 0; t < QT; ++t) pf[t] = x_pack<E>(s[t][2 * c], s[t][2 * c + 1]);
             if constexpr (E::PL == 1) {
 #pragma unroll
-                for (int t = 0; t < QT; ++t) x_mma<E, DT>(vf[c], pf[t], o[t]);
+                for (int t = 0; t < QT; ++t) {
+                    frag_t rest;
+                    x_pack_weights(s[t][2 * c], s[t][2 * c + 1], pf[t], rest);
+                    x_mma<E, DT>(vf[c], rest, o[t]);
+                    x_mma<E, DT>(vf[c], pf[t], o[t]);
+                }
             } else {
+#pragma unroll
+                for (int t = 0; t < QT; ++t) pf[t] = x_pack<E>(s[t][2 * c], s[t][2 * c + 1]);
 #pragma unroll
                 for (int dt0 = 0; dt0 < DT; dt0 += 2) {
                     frag_t v2[2];
@@ -335,8 +340,11 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[nt][r] *= drop_mul(dh, (uint32_t)qrow, (uint32_t)(kbase + nt * 16 + r));
         }
-        const frag_t pf = x_pack<E>(s[0], s[1]);
-        if constexpr (E::PL == 3) {
+        frag_t pf, rest;
+        if constexpr (E::PL == 1) {
+            x_pack_weights(s[0], s[1], pf, rest);
+        } else {
+            pf = x_pack<E>(s[0], s[1]);
             fv.put(Vs, 0, lane);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
@@ -348,6 +356,7 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
                 v2[u] = TV::col_frag(Vs, 0, dt0 + u, g, i);
                 o[dt0 + u] = o[dt0 + u] * alpha;
             }
+            if constexpr (E::PL == 1) x_mma<E, 2>(v2, rest, &o[dt0]);
             x_mma<E, 2>(v2, pf, &o[dt0]);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read before the next tile overwrites it

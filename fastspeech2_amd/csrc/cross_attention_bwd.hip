@@ -396,10 +396,10 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
                 }
             }
         }
-        frag_t pf[KT], dsf[KT], dsr[KT];
+        frag_t pf[KT], pr[KT], dsf[KT], dsr[KT];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-            pf[kt] = x_pack<E>(s[0][kt], s[1][kt]);
+            x_pack_weights(s[0][kt], s[1][kt], pf[kt], pr[kt]);
             dsf[kt] = x_pack<E>(dp[0][kt], dp[1][kt]);
             dsr[kt] = x_pack_rest(dp[0][kt], dp[1][kt], dsf[kt]);
         }
@@ -408,7 +408,10 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
         for (int dt = 0; dt < DT; ++dt) {
             const frag_t dot = TL::col_frag(Ds, 0, dt, g, i);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) dv_[dt][kt] = mma16(dot.p[0], pf[kt].p[0], dv_[dt][kt]);
+            for (int kt = 0; kt < KT; ++kt) {
+                dv_[dt][kt] = mma16(dot.p[0], pr[kt].p[0], dv_[dt][kt]);
+                dv_[dt][kt] = mma16(dot.p[0], pf[kt].p[0], dv_[dt][kt]);
+            }
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {

@@ -1,0 +1,65 @@
+"""-m gpu: the alignment operators where they are easily wrong: roundings beyond that of the result, infinities next to a tile's end,
+sides without rows, long chunked utterances.  Bounds are counted as in test_gpu_alignment.py: u = 2^-24 per fp32 operation,
+h = half a step of the output's type."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from fastspeech2_amd import hip
+from fastspeech2_amd.hip import call, ptr, stream
+from tests.test_gpu_alignment import ACT_CODE, CODE, DEV, EPS, HALF, LOG2E, TDT, U, Norm, Problem, _bytes, _cu, _half, _near
+from tests.test_gpu_dropout import drop_mul
+
+pytestmark = pytest.mark.gpu
+
+
+def _weights_and_bounds(p, drop):
+    """(utterance, head, rows, keys, dropped probabilities, relative error of one) in float64, the error as fp32 arithmetic makes it:
+    scores dS = (dk + 4) u sum|q||k| / sqrt(dk), exp2 and its argument, the sum of n terms (Problem.exact), and 2^-15 for a probability
+    held as the sum of two bf16 numbers (the first off by less than 2^-7 of it, what is left rounded to half a step)"""
+    q, kv = p.q.double(), p.kv.double()
+    s = p.dk ** -0.5
+    for b, h, rq, rk, hc, kc, vc in p.pairs():
+        n, nq = rk.stop - rk.start, rq.stop - rq.start
+        if n == 0 or nq == 0:
+            continue
+        Q, K = q[rq, hc], kv[rk, kc]
+        S = Q @ K.T * s
+        dS = (p.dk + 4) * U * (Q.abs() @ K.abs().T) * s
+        rP = dS + dS.max(1, keepdim=True).values + (2 * n + 16) * U + 4 * U * LOG2E * S.abs().max(1, keepdim=True).values
+        P = torch.softmax(S, 1)
+        if drop[2]:
+            P = P * drop_mul(drop[0], drop[1] + h, nq, n, drop[2], rq.start)
+        lse = torch.logsumexp(S, 1, keepdim=True).abs() * LOG2E
+        yield rq, rk, hc, vc, P, rP + (n + 2) * U + 2.0 ** -15, rP + 8 * U * (1 + lse) + 2.0 ** -15, nq
+
+
+@pytest.mark.parametrize("lq,lk,H,KV,dk,drop", [
+    ([200, 33], [120, 70], 2, 2, 128, 0.0),          # many rows
+    ([300, 64], [65, 200], 4, 2, 64, 0.1),
+    ([40], [900], 2, 2, 64, 0.0),                    # keys over several workgroups
+    ([1, 1, 2], [120, 33, 700], 4, 1, 96, 0.0),      # few rows
+    ([1], [1500], 2, 2, 32, 0.1),                    # ... over several workgroups
+])
+def test_bf16_results_are_rounded_once(lq, lk, H, KV, dk, drop):
+    """ctx and dv in bf16 are off by half a step of the RESULT and fp32 errors: the probabilities lose nothing on the way to the
+    matrix pipe (an element whose terms cancel shows it: rounding them to 2^-8 moves it by far more than its own half step)"""
+    p = Problem(lq, lk, H, KV, dk, "bf16", seed=21)
+    drop = (99, 3, drop)
+    ctx, lse = p.forward(drop)
+    _, dkv = p.backward(ctx, lse, drop)
+    V, D = p.kv.double(), p.dctx.double()
+    want, tol = torch.zeros(p.Mq, H * dk, dtype=torch.float64), torch.zeros(p.Mq, H * dk, dtype=torch.float64)
+    wv, tv = torch.zeros(p.Mk, KV * dk, dtype=torch.float64), torch.zeros(p.Mk, KV * dk, dtype=torch.float64)
+    for rq, rk, hc, vc, P, r, rb, nq in _weights_and_bounds(p, drop):
+        O = P @ V[rk, vc]
+        e = (P * r) @ V[rk, vc].abs() + 2 * U * O.abs()
+        want[rq, hc], tol[rq, hc] = O, e + HALF["bf16"] * (O.abs() + e)
+        out = slice(vc.start - KV * dk, vc.stop - KV * dk)
+        wv[rk, out] += P.T @ D[rq, hc]
+        tv[rk, out] += (P * (rb + (H // KV * nq + 40) * U)).T @ D[rq, hc].abs()
+    tv += HALF["bf16"] * (wv.abs() + tv)
+    _near(ctx, want, tol, sum(lq), "ctx")
+    _near(dkv[:, KV * dk:].contiguous(), wv, tv, sum(lk), "dv")
