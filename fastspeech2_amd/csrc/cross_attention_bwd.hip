@@ -78,8 +78,11 @@ template <typename E, int DK, bool DROP> __device__ __forceinline__ void x_dq_bl
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) dof[ks] = TQ::row_frag(own + NEXT, i, ks, g);
     }
-    const float del = a.delta[(size_t)head * a.Mq + qrow];
-    const float lse_q = a.lse[(size_t)head * a.Mq + qrow];
+    float del = 0.f, lse_q = 0.f;
+    if (lenk > 0) {                    // (a batch without keys has no delta: nobody wrote it and its workspace has no room for it)
+        del = a.delta[(size_t)head * a.Mq + qrow];
+        lse_q = a.lse[(size_t)head * a.Mq + qrow];
+    }
 
     f32x4 dq[DT];
 #pragma unroll

@@ -63,3 +63,35 @@ def test_bf16_results_are_rounded_once(lq, lk, H, KV, dk, drop):
     tv += HALF["bf16"] * (wv.abs() + tv)
     _near(ctx, want, tol, sum(lq), "ctx")
     _near(dkv[:, KV * dk:].contiguous(), wv, tv, sum(lk), "dv")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lq,H,KV", [([70, 3, 129], 4, 2), ([1, 1], 2, 2)])
+def test_a_batch_without_keys(lq, H, KV, dtype):
+    """ctx = 0, lse = -inf, dq = 0, with no key matrix and the 16 bytes of workspace that the query asks for"""
+    p = Problem(lq, [0] * len(lq), H, KV, 64, dtype, seed=5)
+    assert p.max_k == 0
+    n = int(hip.load().fs2_cross_attention_bwd_workspace(p.B, p.max_q, 0, p.Mq, p.Mk, H, KV, 64, CODE[dtype]))
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device=DEV)
+    rows = sum(lq)
+    ctx, lse = p.forward()
+    assert (ctx[:rows, :H * 64] == 0).all() and (ctx[rows:] == 7).all()
+    assert (lse[:, :rows] == -math.inf).all() and (lse[:, rows:] == 7).all()
+    dq, dkv = p.backward(ctx, lse, ws=ws)
+    assert (dq[:rows, :H * 64] == 0).all() and (dq[rows:] == 7).all() and (dkv == 7).all()
+    assert (p.mass(lse) == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lk", [[90, 5, 33], [700]])
+def test_a_batch_without_queries(lk, dtype):
+    """dk = dv = 0 and no key receives anything; nothing of the query side is touched"""
+    p = Problem([0] * len(lk), lk, 4, 2, 64, dtype, seed=6)
+    assert p.max_q == 0
+    ctx, lse = p.forward()
+    assert (ctx == 7).all() and (lse == 7).all()
+    dq, dkv = p.backward(ctx, lse)
+    rows = sum(lk)
+    assert (dq == 7).all() and (dkv[:rows, :256] == 0).all() and (dkv[rows:] == 7).all()
+    m = p.mass(lse)
+    assert (m[:, :rows] == 0).all() and (m[:, rows:] == 7).all()
