@@ -212,6 +212,19 @@ __device__ __forceinline__ void x_pack_weights(const f32x4& lo, const f32x4& hi,
     for (int e = 0; e < 8; ++e) r.p[0][e] = (bf16_t)rest[e];
 }
 
+// A transposed fragment (XTile::col_frag, c = 0) of a tile with `left` rows: those behind them, copies of the last one, become zero.  Their
+// weights are zero, but zero times an infinite element is NaN.
+__device__ __forceinline__ void x_keep_rows(XFrag<XB16>& f, int left, int g) {
+    uint4 w = __builtin_bit_cast(uint4, f.p[0]);
+    auto mask = [](int n) { return n >= 2 ? 0xffffffffu : (n == 1 ? 0xffffu : 0u); };
+    const int n = left - 4 * g;
+    w.x &= mask(n);
+    w.y &= mask(n - 2);
+    w.z &= mask(n - 16);
+    w.w &= mask(n - 18);
+    f.p[0] = __builtin_bit_cast(bf16x8, w);
+}
+
 // ---- tiles of ROWS rows x DK in LDS ---------------------------------------------------------------------------------
 // Fragment reads take one 16-byte slot of 16 rows, transposed reads 32 bytes of 8 rows at a time; both should meet all 64 banks once.
 //   XB16 (filled by LDS-DMA, lane-linear): unpadded rows whose slots are rotated by WAY * (row >> RSH); rows narrower than 256 bytes

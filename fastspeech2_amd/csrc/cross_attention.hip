@@ -207,6 +207,10 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
         for (int c = 0; c < NC; ++c) {
             frag_t pf[QT];
             if constexpr (E::PL == 1) {
+                if (kt * KB + KB > lenk) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) x_keep_rows(vf[c][dt], lenk - kt * KB - 32 * c, g);
+                }
 #pragma unroll
                 for (int t = 0; t < QT; ++t) {
                     frag_t rest;
@@ -354,6 +358,8 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 v2[u] = TV::col_frag(Vs, 0, dt0 + u, g, i);
+                if constexpr (E::PL == 1)
+                    if (kt * 32 + 32 > lenk) x_keep_rows(v2[u], lenk - kt * 32, g);
                 o[dt0 + u] = o[dt0 + u] * alpha;
             }
             if constexpr (E::PL == 1) x_mma<E, 2>(v2, rest, &o[dt0]);

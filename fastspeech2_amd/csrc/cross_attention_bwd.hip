@@ -409,7 +409,8 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            const frag_t dot = TL::col_frag(Ds, 0, dt, g, i);
+            frag_t dot = TL::col_frag(Ds, 0, dt, g, i);
+            if (qt * 32 + 32 > nrow) x_keep_rows(dot, nrow - qt * 32, g);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 dv_[dt][kt] = mma16(dot.p[0], pr[kt].p[0], dv_[dt][kt]);

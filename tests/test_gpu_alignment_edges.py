@@ -95,3 +95,38 @@ def test_a_batch_without_queries(lk, dtype):
     assert (dq == 7).all() and (dkv[:rows, :256] == 0).all() and (dkv[rows:] == 7).all()
     m = p.mass(lse)
     assert (m[:, :rows] == 0).all() and (m[:, rows:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lq,H,KV", [(40, 2, 2), (33, 4, 2), (1, 2, 2), (64, 2, 1)])
+@pytest.mark.parametrize("lk", [1, 31, 32, 33, 63, 64, 65, 120])
+def test_an_infinite_last_value_row(lk, lq, H, KV, dtype):
+    """an infinite element of the last value row is infinite in its column of ctx, whether or not a tile ends there (fp32: NaN, as
+    announced), and nothing else changes a bit"""
+    p = Problem([lq, 7], [lk, 20], H, KV, 64, dtype, seed=8)
+    clean = p.forward()[0][:lq + 7].float()
+    col = KV * 64 + 3                                      # element 3 of shared head 0
+    p.d["kv"][p.ck[1] - 1, col] = -math.inf
+    got = p.forward()[0][:lq + 7].float()
+    hit = [h * 64 + 3 for h in range(H // KV)]             # the query heads that read it
+    want = clean.clone()
+    want[:lq, hit] = math.nan if dtype == "fp32" else -math.inf
+    assert torch.equal(torch.nan_to_num(got, nan=5.0, neginf=-9.0), torch.nan_to_num(want, nan=5.0, neginf=-9.0))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lq", [1, 31, 32, 33, 64, 100, 250])
+@pytest.mark.parametrize("H,KV", [(2, 2), (2, 1)])
+def test_an_infinite_last_gradient_row(H, KV, lq, dtype):
+    """an infinite element of the last row of dctx in the same way in dv (dq of that row and dk are no numbers, dP - delta being none)"""
+    p = Problem([lq, 9], [50, 20], H, KV, 64, dtype, seed=9)
+    ctx, lse = p.forward()
+    clean = p.backward(ctx, lse)[1].float()
+    p.d["dctx"][lq - 1, (H - 1) * 64 + 5] = math.inf       # the last head's: the last of the packed rows
+    dq, got = p.backward(ctx, lse)
+    got, v = got.float(), slice(KV * 64, 2 * KV * 64)
+    want = clean[:, v].clone()
+    want[:50, (KV - 1) * 64 + 5] = math.nan if dtype == "fp32" else math.inf
+    rows = 70
+    assert torch.equal(torch.nan_to_num(got[:rows, v], nan=5.0, posinf=9.0), torch.nan_to_num(want[:rows], nan=5.0, posinf=9.0))
+    assert torch.equal(got[50:rows], clean[50:rows])       # the other utterance
