@@ -93,9 +93,10 @@ __device__ __forceinline__ bool x_decode_line(const XArgs& a, unsigned id, unsig
 // ---- operands ---------------------------------------------------------------------------------------------------------
 // Both types run on the bf16 matrix pipe (v_mfma_f32_16x16x32_bf16, fp32 accumulation).
 //   XB16: bf16 operands as they are.
-//   XF32: an fp32 value is the exact sum of three bf16 numbers, its significand cut 8 + 8 + 8 bits (x0 = top half of x, x1 = top half of
-//         x - x0, x2 = the rest): a product of two is x0 y0 + (x0 y1 + x1 y0) + (x0 y2 + x1 y1 + x2 y0) up to 2^-23 |x y|, six MFMAs of
-//         16 cycles where the fp32 MFMA form of the same tile (eight 16x16x4, 32 cycles each) takes 256.
+//   XF32: an fp32 value is the exact sum of three bf16 numbers, x0 = x to the nearest, x1 = x - x0 to the nearest, x2 = the rest (|x1| <=
+//         2^-8 |x|, |x2| <= 2^-17 |x|, of either sign).  A product of two is x0 y0 + (x0 y1 + x1 y0) + (x0 y2 + x1 y1 + x2 y0) up to
+//         (2^-24 + 2^-34) |x y|, six MFMAs of 16 cycles where the fp32 MFMA form of the same tile (eight 16x16x4, 32 cycles each) takes
+//         256.  (Planes cut off instead of rounded leave up to 2^-21 |x y|, always towards zero.)
 struct XB16 { typedef bf16_t mem; static constexpr int PL = 1; };
 struct XF32 { typedef float mem; static constexpr int PL = 3; };
 template <typename E> struct XFrag { bf16x8 p[E::PL]; };
@@ -113,24 +114,27 @@ template <typename E, int N> __device__ __forceinline__ void x_mma(const XFrag<E
     }
 }
 
-// the three planes of two values, packed in pairs (an infinity becomes a NaN: infinity - infinity is its rest)
-__device__ __forceinline__ void x_split2(float a, float b, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
-    const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
-    w0 = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-    const float a0 = __builtin_bit_cast(float, ua & 0xffff0000u), b0 = __builtin_bit_cast(float, ub & 0xffff0000u);
-    const float ra = a - a0, rb = b - b0;
-    const uint32_t va = __builtin_bit_cast(uint32_t, ra), vb = __builtin_bit_cast(uint32_t, rb);
-    w1 = __builtin_amdgcn_perm(vb, va, 0x07060302u);
-    const float sa = ra - __builtin_bit_cast(float, va & 0xffff0000u), sb = rb - __builtin_bit_cast(float, vb & 0xffff0000u);
-    w2 = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, sb), __builtin_bit_cast(uint32_t, sa), 0x07060302u);
+// the three planes of two values, packed in pairs.  Between bf16's largest number and fp32's the first plane stays at the former instead of
+// rounding to infinity (CLAMP: values from memory; weights and their gradients are not that large).  An infinity becomes a NaN: infinity
+// - infinity is in its rest.  32 x 120 rows over 810 keys, dk = 96: 60.0 us, 58.5 without the clamp, 56.2 with planes cut off.
+__device__ __forceinline__ uint32_t x_round2(float a, float b) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    return __builtin_bit_cast(uint32_t, (bf16x2){(bf16_t)a, (bf16_t)b});
+}
+template <bool CLAMP> __device__ __forceinline__ void x_split2(float a, float b, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
+    constexpr float most = 3.3895313892515355e38f;
+    w0 = CLAMP ? x_round2(__builtin_amdgcn_fmed3f(a, -most, most), __builtin_amdgcn_fmed3f(b, -most, most)) : x_round2(a, b);
+    const float ra = a - __builtin_bit_cast(float, w0 << 16), rb = b - __builtin_bit_cast(float, w0 & 0xffff0000u);
+    w1 = x_round2(ra, rb);
+    w2 = x_round2(ra - __builtin_bit_cast(float, w1 << 16), rb - __builtin_bit_cast(float, w1 & 0xffff0000u));
 }
 struct XRaw { float v[8]; };          // eight consecutive fp32 values on their way to a fragment
-__device__ __forceinline__ XFrag<XF32> x_split8(const XRaw& x) {
+template <bool CLAMP> __device__ __forceinline__ XFrag<XF32> x_split8(const XRaw& x) {
     uint4 w[3];
-    x_split2(x.v[0], x.v[1], w[0].x, w[1].x, w[2].x);
-    x_split2(x.v[2], x.v[3], w[0].y, w[1].y, w[2].y);
-    x_split2(x.v[4], x.v[5], w[0].z, w[1].z, w[2].z);
-    x_split2(x.v[6], x.v[7], w[0].w, w[1].w, w[2].w);
+    x_split2<CLAMP>(x.v[0], x.v[1], w[0].x, w[1].x, w[2].x);
+    x_split2<CLAMP>(x.v[2], x.v[3], w[0].y, w[1].y, w[2].y);
+    x_split2<CLAMP>(x.v[4], x.v[5], w[0].z, w[1].z, w[2].z);
+    x_split2<CLAMP>(x.v[6], x.v[7], w[0].w, w[1].w, w[2].w);
     XFrag<XF32> f;
 #pragma unroll
     for (int pl = 0; pl < 3; ++pl) f.p[pl] = __builtin_bit_cast(bf16x8, w[pl]);
@@ -149,7 +153,7 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_load(const typename 
         f.p[0] = *(const bf16x8*)p;
         return f;
     } else {
-        return x_split8(x_raw(p));
+        return x_split8<true>(x_raw(p));
     }
 }
 // element j of an operand
@@ -176,7 +180,7 @@ template <typename E> __device__ __forceinline__ XFrag<E> x_pack(const f32x4& lo
             x.v[r] = lo[r];
             x.v[4 + r] = hi[r];
         }
-        return x_split8(x);
+        return x_split8<false>(x);
     }
 }
 
@@ -370,8 +374,8 @@ template <int DK, int ROWS, int WAY, int NW> struct XFetch<XF32, DK, ROWS, WAY, 
             const int id = n * 64 * NW + wave * 64 + lane, row = id / CPR, c = id - row * CPR;
             if (!has(id)) continue;
             uint2 w[3];
-            x_split2(r[n][0], r[n][1], w[0].x, w[1].x, w[2].x);
-            x_split2(r[n][2], r[n][3], w[0].y, w[1].y, w[2].y);
+            x_split2<true>(r[n][0], r[n][1], w[0].x, w[1].x, w[2].x);
+            x_split2<true>(r[n][2], r[n][3], w[0].y, w[1].y, w[2].y);
             unsigned char* at = dst + TL::at(row, c >> 1) + (c & 1) * 8;
 #pragma unroll
             for (int pl = 0; pl < 3; ++pl) *(uint2*)(at + pl * TL::PLANE) = w[pl];

@@ -426,7 +426,7 @@ int fs2_bn_bwd(const float* y, const float* stats, const float* gamma, const flo
  * are left as they were; offsets outside the matrices are clamped to them.)  Outputs overlap no input.  Serves one
  * query per utterance (autoregressive decoding against fixed encoder states) to whole batches; the kernel and a split of the
  * keys over workgroups follow from the shape.  Softmax statistics and sums are fp32; bf16 rounds the result alone (the
- * probabilities are held to 2^-15); fp32 products are exact to 2^-23, an infinite element of fp32 q, k, v (or dctx) counts as NaN, of bf16 as what it is.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row = packed query row, col =
+ * probabilities are held to 2^-15); fp32 products are exact to 2^-24, an infinite element of fp32 q, k, v (or dctx) counts as NaN, of bf16 as what it is.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row = packed query row, col =
  * key index inside the utterance; rate 0 = none).
  * workspace: fs2_cross_attention_workspace bytes, 16-byte aligned (0: NULL is fine).  It is written by every call: two calls
  * that may overlap (streams, captured graphs) need one each. */

@@ -130,3 +130,40 @@ def test_an_infinite_last_gradient_row(H, KV, lq, dtype):
     rows = 70
     assert torch.equal(torch.nan_to_num(got[:rows, v], nan=5.0, posinf=9.0), torch.nan_to_num(want[:rows], nan=5.0, posinf=9.0))
     assert torch.equal(got[50:rows], clean[50:rows])       # the other utterance
+
+
+@pytest.mark.parametrize("lq", [1, 20])                    # the few-rows and the rows kernel
+def test_fp32_scores_are_products_of_fp32(lq):
+    """one key and one element of q and k other than zero: lse = x y log2(e) / 8 shows a single product.  It may be off by 2^-24 of the
+    six products' missing terms, by two roundings of the matrix pipe's sum (one, or a truncation), by those of log2(e), of its
+    multiplication and of the last addition: 6.1 * 2^-24.  Significands whose lower half is all ones, where planes that are cut off
+    leave 2^-21, and random ones."""
+    B, dk = 64, 64
+    p = Problem([lq] * B, [1] * B, 1, 1, dk, "fp32")
+    rng = np.random.default_rng(5)
+
+    def some(n):
+        bits = (0x42000000 + (rng.integers(0, 16, n).astype(np.uint32) << 16) + 0xFFFF)
+        x = bits.astype(np.uint32).view(np.float32)
+        other = (32 * (1 + rng.random(n))).astype(np.float32)
+        return torch.from_numpy(np.where(rng.random(n) < 0.5, x, other).astype(np.float32))
+    x, y = some(B * lq), some(B)
+    p.d["q"].zero_()
+    p.d["kv"].zero_()
+    p.d["q"][:B * lq, 7] = x.to(DEV)
+    p.d["kv"][:B, 7] = y.to(DEV)
+    lse = p.forward()[1][0, :B * lq].cpu().double()
+    want = x.double() * y.double().repeat_interleave(lq) * LOG2E / 8
+    assert float(((lse - want).abs() / want).max()) <= 6.1 * U
+
+
+def test_fp32_values_pass_whole():
+    """weights of exactly one: ctx is v, bit by bit, up to the largest fp32 numbers (beyond bf16's) and down to small ones"""
+    top = torch.finfo(torch.float32).max
+    v = torch.tensor([top, -top, 3.3895e38, 3.396e38, -3.397e38, 1e-30, -1e-28, 0.0, 1 / 3, 65535.0 / 65536, 2 - 2 ** -23])
+    for lq in (1, 40):
+        p = Problem([lq], [1], 1, 1, 32, "fp32")
+        p.d["q"].zero_()
+        p.d["kv"][0, 32:32 + v.numel()] = v.to(DEV)
+        ctx = p.forward()[0][:lq, :v.numel()].cpu()
+        assert torch.equal(ctx, v.expand(lq, -1))
