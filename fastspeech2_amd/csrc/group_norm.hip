@@ -47,16 +47,31 @@ struct GnArgs {
 };
 
 // ---- activations: 0 none, 1 ReLU, 2 tanh, 3 SiLU -------------------------------------------------------------------
-// tanh from one exp2 and one reciprocal, 1 - 2 / (1 + e^2z): absolute error below 2e-7.  Near zero, where that would lose
-// relative accuracy, the odd series to z^5 (the next term is below 4e-9 relative at 1/16).
+// tanh z = z P(z^2) / Q(z^2), P and Q of degree 4 fitted to 0.1 u of it for |z| <= 8 (u = 2^-24; beyond, where 1 - tanh < 4 u, z^2 stays at 64 and
+// the quotient is cut at 1): 7 u with the rounding, in as many operations as 1 - 2 / (1 + e^2z), which keeps no relative accuracy near 0.
+// Slopes and sigmoid from e = exp(-2|z|) or exp(-|z|) <= 1 and one reciprocal: nothing overflows, and they keep their relative accuracy
+// where the activation saturates: tanh' = 4 e / (1 + e)^2 to (4 |z| + 10) u; sigmoid to 8 u of either sign, the exponent's own rounding
+// added back, and silu to 9 u.
 __device__ __forceinline__ float gn_tanh(float z) {
-    const float t = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * 2.8853900817779268f)), 1.0f);
-    const float u = z * z;
-    const float series = z * fmaf(u, fmaf(u, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
-    return fabsf(z) < 0.0625f ? series : t;
+    const float u = fminf(z * z, 64.0f);
+    const float p = fmaf(fmaf(fmaf(fmaf(1.523053150265241e-8f, u, 2.1894744349992834e-5f), u, 3.571603214368224e-3f), u, 0.13444502651691437f), u, 1.0f);
+    const float q = fmaf(fmaf(fmaf(fmaf(8.522493430973554e-7f, u, 3.411300422158092e-4f), u, 2.616446278989315e-2f), u, 0.4677782952785492f), u, 1.0f);
+    const float t = z * p * __builtin_amdgcn_rcpf(q);
+    return __builtin_elementwise_maximum(__builtin_elementwise_minimum(t, 1.0f), -1.0f);         // (these keep a NaN)
 }
-__device__ __forceinline__ float gn_sigmoid(float z) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+__device__ __forceinline__ float gn_tanh_slope(float z) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(z) * -2.8853900817779268f), r = __builtin_amdgcn_rcpf(1.0f + e);
+    return 4.0f * e * (r * r);
+}
+// sigmoid(z) and sigmoid(-z)
+__device__ __forceinline__ void gn_sigmoid(float z, float& s, float& other) {
+    const float a = fminf(fabsf(z), 128.0f), x = a * -1.4426950408889634f;            // (e is 0 from 104 on)
+    float e = __builtin_amdgcn_exp2f(x);
+    // a log2(e) - what x has of it, its rounding and the constant's: log2(e) = 1.44269502162933 + 1.92596e-8
+    e = fmaf(e, fmaf(a, -1.3349758e-8f, fmaf(a, -1.4426950408889634f, -x) * 0.6931471805599453f), e);
+    const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+    s = z >= 0.f ? r : er;
+    other = z >= 0.f ? er : r;
 }
 // act of V values, or act' times u: one (uniform) branch for the vector
 template <int V> __device__ __forceinline__ void gn_act(int act, float (&z)[V]) {
@@ -68,7 +83,11 @@ template <int V> __device__ __forceinline__ void gn_act(int act, float (&z)[V]) 
         for (int j = 0; j < V; ++j) z[j] = gn_tanh(z[j]);
     } else if (act == 3) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) z[j] = z[j] == -INFINITY ? 0.f : z[j] * gn_sigmoid(z[j]);
+        for (int j = 0; j < V; ++j) {
+            float g, h;
+            gn_sigmoid(z[j], g, h);
+            z[j] = z[j] == -INFINITY ? 0.f : z[j] * g;
+        }
     }
 }
 template <int V> __device__ __forceinline__ void gn_slope(int act, const float (&z)[V], float (&u)[V]) {
@@ -77,15 +96,13 @@ template <int V> __device__ __forceinline__ void gn_slope(int act, const float (
         for (int j = 0; j < V; ++j) u[j] = z[j] > 0.f ? u[j] : u[j] * 0.f;
     } else if (act == 2) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float t = gn_tanh(z[j]);
-            u[j] *= fmaf(-t, t, 1.0f);
-        }
+        for (int j = 0; j < V; ++j) u[j] *= gn_tanh_slope(z[j]);
     } else if (act == 3) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float s = gn_sigmoid(z[j]);
-            u[j] *= s * fmaf(z[j], 1.0f - s, 1.0f);
+            float g, h;
+            gn_sigmoid(z[j], g, h);
+            u[j] *= g * fmaf(z[j], h, 1.0f);
         }
     }
 }

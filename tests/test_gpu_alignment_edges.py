@@ -167,3 +167,45 @@ def test_fp32_values_pass_whole():
         p.d["kv"][0, 32:32 + v.numel()] = v.to(DEV)
         ctx = p.forward()[0][:lq, :v.numel()].cpu()
         assert torch.equal(ctx, v.expand(lq, -1))
+
+
+# ---------------------------------------------------------------------------------------------------------- group norm
+@pytest.mark.parametrize("act,xt", [("tanh", "fp32"), ("tanh", "bf16"), ("silu", "fp32"), ("silu", "bf16")])
+def test_activations_and_slopes_are_fp32(act, xt):
+    """gamma = 0: y is the activation of beta and, with one row and dout = 1, dbeta its slope.  u = 2^-24; exp2 and the reciprocal are
+    good to one unit of the last place, 2 u.  tanh = z P / Q: 2 u for the reciprocal, 5 u for the fit and the other operations (an
+    evaluation of the quotient in fp32, rounded each time, is off by 6.6 u at worst with its reciprocal one unit off).  Its slope
+    4 e / (1 + e)^2 with e = exp(-2|z|) off by (2.5 |z| + 2) u: (4 |z| + 10) u.  Sigmoid of either sign 8 u, so silu 9 u; its slope
+    s (1 + z s') 12 u of s (1 + |z| s')."""
+    rng = np.random.default_rng(7)
+    C = 1024
+    z = np.concatenate([rng.standard_normal(400) * 2, np.exp(rng.uniform(-12, 4.3, 616)) * rng.choice([-1, 1], 616),
+                        [0.0, 8.0, -8.000001, 0.0625, 7.99999, 1e-30, -80.0, 60.0]]).astype(np.float32)
+    if act == "tanh":
+        z = np.clip(z, -40, 40)
+    p = Norm([1], C, 4, act, xt)
+    p.gd.zero_()
+    p.bd = torch.from_numpy(z).to(DEV)
+    p.dout = torch.ones(p.M, p.ld)
+    y, stats = p.forward("fp32")
+    _, _, slope = p.backward(stats, "fp32", "fp32")
+    Z = torch.from_numpy(z).double()
+    if act == "tanh":
+        want, ws = torch.tanh(Z), torch.cosh(Z) ** -2
+        ty, ts = 7 * U * want.abs(), (4 * Z.abs() + 10) * U * ws
+    else:
+        g, h = torch.sigmoid(Z), torch.sigmoid(-Z)
+        want, ws = Z * g, g * (1 + Z * h)
+        ty, ts = 9 * U * want.abs(), 12 * U * g * (1 + Z.abs() * h)
+    off, offs = (y[0, :C].cpu().double() - want).abs(), (slope.cpu().double() - ws).abs()
+    assert (off <= ty + 1e-37).all(), ("value", float((off / (ty + 1e-37)).max()))
+    assert (offs <= ts + 1e-37).all(), ("slope", float((offs / (ts + 1e-37)).max()))
+
+
+def test_activations_of_infinities():
+    for act, up, down in (("tanh", 1.0, -1.0), ("silu", math.inf, 0.0), ("relu", math.inf, 0.0)):
+        p = Norm([3], 8, 2, act, "fp32")
+        p.gd.zero_()
+        p.bd = torch.tensor([math.inf, -math.inf, math.nan, 3e38, -3e38, 100.0, -100.0, 0.0], device=DEV)
+        y = p.forward("fp32")[0][0].cpu()
+        assert y[0] == up and y[1] == down and math.isnan(y[2]) and abs(float(y[4])) <= (1 if act == "tanh" else 0) and y[7] == 0
