@@ -8,11 +8,11 @@
 // Memory-bound: the floor is one read of the inputs and one write of the output.  A workgroup owns a STRIP of whole groups (at least
 // GN_STRIP_BYTES of a row) of one utterance and holds its rows in REGISTERS: it reads them once, takes the mean, then the centred
 // squares (two passes over registers, no cancellation), and writes.  An utterance too long for the registers is cut into chunks: a first
-// kernel leaves (mean, centred squares) of every chunk, or the backward's channel sums, a second reads the rows again and applies.
+// kernel leaves (mean, centred squares) of every chunk, or the backward's sums; behind the join of these a last one reads the rows again and applies.
 // Chunks merge by M2 = sum M2_i + n_i (mean_i - mean)^2 in a fixed order; no atomics.
 //
-// Measured, 32 utterances x 800 rows x 256 channels in 16 groups, tanh: forward fp32 -> bf16 13.9 us for 39 MB (2.8 TB/s); backward
-// 20.0 us for 65 MB (3.3 TB/s), 3.9 of it the sums of dgamma and dbeta; 256 x 800 x 80, bf16 backward: 35.5 us for 97 MB (2.7 TB/s).
+// Measured, 32 utterances x 800 rows x 256 channels in 16 groups, tanh: forward fp32 -> bf16 14.5 us for 39 MB (2.7 TB/s); backward
+// 19.2 us for 65 MB (3.4 TB/s), 3.9 of it the sums of dgamma and dbeta; 256 x 800 x 80, bf16 backward: 34.9 us for 97 MB (2.8 TB/s).
 // What is left: all workgroups read, reduce and write at the same time, so the memory waits while they reduce (of the 34 us of the
 // last, 15 are the read at 4.2 TB/s, 4 the sums, 15 the write).  Activation and dropout are chosen by the vector of values: by the
 // value, with its branches, the three took 15.4, 22.5 and 47.4 us.
@@ -21,8 +21,8 @@
 namespace fs2 {
 
 // Threads of a workgroup: 512 where it holds a whole utterance's strip, 256 where it streams a chunk: small groups overlap each other's
-// phases (64 x 6000 rows x 80 channels, bf16 backward: sums 35 us with 256 and 44 with 512 threads, gradient 52 and 40; 32 x 6000 x 256
-// fp32 forward 48 + 83 and 53 + 91; one utterance of 6000: 9.8 + 10.3 and 11.6 + 10.1).
+// phases (64 x 6000 rows x 80 channels, bf16 backward 85 us with 256 and 93 with 512 threads; 32 x 6000 x 256 fp32 forward 149 and 165; one
+// utterance of 6000 13.3 and 15.1; all with the chunks joined by a launch of its own).
 constexpr int GN_WHOLE_THREADS = 512, GN_CHUNK_THREADS = 256;
 constexpr int GN_CHUNK_ROWS = 8;          // rows per thread of a chunk
 constexpr int GN_HOLD = 4;                // rows per thread in registers at a time, in a chunk
@@ -38,6 +38,8 @@ struct GnArgs {
     const void* dout;        // [M, ldd]
     void* dx;                // [M, ldg]
     float* part;             // forward chunks: [B][nchunk][G][2] mean, M2; backward: [B][nchunk][2][C] sums of dz, dz xhat
+    float* gpart;            // backward chunks: [B][nchunk][G][2] sums of dh, dh xhat
+    float* gsum;             // backward of chunked utterances: [B][G][2] means of the same
     int M, max_len, C, G, cg, ldx, ldo, ldd, ldg, act, nchunk, nstrip;
     int units;               // B * nchunk
     int W, LX, LY;           // channels of a strip, lanes per row, rows per pass of the workgroup
@@ -235,9 +237,8 @@ template <int N> __device__ __forceinline__ void gn_put_sums(const GnArgs& a, co
     }
     __builtin_amdgcn_wave_barrier();
 }
-// sum over red's entries and a group's `n` columns (* weight[column]) -> grp[group of the strip], one wave per group
-template <int NT>
-__device__ __forceinline__ void gn_group_sums(const GnArgs& a, const float* red, int w, int n, const float* weight, float* grp) {
+// sum over red's entries and a group's `n` columns -> grp[group of the strip], one wave per group
+template <int NT> __device__ __forceinline__ void gn_group_sums(const GnArgs& a, const float* red, int w, int n, float* grp) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ng = a.W / a.cg;
     const int entries = a.LX <= 64 ? NT / 64 : a.LY;
     for (int gi = wave; gi < ng; gi += NT / 64) {
@@ -246,10 +247,37 @@ __device__ __forceinline__ void gn_group_sums(const GnArgs& a, const float* red,
             float u = 0.f;
 #pragma unroll 4
             for (int e = 0; e < entries; ++e) u += red[e * w + c];
-            t += weight ? u * weight[c] : u;
+            t += u;
         }
         t = wave_sum(t);
         if (lane == 0) grp[gi] = t;
+    }
+}
+// the same of two sums at once, * weight[column]
+template <int NT>
+__device__ __forceinline__ void gn_weighted_sums(const GnArgs& a, const float* red0, const float* red1, const float* weight, float* grp,
+                                                 float* grp2) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ng = a.W / a.cg, n = a.cg;
+    const int entries = a.LX <= 64 ? NT / 64 : a.LY;
+    for (int gi = wave; gi < ng; gi += NT / 64) {
+        float t0 = 0.f, t1 = 0.f;
+        for (int c = gi * n + lane; c < gi * n + n; c += 64) {
+            const float w = weight[c];
+            float u0 = 0.f, u1 = 0.f;
+#pragma unroll 4
+            for (int e = 0; e < entries; ++e) {
+                u0 += red0[e * a.W + c];
+                u1 += red1[e * a.W + c];
+            }
+            t0 = fmaf(u0, w, t0);
+            t1 = fmaf(u1, w, t1);
+        }
+        t0 = wave_sum(t0);
+        t1 = wave_sum(t1);
+        if (lane == 0) {
+            grp[gi] = t0;
+            grp2[gi] = t1;
+        }
     }
 }
 // the group sums of per-channel values: a lane whose vector lies inside one group adds it up first
@@ -261,11 +289,11 @@ __device__ __forceinline__ void gn_reduce(const GnArgs& a, const GnPlace& p, con
         for (int j = 0; j < V; ++j) t[0] += s[j];
         gn_put_sums<1>(a, p, t, tmp, red);
         __syncthreads();
-        gn_group_sums<NT>(a, red, a.LX, a.cg / V, nullptr, grp);
+        gn_group_sums<NT>(a, red, a.LX, a.cg / V, grp);
     } else {
         gn_put_sums<V>(a, p, s, tmp, red);
         __syncthreads();
-        gn_group_sums<NT>(a, red, a.W, a.cg, nullptr, grp);
+        gn_group_sums<NT>(a, red, a.W, a.cg, grp);
     }
     __syncthreads();
 }
@@ -284,6 +312,22 @@ template <int V> __device__ __forceinline__ void gn_params(const float* src, flo
         const f32x4 t = *(const f32x4*)(src + j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[j + e] = t[e];
+    }
+}
+
+// mean, rstd, gamma, beta of a lane's channels
+template <int V>
+__device__ __forceinline__ void gn_lane_params(const GnArgs& a, const GnPlace& p, float (&mean)[V], float (&rs)[V], float (&ga)[V],
+                                               float (&be)[V]) {
+    const int c0 = p.on ? p.c0 : p.strip * a.W;
+    const float* st = a.stats + (size_t)p.b * a.G * 2;
+    gn_params<V>(a.gamma + c0, ga);
+    gn_params<V>(a.beta + c0, be);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int gi = gn_div(c0 + j, a.inv_cg);
+        mean[j] = st[gi * 2];
+        rs[j] = st[gi * 2 + 1];
     }
 }
 
@@ -375,46 +419,97 @@ __global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void g
     }
 }
 
-// chunked forward, second kernel: merge the chunks' statistics, apply
+// Chunks -> utterance, one wave to a group: lanes take every 64th chunk, sums in 64 bits, then over the wave; a fixed order.  Up to GN_JOIN_HERE
+// chunks (one load to a lane) each workgroup of the last kernel does that for itself; beyond, where a workgroup would take longer over the
+// chunks than over its rows, a launch of its own does it once (3 us; 3 x 3500 rows x 512 channels in one group, 219 chunks: forward 19.8 us,
+// backward 34.5; a serial join in each workgroup took 62 and 495).
+constexpr int GN_JOIN_HERE = 64;
+// mean = sum n_i mean_i / n,  variance = (sum M2_i + n_i (mean_i - mean)^2) / n
+__device__ __forceinline__ void gn_join(const GnArgs& a, int b, int g, int rows, int total, float& mean, float& rstd) {
+    const unsigned lane = threadIdx.x & 63;
+    const float* src = a.part + ((size_t)b * a.nchunk * a.G + g) * 2;
+    const size_t step = (size_t)a.G * 2;
+    const float inv = total > 0 ? 1.0f / (float)total : 0.f;
+    double t = 0.0;
+#pragma unroll 4
+    for (unsigned c = lane; c * rows < (unsigned)total; c += 64) t += (double)src[c * step] * (double)min(total - (int)c * rows, rows);
+    mean = wave_sum((float)t) * inv;
+    t = 0.0;
+#pragma unroll 4
+    for (unsigned c = lane; c * rows < (unsigned)total; c += 64) {
+        const float d = src[c * step] - mean;
+        t += (double)(d * d * ((float)min(total - (int)c * rows, rows) * (float)a.cg) + src[c * step + 1]);
+    }
+    rstd = 1.0f / sqrtf(wave_sum((float)t) * (inv / (float)a.cg) + a.eps);
+}
+// the means of dh and dh xhat
+__device__ __forceinline__ void gn_join_bwd(const GnArgs& a, int b, int g, int rows, int total, float& m1, float& m2) {
+    const unsigned lane = threadIdx.x & 63;
+    const float* src = a.gpart + ((size_t)b * a.nchunk * a.G + g) * 2;
+    const size_t step = (size_t)a.G * 2;
+    double t0 = 0.0, t1 = 0.0;
+#pragma unroll 4
+    for (unsigned c = lane; c * rows < (unsigned)total; c += 64) {
+        t0 += (double)src[c * step];
+        t1 += (double)src[c * step + 1];
+    }
+    const float inv_n = total > 0 ? 1.0f / ((float)total * (float)a.cg) : 0.f;
+    m1 = wave_sum((float)t0) * inv_n;
+    m2 = wave_sum((float)t1) * inv_n;
+}
+// the launch for many chunks: forward to stats, backward to gsum
+template <int R, bool BWD> __global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_join_kernel(GnArgs a) {
+    const unsigned slot = blockIdx.x * (GN_CHUNK_THREADS / 64) + (threadIdx.x >> 6);
+    const int b = (int)(slot / (unsigned)a.G), g = (int)(slot - (unsigned)b * (unsigned)a.G);
+    if (b >= a.units / a.nchunk) return;
+    const int c0 = min(max(a.cu[b], 0), a.M), c1 = min(max(a.cu[b + 1], c0), a.M), total = min(c1 - c0, a.max_len);
+    float u, v;
+    if (BWD) gn_join_bwd(a, b, g, a.LY * R, total, u, v);
+    else gn_join(a, b, g, a.LY * R, total, u, v);
+    if ((threadIdx.x & 63) == 0) {
+        float* dst = (BWD ? a.gsum : a.stats) + ((size_t)b * a.G + g) * 2;
+        dst[0] = u;
+        dst[1] = v;
+    }
+}
+
+// chunked forward, last kernel: apply
 template <typename TX, typename TO, int R>
 __global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_apply_kernel(GnArgs a) {
-    constexpr int NT = GN_CHUNK_THREADS;
     constexpr int V = 16 / (int)sizeof(TX);
     extern __shared__ float gn_dyn[];
-    float *grp = gn_dyn, *grp2 = gn_dyn + a.W / a.cg;
+    const int ng = a.W / a.cg;
+    float *grp = gn_dyn, *grp2 = gn_dyn + ng;
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
     if (p.b < 0 || (p.len == 0 && p.chunk > 0)) return;
-    const int g0 = p.strip * (a.W / a.cg), ng = a.W / a.cg, rows = a.LY * R, nch = (total + rows - 1) / rows;
-    const float n_all = (float)total * (float)a.cg;
-    for (int t = threadIdx.x; t < ng; t += NT) {
-        const float* src = a.part + ((size_t)p.b * a.nchunk * a.G + g0 + t) * 2;
-        const size_t step = (size_t)a.G * 2;
-        float mean = 0.f, m2 = 0.f;
-        for (int c = 0; c < nch; ++c) mean = fmaf(src[c * step], (float)min(total - c * rows, rows) * (float)a.cg / n_all, mean);
-        for (int c = 0; c < nch; ++c) {
-            const float d = src[c * step] - mean;
-            m2 += fmaf(d * d, (float)min(total - c * rows, rows) * (float)a.cg, src[c * step + 1]);
+    const bool here = a.nchunk <= GN_JOIN_HERE;
+    if (here) {
+        for (int gi = threadIdx.x >> 6; gi < ng; gi += GN_CHUNK_THREADS / 64) {
+            float u, v;
+            gn_join(a, p.b, p.strip * ng + gi, a.LY * R, total, u, v);
+            if ((threadIdx.x & 63) == 0) {
+                grp[gi] = u;
+                grp2[gi] = v;
+                if (p.chunk == 0) {
+                    float* st = a.stats + ((size_t)p.b * a.G + p.strip * ng + gi) * 2;
+                    st[0] = u;
+                    st[1] = v;
+                }
+            }
         }
-        const float rstd = 1.0f / sqrtf((n_all > 0.f ? m2 / n_all : 0.f) + a.eps);
-        grp[t] = mean;
-        grp2[t] = rstd;
-        if (p.chunk == 0) {
-            float* st = a.stats + ((size_t)p.b * a.G + g0 + t) * 2;
-            st[0] = mean;
-            st[1] = rstd;
-        }
+        __syncthreads();
     }
-    __syncthreads();
     if (!p.on) return;
+    const float* st = a.stats + ((size_t)p.b * a.G + p.strip * ng) * 2;
     float mean[V], rg[V], be[V];
     gn_params<V>(a.gamma + p.c0, rg);
     gn_params<V>(a.beta + p.c0, be);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int gi = gn_div(p.x * V + j, a.inv_cg);
-        mean[j] = grp[gi];
-        rg[j] *= grp2[gi];
+        mean[j] = here ? grp[gi] : st[gi * 2];
+        rg[j] *= here ? grp2[gi] : st[gi * 2 + 1];
     }
     const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
 #pragma unroll 4
@@ -435,22 +530,6 @@ __device__ __forceinline__ void gn_dz(const GnArgs& a, int row, int c0, const Gn
     }
     gn_drop<V>(a.drop, row, c0, dz);
     gn_slope<V>(a.act, z, dz);
-}
-
-// mean, rstd, gamma, beta of a lane's channels
-template <int V>
-__device__ __forceinline__ void gn_lane_params(const GnArgs& a, const GnPlace& p, float (&mean)[V], float (&rs)[V], float (&ga)[V],
-                                               float (&be)[V]) {
-    const int c0 = p.on ? p.c0 : p.strip * a.W;
-    const float* st = a.stats + (size_t)p.b * a.G * 2;
-    gn_params<V>(a.gamma + c0, ga);
-    gn_params<V>(a.beta + c0, be);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int gi = gn_div(c0 + j, a.inv_cg);
-        mean[j] = st[gi * 2];
-        rs[j] = st[gi * 2 + 1];
-    }
 }
 
 // WHOLE: sums and dx in one pass; always: the chunk's channel sums of dz and dz xhat to part
@@ -516,10 +595,17 @@ __global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void g
         dst[c] = t0;
         dst[a.C + c] = t1;
     }
-    if (!WHOLE) return;
-    gn_group_sums<NT>(a, red[0], a.W, a.cg, a.gamma + p.strip * a.W, grp);
-    gn_group_sums<NT>(a, red[1], a.W, a.cg, a.gamma + p.strip * a.W, grp2);
+    gn_weighted_sums<NT>(a, red[0], red[1], a.gamma + p.strip * a.W, grp, grp2);
     __syncthreads();
+    if (!WHOLE) {
+        const int ng = a.W / a.cg;
+        float* gdst = a.gpart + (((size_t)p.b * a.nchunk + p.chunk) * a.G + p.strip * ng) * 2;
+        for (int t = threadIdx.x; t < ng; t += NT) {
+            gdst[t * 2] = grp[t];
+            gdst[t * 2 + 1] = grp2[t];
+        }
+        return;
+    }
     if (!p.on) return;
     const float inv_n = p.len > 0 ? 1.0f / ((float)p.len * (float)a.cg) : 0.f;
     float m1[V], m2[V];
@@ -549,48 +635,37 @@ __global__ __launch_bounds__(WHOLE ? GN_WHOLE_THREADS : GN_CHUNK_THREADS) void g
     }
 }
 
-// chunked backward, second kernel: the utterance's sums from the chunks', then dx from a second read
+// chunked backward, last kernel: dx from a second read
 template <typename TX, typename TD, typename TG, int R>
 __global__ __launch_bounds__(GN_CHUNK_THREADS) void gn_bwd_apply_kernel(GnArgs a) {
-    constexpr int NT = GN_CHUNK_THREADS;
     constexpr int V = 16 / (int)sizeof(TX);
     extern __shared__ float gn_dyn[];
-    float *grp = gn_dyn, *grp2 = grp + a.W / a.cg;
+    const int ng = a.W / a.cg;
+    float *grp = gn_dyn, *grp2 = gn_dyn + ng;
     int total;
     const GnPlace p = gn_place<V, R>(a, total);
     if (p.b < 0 || p.len == 0) return;
-    const int rows = a.LY * R, nch = (total + rows - 1) / rows, ng = a.W / a.cg;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float* part = a.part + (size_t)p.b * a.nchunk * 2 * a.C + p.strip * a.W;
-    for (int gi = wave; gi < ng; gi += NT / 64) {
-        float t0 = 0.f, t1 = 0.f;
-        for (int c = gi * a.cg + lane; c < gi * a.cg + a.cg; c += 64) {
-            float u0 = 0.f, u1 = 0.f;
-            for (int q = 0; q < nch; ++q) {
-                u0 += part[(size_t)q * 2 * a.C + c];
-                u1 += part[(size_t)q * 2 * a.C + a.C + c];
+    const bool here = a.nchunk <= GN_JOIN_HERE;
+    if (here) {
+        for (int gi = threadIdx.x >> 6; gi < ng; gi += GN_CHUNK_THREADS / 64) {
+            float u, v;
+            gn_join_bwd(a, p.b, p.strip * ng + gi, a.LY * R, total, u, v);
+            if ((threadIdx.x & 63) == 0) {
+                grp[gi] = u;
+                grp2[gi] = v;
             }
-            const float w = a.gamma[p.strip * a.W + c];
-            t0 = fmaf(u0, w, t0);
-            t1 = fmaf(u1, w, t1);
         }
-        t0 = wave_sum(t0);
-        t1 = wave_sum(t1);
-        if (lane == 0) {
-            grp[gi] = t0;
-            grp2[gi] = t1;
-        }
+        __syncthreads();
     }
-    __syncthreads();
     if (!p.on) return;
-    const float inv_n = 1.0f / ((float)total * (float)a.cg);
+    const float* sums = a.gsum + ((size_t)p.b * a.G + p.strip * ng) * 2;
     float mean[V], rs[V], ga[V], be[V], m1[V], m2[V];
     gn_lane_params<V>(a, p, mean, rs, ga, be);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int gi = gn_div(p.x * V + j, a.inv_cg);
-        m1[j] = grp[gi] * inv_n;
-        m2[j] = grp2[gi] * inv_n;
+        m1[j] = here ? grp[gi] : sums[gi * 2];
+        m2[j] = here ? grp2[gi] : sums[gi * 2 + 1];
     }
     const TX* src = (const TX*)a.x + (size_t)p.r0 * a.ldx + p.c0;
     const TD* sd = (const TD*)a.dout + (size_t)p.r0 * a.ldd + p.c0;
@@ -642,9 +717,10 @@ __global__ __launch_bounds__(1024) void gn_param_kernel(const float* __restrict_
 // Strip: the narrowest run of whole groups and whole vectors that is at least GN_STRIP_BYTES wide and divides C.  R: rows per thread,
 // the smallest compiled one that holds the utterance; none does: chunks of GN_CHUNK_ROWS.
 // More than 8 rows per thread of a bf16 backward (128 registers of data): only for bf16 dout (the thread recomputes dz instead of
-// keeping it; 32 x 1600 rows x 256 channels with fp32 dout: 51 us against 48 in chunks), and only where the workgroups fill the chip
-// (512 of them, 256 x 800 x 80: 35 us against 41 in chunks; 256: 34 against 38; 64: 29 against 21).  All others hold 16 rows
-// (32 x 1600 x 256 fp32: forward 23 us against 35 in chunks, backward 43 against 63; one utterance 10.7 against 11.6, 11.7 against 14.5).
+// keeping it; 4 x 1500 rows x 256 channels with fp32 dout: 27 us against 18 in chunks), and only where the workgroups fill the chip
+// (512 of them, 256 x 800 x 80: 35 us against 47 in chunks; 256: 19 against 27; 64: 15, 20 and 25 us without activation, with tanh and with
+// SiLU against 18, 20 and 22).  All others hold 16 rows (32 x 1600 x 256 fp32: forward 30 us against 44 in chunks, backward 47 against 77;
+// one utterance 8.6 against 12.4, 10.6 against 16.1).
 struct GnPlan { int W, LX, LY, R, nchunk; bool whole; };
 
 static int gn_gcd(int a, int b) { return b ? gn_gcd(b, a % b) : a; }
@@ -674,6 +750,10 @@ static unsigned gn_grid(const GnArgs& a) {
     return (unsigned)(a.units >= 8 ? 8LL * a.nstrip * ((a.units + 7) / 8) : (long long)a.units * a.nstrip);
 }
 
+static unsigned gn_join_grid(const GnArgs& a) {          // a wave to every (utterance, group)
+    return (unsigned)(((long long)(a.units / a.nchunk) * a.G + GN_CHUNK_THREADS / 64 - 1) / (GN_CHUNK_THREADS / 64));
+}
+
 template <typename TX, typename TO, int R> static void gn_launch_fwd(const GnArgs& a, const GnPlan& p, hipStream_t s) {
     const unsigned grid = gn_grid(a);
     const int lds = 2 * (a.W / a.cg) * (int)sizeof(float);
@@ -681,6 +761,7 @@ template <typename TX, typename TO, int R> static void gn_launch_fwd(const GnArg
         hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, true>), dim3(grid), dim3(GN_WHOLE_THREADS), lds, s, a);
     } else if constexpr (R == GN_CHUNK_ROWS) {
         hipLaunchKernelGGL((gn_fwd_kernel<TX, TO, R, false>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
+        if (a.nchunk > GN_JOIN_HERE) hipLaunchKernelGGL((gn_join_kernel<R, false>), dim3(gn_join_grid(a)), dim3(GN_CHUNK_THREADS), 0, s, a);
         hipLaunchKernelGGL((gn_apply_kernel<TX, TO, R>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
     }
 }
@@ -698,6 +779,7 @@ static void gn_launch_bwd(const GnArgs& a, const GnPlan& p, hipStream_t s) {
         hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, true>), dim3(grid), dim3(GN_WHOLE_THREADS), lds, s, a);
     } else if constexpr (R == GN_CHUNK_ROWS) {
         hipLaunchKernelGGL((gn_bwd_kernel<TX, TD, TG, R, false>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
+        if (a.nchunk > GN_JOIN_HERE) hipLaunchKernelGGL((gn_join_kernel<R, true>), dim3(gn_join_grid(a)), dim3(GN_CHUNK_THREADS), 0, s, a);
         hipLaunchKernelGGL((gn_bwd_apply_kernel<TX, TD, TG, R>), dim3(grid), dim3(GN_CHUNK_THREADS), lds, s, a);
     }
 }
@@ -769,12 +851,18 @@ extern "C" int fs2_group_norm(const void* x, const int* cu, const float* gamma, 
     return FS2_OK;
 }
 
+// a chunked backward's workspace: the chunks' channel sums, their group sums, the utterances' group means
+static long long gn_bwd_floats(int B, int C, int groups, const GnPlan& p) {
+    const long long units = (long long)B * p.nchunk;
+    return units * 2 * C + (p.whole ? 0 : (units + B) * groups * 2);
+}
+
 extern "C" long long fs2_group_norm_bwd_workspace(int B, int max_len, int C, int groups) {
     if (B <= 0 || C <= 0 || groups <= 0 || C % groups || C % 4) return 16;
     long long most = 0;
     for (int t = 0; t < (C % 8 ? 2 : 4); ++t) {
         const GnPlan p = gn_plan(B, max_len, C, groups, t >> 1, t & 1);
-        const long long n = (long long)B * p.nchunk * 2 * C * (long long)sizeof(float);
+        const long long n = gn_bwd_floats(B, C, groups, p) * (long long)sizeof(float);
         most = n > most ? n : most;
     }
     return most;
@@ -797,6 +885,8 @@ extern "C" int fs2_group_norm_bwd(const void* x, const float* stats, const int* 
     FS2_CHECK_ARG((long long)B * p.nchunk * (C / p.W) < (1ll << 22), "fs2_group_norm_bwd: too many workgroups (B=%d)", B);
     GnArgs a = gn_args(B, x, cu, gamma, beta, (float*)stats, workspace, max_len, M, C, groups, ldx, act, p, fs2_make_dropout(seed, site, rate));
     a.dout = dout; a.dx = dx; a.ldd = ldd; a.ldg = ldg;
+    a.gpart = a.part + (size_t)a.units * 2 * C;
+    a.gsum = a.gpart + (size_t)a.units * groups * 2;
 #define FS2_GN(TX, TD)                                              \
     if (dx_dtype == 0) gn_launch_bwd_r<TX, TD, float>(a, p, stream); \
     else gn_launch_bwd_r<TX, TD, bf16_t>(a, p, stream)

@@ -9,6 +9,7 @@ import torch
 
 from fastspeech2_amd import hip
 from fastspeech2_amd.hip import call, ptr, stream
+from tests import test_gpu_alignment as base
 from tests.test_gpu_alignment import ACT_CODE, CODE, DEV, EPS, HALF, LOG2E, TDT, U, Norm, Problem, _bytes, _cu, _half, _near
 from tests.test_gpu_dropout import drop_mul
 
@@ -209,3 +210,22 @@ def test_activations_of_infinities():
         p.bd = torch.tensor([math.inf, -math.inf, math.nan, 3e38, -3e38, 100.0, -100.0, 0.0], device=DEV)
         y = p.forward("fp32")[0][0].cpu()
         assert y[0] == up and y[1] == down and math.isnan(y[2]) and abs(float(y[4])) <= (1 if act == "tanh" else 0) and y[7] == 0
+
+
+@pytest.mark.parametrize("types", [("fp32", "fp32", "fp32", "fp32"), ("fp32", "bf16", "bf16", "bf16"), ("bf16", "fp32", "fp32", "bf16")])
+@pytest.mark.parametrize("lens,C,G,act", [
+    ([700, 0, 35], 512, 1, "silu"),                  # a row takes more than a wave, 16 rows to a chunk
+    ([300, 9], 1024, 1, "tanh"),                     # ... 8 rows
+    ([100, 4], 1024, 2, "none"),
+    ([2500], 512, 1, "none"),                        # 157 chunks of one group
+    ([600, 0, 1], 768, 3, "relu"),                   # a strip is one of three groups
+    ([5000, 17, 90], 24, 8, "tanh"),                 # groups of three channels, narrow strips
+])
+def test_group_norm_of_wide_rows_in_chunks(lens, C, G, act, types):
+    base.test_group_norm(lens, C, G, act, *types)
+
+
+@pytest.mark.parametrize("lens", [[100], [13, 0, 100]])
+def test_group_norm_of_rows_that_no_power_of_two_divides(lens):
+    """524 channels in 131 groups: a row of 131 lanes, one row at a time in a chunk of 256 threads"""
+    base.test_group_norm(lens, 524, 131, "silu", "fp32", "fp32", "fp32", "fp32")
