@@ -29,7 +29,8 @@ struct XArgs {
     unsigned kv_magic;   // 1 / heads-per-utterance of the pair index
     Dropout drop;        // dropout of the probabilities: site drop.stream + head, row = packed query row, col = key index
     int nsplit;          // ranges of the summed axis over workgroups (1: none), partial results to `part`
-    float* part;
+    float* part;         // by slot, b * longest + row of the utterance: the rows at work and no others of the matrix
+    int slots;           // B * longest (of the queries, or of the keys in the backward and the mass)
     // backward
     const void* dctx;    // [Mq, ldo] T
     float* delta;        // [H][Mq]

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
     if (t0 >= t1) {         // this split has no keys: (max, sum) = (-inf, 0)
         for (int r = blk * BQ + tid; r < min(nrow, blk * BQ + BQ); r += 256) {
             const int q = x_query(a, r), head = kvh * a.g + r - q * a.g;
-            float* ml = a.part + (size_t)a.nsplit * a.Mq * a.H * DK + (((size_t)split * a.H + head) * a.Mq + q0 + q) * 2;
+            float* ml = a.part + (size_t)a.nsplit * a.slots * a.H * DK + (((size_t)split * a.H + head) * a.slots + b * a.max_q + q) * 2;
             ml[0] = -INFINITY;
             ml[1] = 0.f;
         }
@@ -247,8 +247,8 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
             x_store_rows<T, DK>(a, (T*)a.ctx, a.ldo, q0, kvh, first, nrow, o[t], own, lane);
         } else {
             const int d = a.H * DK;
-            x_store_rows<float, DK>(a, a.part + (size_t)split * a.Mq * d, d, q0, kvh, first, nrow, o[t], own, lane);
-            float* ml = a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)split * a.H + head) * a.Mq + q0 + q) * 2;
+            x_store_rows<float, DK>(a, a.part + (size_t)split * a.slots * d, d, b * a.max_q, kvh, first, nrow, o[t], own, lane);
+            float* ml = a.part + (size_t)a.nsplit * a.slots * d + (((size_t)split * a.H + head) * a.slots + b * a.max_q + q) * 2;
             if (g == 0 && r < nrow) {
                 ml[0] = m_run[t];
                 ml[1] = l;
@@ -400,8 +400,9 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
             if (a.lse && c == 0) a.lse[(size_t)h * a.Mq + q0 + qq] = mx + __log2f(L);
         } else {
             const size_t d = (size_t)a.H * DK;
-            *(f32x4*)(a.part + ((size_t)split * a.Mq + q0 + qq) * d + h * DK + c) = acc;
-            float* ml = a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)split * a.H + h) * a.Mq + q0 + qq) * 2;
+            const int slot = b * a.max_q + qq;
+            *(f32x4*)(a.part + ((size_t)split * a.slots + slot) * d + h * DK + c) = acc;
+            float* ml = a.part + (size_t)a.nsplit * a.slots * d + (((size_t)split * a.H + h) * a.slots + slot) * 2;
             if (c == 0) {
                 ml[0] = mx;
                 ml[1] = L;
@@ -419,8 +420,8 @@ __global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int 
     if (slot >= (unsigned)B * (unsigned)a.max_q) return;
     const int m = x_row_of(a.cu_q, a.Mq, a.max_q, slot), c = (int)(idx - slot * (unsigned)dv) * 4, h = c / dk;
     if (m < 0) return;
-    const float* ml = a.part + (size_t)a.nsplit * a.Mq * d + ((size_t)h * a.Mq + m) * 2;
-    const size_t step = (size_t)a.H * a.Mq * 2;
+    const float* ml = a.part + (size_t)a.nsplit * a.slots * d + ((size_t)h * a.slots + slot) * 2;
+    const size_t step = (size_t)a.H * a.slots * 2;
     float mx = -INFINITY;
 #pragma unroll 4
     for (int s = 0; s < a.nsplit; ++s) mx = fmaxf(mx, ml[s * step]);
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(256) void xattn_combine_kernel(XArgs a, int B, int 
 #pragma unroll 4
     for (int s = 0; s < a.nsplit; ++s) {
         const float l = ml[s * step + 1], f = __builtin_amdgcn_exp2f(ml[s * step] - mu);
-        const f32x4 o = *(const f32x4*)(a.part + ((size_t)s * a.Mq + m) * d + c);
+        const f32x4 o = *(const f32x4*)(a.part + ((size_t)s * a.slots + slot) * d + c);
         if (l != 0.f) {
             any = true;
             L = fmaf(l, f, L);
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(256) void xattn_combine_few_kernel(XArgs a) {
     if (m < 0) return;
     const size_t d = (size_t)a.H * DK;
     if (tid < a.nsplit) {
-        const float2 t = *(const float2*)(a.part + (size_t)a.nsplit * a.Mq * d + (((size_t)tid * a.H + h) * a.Mq + m) * 2);
+        const float2 t = *(const float2*)(a.part + (size_t)a.nsplit * a.slots * d + (((size_t)tid * a.H + h) * a.slots + blockIdx.y) * 2);
         ms[tid] = t.x;
         ls[tid] = t.y;
     }
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(256) void xattn_combine_few_kernel(XArgs a) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = lane_s; s < a.nsplit; s += NL) {
-        const f32x4 o = *(const f32x4*)(a.part + ((size_t)s * a.Mq + m) * d + h * DK + c);
+        const f32x4 o = *(const f32x4*)(a.part + ((size_t)s * a.slots + blockIdx.y) * d + h * DK + c);
         if (ls[s] != 0.f) acc += o * __builtin_amdgcn_exp2f(ms[s] - mu);
     }
     if (lane_s < NL) *(f32x4*)(red[lane_s] + c) = acc;
@@ -571,7 +572,7 @@ extern "C" long long fs2_cross_attention_workspace(int B, int max_q, int max_k, 
                                                    int dtype) {
     if (B <= 0 || max_q <= 0 || max_k <= 0 || Mq <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return 0;
     const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dtype);
-    return p.nsplit == 1 ? 0 : (long long)p.nsplit * Mq * n_heads * (dk + 2) * (long long)sizeof(float);
+    return p.nsplit == 1 ? 0 : (long long)p.nsplit * B * max_q * n_heads * (dk + 2) * (long long)sizeof(float);
 }
 
 extern "C" int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, float* lse, const int* cu_q,
@@ -595,6 +596,7 @@ extern "C" int fs2_cross_attention(const void* q, const void* k, const void* v, 
     const XPlan p = x_plan(B, max_q, max_k, n_heads, n_kv_heads, dtype);
     a.nsplit = p.nsplit;
     a.part = (float*)workspace;
+    a.slots = p.nsplit > 1 ? B * max_q : 0;                 // (few rows where keys are split)
     FS2_CHECK_ARG(p.nsplit == 1 || (workspace && ((uintptr_t)workspace & 15) == 0),
                   "fs2_cross_attention: this shape needs fs2_cross_attention_workspace bytes, 16-byte aligned");
 #define FS2_X(TT, DKK) return launch_xattn<TT, DKK>(a, p, B, max_q, dk, stream)

@@ -273,9 +273,9 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv_block(const X
             store4<T>(dk + dt * 16, dk_[dt] * a.scale);
             store4<T>(dv + dt * 16, dv_[dt]);
         }
-    } else {                          // part[split][dk, dv][Mk][KV * DK]
-        const size_t w = (size_t)a.KV * DK, half = (size_t)a.Mk * w;
-        float* dst = a.part + (size_t)split * 2 * half + (size_t)(k0 + key) * w + kvh * DK + 4 * g;
+    } else {                          // part[split][dk, dv][slots][KV * DK]
+        const size_t w = (size_t)a.KV * DK, half = (size_t)a.slots * w;
+        float* dst = a.part + (size_t)split * 2 * half + (size_t)(b * a.max_k + key) * w + kvh * DK + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             *(f32x4*)(dst + dt * 16) = dk_[dt] * a.scale;
@@ -432,7 +432,7 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
     // add the four waves' gradients: [wave][32 keys][DK + 4] floats, dv then dk
     constexpr int LDR = DK + 4, SL = DK / 4;
     float* red = (float*)smem;
-    const size_t w = (size_t)a.KV * DK, half = (size_t)a.Mk * w;
+    const size_t w = (size_t)a.KV * DK, half = (size_t)a.slots * w;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
@@ -449,8 +449,9 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
 #pragma unroll
             for (int u = 1; u < 4; ++u) sum += *(const f32x4*)(red + (u * KB + key) * LDR + c);
             const size_t m = (size_t)(k0 + blk * KB + key);
-            if (a.nsplit > 1)                          // part[split][dk, dv][Mk][KV * DK]
-                *(f32x4*)(a.part + (size_t)split * 2 * half + (which == 0 ? half : 0) + m * w + kvh * DK + c) = sum;
+            if (a.nsplit > 1)                          // part[split][dk, dv][slots][KV * DK]
+                *(f32x4*)(a.part + (size_t)split * 2 * half + (which == 0 ? half : 0) + (size_t)(b * a.max_k + blk * KB + key) * w + kvh * DK +
+                          c) = sum;
             else if (which == 0)
                 store4<T>((T*)a.dv + m * a.ldv + kvh * DK + c, sum);
             else
@@ -511,8 +512,8 @@ __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int 
     const unsigned e = idx - slot * 2 * wv;
     const bool is_v = e >= wv;
     const int c = (int)(is_v ? e - wv : e) * 4;
-    const size_t half = (size_t)a.Mk * w;
-    const float* src = a.part + (is_v ? half : 0) + (size_t)m * w + c;
+    const size_t half = (size_t)a.slots * w;
+    const float* src = a.part + (is_v ? half : 0) + (size_t)slot * w + c;
     f32x4 sum = *(const f32x4*)src;
     for (int s = 1; s < a.nsplit; ++s) sum += *(const f32x4*)(src + (size_t)s * 2 * half);
     if (is_v)
@@ -619,8 +620,8 @@ __global__ __launch_bounds__(64 * X_MASS_WAVES, 2) void xattn_mass_kernel(XArgs 
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += red[w][tid];
-        float* dst = a.nsplit == 1 ? a.mass : a.part + (size_t)split * a.H * a.Mk;
-        dst[(size_t)h * a.Mk + k0 + key] = v;
+        if (a.nsplit == 1) a.mass[(size_t)h * a.Mk + k0 + key] = v;
+        else a.part[((size_t)split * a.H + h) * a.slots + b * a.max_k + key] = v;
     }
 }
 
@@ -629,10 +630,10 @@ __global__ __launch_bounds__(256) void xattn_mass_sum_kernel(XArgs a, int B) {
     if (h >= (unsigned)a.H) return;
     const int m = x_row_of(a.cu_k, a.Mk, a.max_k, idx - h * n);
     if (m < 0) return;
-    const size_t at = (size_t)h * a.Mk + m, step = (size_t)a.H * a.Mk;
-    float sum = a.part[at];
-    for (int s = 1; s < a.nsplit; ++s) sum += a.part[s * step + at];
-    a.mass[at] = sum;
+    const size_t step = (size_t)a.H * n;
+    float sum = a.part[idx];
+    for (int s = 1; s < a.nsplit; ++s) sum += a.part[s * step + idx];
+    a.mass[(size_t)h * a.Mk + m] = sum;
 }
 
 // Row ranges of the key workgroups, chosen from the shape: one workgroup for every CU where the keys alone do not give one (the row
@@ -722,7 +723,7 @@ extern "C" long long fs2_cross_attention_bwd_workspace(int B, int max_q, int max
                                                        int dk, int dtype) {
     if (B <= 0 || max_q <= 0 || max_k <= 0 || Mq <= 0 || Mk <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return 16;
     const int n = x_dkv_split(B, max_q, max_k, n_heads, n_kv_heads, dtype);
-    return (x_delta_floats(n_heads, Mq) + (n > 1 ? 2LL * n * Mk * n_kv_heads * dk : 0)) * (long long)sizeof(float);
+    return (x_delta_floats(n_heads, Mq) + (n > 1 ? 2LL * n * B * max_k * n_kv_heads * dk : 0)) * (long long)sizeof(float);
 }
 
 extern "C" int fs2_cross_attention_bwd(const void* q, const void* k, const void* v, const void* ctx, const void* dctx,
@@ -749,6 +750,7 @@ extern "C" int fs2_cross_attention_bwd(const void* q, const void* k, const void*
     a.delta = (float*)workspace;
     a.part = (float*)workspace + x_delta_floats(n_heads, Mq);
     a.nsplit = max_q > 0 && max_k > 0 ? x_dkv_split(B, max_q, max_k, n_heads, n_kv_heads, dtype) : 1;
+    a.slots = a.nsplit > 1 ? B * max_k : 0;                 // (few keys where rows are split)
 #define FS2_X(TT, DKK) return launch_xattn_bwd<TT, DKK>(a, B, max_q, max_k, dk, stream)
     if (dtype == 0) {
         if (dk == 32) FS2_X(XF32, 32);
@@ -768,7 +770,7 @@ extern "C" long long fs2_cross_attention_mass_workspace(int B, int max_q, int ma
     (void)n_kv_heads; (void)dk;
     if (B <= 0 || max_q <= 0 || max_k <= 0 || Mk <= 0 || n_heads <= 0) return 0;
     const int n = x_mass_split(B, max_q, max_k, n_heads, dtype);
-    return n > 1 ? (long long)n * n_heads * Mk * (long long)sizeof(float) : 0;
+    return n > 1 ? (long long)n * n_heads * B * max_k * (long long)sizeof(float) : 0;
 }
 
 extern "C" int fs2_cross_attention_mass(const void* q, const void* k, const float* lse, float* mass, const int* cu_q,
@@ -783,6 +785,7 @@ extern "C" int fs2_cross_attention_mass(const void* q, const void* k, const floa
     a.lse = (float*)lse;
     a.mass = mass;
     a.nsplit = max_q > 0 ? x_mass_split(B, max_q, max_k, n_heads, dtype) : 1;
+    a.slots = a.nsplit > 1 ? B * max_k : 0;
     a.part = (float*)workspace;
     FS2_CHECK_ARG(a.nsplit == 1 || workspace, "fs2_cross_attention_mass: this shape needs fs2_cross_attention_mass_workspace bytes");
 #define FS2_X(TT, DKK) return launch_xattn_mass<TT, DKK>(a, B, max_k, stream)

@@ -170,6 +170,41 @@ def test_fp32_values_pass_whole():
         assert torch.equal(ctx, v.expand(lq, -1))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lq,lk,H,KV", [([1], [5000], 2, 2), ([3, 1], [1900, 0], 4, 2), ([40, 7], [900, 30], 2, 2), ([700, 64], [33, 40], 4, 1)])
+def test_workspaces_hold_what_their_queries_say(lq, lk, H, KV, dtype):
+    """few utterances in the middle of large matrices: the bits of the call on matrices of their own, nothing behind a workspace written"""
+    p = Problem(lq, lk, H, KV, 64, dtype, seed=12)
+    want = p.forward()
+    want = [*want, *p.backward(*want), p.mass(want[1])]
+    front, behind = 3000, 2000
+    big = Problem(lq, lk, H, KV, 64, dtype, seed=12)
+    for name, n in (("q", front), ("kv", front), ("dctx", front)):
+        t = big.d[name]
+        big.d[name] = torch.cat([torch.full((n, t.shape[1]), math.nan, dtype=t.dtype, device=DEV), t,
+                                 torch.full((behind, t.shape[1]), math.nan, dtype=t.dtype, device=DEV)])
+    big.cu_q, big.cu_k = big.cu_q + front, big.cu_k + front
+    big.Mq, big.Mk = big.Mq + front + behind, big.Mk + front + behind
+
+    def guarded(name, *args):
+        n = int(getattr(hip.load(), name)(*args))
+        return torch.full((n + 4096,), 0xAB, dtype=torch.uint8, device=DEV), n
+    n = (p.B, p.max_q, p.max_k)
+    ws = [guarded("fs2_cross_attention_workspace", *n, big.Mq, H, KV, 64, CODE[dtype]),
+          guarded("fs2_cross_attention_bwd_workspace", *n, big.Mq, big.Mk, H, KV, 64, CODE[dtype]),
+          guarded("fs2_cross_attention_mass_workspace", *n, big.Mk, H, KV, 64, CODE[dtype])]
+    ctx, lse = big.forward(ws=ws[0][0])
+    dq, dkv = big.backward(ctx, lse, ws=ws[1][0])
+    m = big.mass(lse, ws=ws[2][0])
+    rq, rk = slice(front, front + sum(lq)), slice(front, front + sum(lk))
+    for got, w, rows in ((ctx, want[0], rq), (dq, want[2], rq), (dkv, want[3], rk)):
+        assert torch.equal(got[rows], w[:rows.stop - rows.start])
+        assert (got[:rows.start] == 7).all() and (got[rows.stop:] == 7).all()
+    for got, w, rows in ((lse, want[1], rq), (m, want[4], rk)):
+        assert torch.equal(got[:, rows], w[:, :rows.stop - rows.start])
+    assert all((t[k:] == 0xAB).all() for t, k in ws)
+
+
 # ---------------------------------------------------------------------------------------------------------- group norm
 @pytest.mark.parametrize("act,xt", [("tanh", "fp32"), ("tanh", "bf16"), ("silu", "fp32"), ("silu", "bf16")])
 def test_activations_and_slopes_are_fp32(act, xt):
