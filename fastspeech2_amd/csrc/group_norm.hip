@@ -737,10 +737,10 @@ static GnPlan gn_plan(int B, int max_len, int C, int G, int x_dtype, int dout_dt
     const bool fewer = x_dtype == 1 && dout_dtype >= 0 && (dout_dtype == 0 || (long long)B * (C / p.W) < 256);
     for (int nt = GN_WHOLE_THREADS;; nt = GN_CHUNK_THREADS) {
         p.LY = p.LX <= 64 ? nt / 64 * (64 / p.LX) : nt / p.LX;
-        const int need = (max_len + p.LY - 1) / p.LY;
+        const int need = (int)(((long long)max_len + p.LY - 1) / p.LY);
         p.whole = nt == GN_WHOLE_THREADS && need <= (fewer ? 8 : 16);
         p.R = !p.whole ? GN_CHUNK_ROWS : (need <= 4 ? 4 : (need <= 8 ? 8 : 16));
-        p.nchunk = p.whole ? 1 : (max_len + p.LY * p.R - 1) / (p.LY * p.R);
+        p.nchunk = p.whole ? 1 : (int)(((long long)max_len + p.LY * p.R - 1) / (p.LY * p.R));
         if (p.whole || nt == GN_CHUNK_THREADS) break;
     }
     return p;
