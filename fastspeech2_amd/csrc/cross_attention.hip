@@ -492,7 +492,7 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
     p.few = rows <= 16;
     p.nsplit = 1;
     if (p.few) {
-        const long tiles = (max_k + 31) / 32;
+        const long tiles = ((long)max_k + 31) / 32;
         // the second launch costs 3 to 4 us, which a wave's fifth tile of a row pays (2 heads of 128, bf16, one sentence: 300 keys 7.0 us whole
         // and 9.4 split, 600 9.2 and 9.5, 1200 14.8 and 9.6; 32 sentences: 8.1 and 9.6, 12.7 and 11.8, 21.7 and 15.2)
         if (tiles > 16 && pairs < 256) {
@@ -507,7 +507,7 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
         // against 62; 32 x 120 x 800, dk = 32: 25 against 31), though each splits its keys for half the rows
         p.qt = rows > 64 && dtype == 1 ? 2 : 1;
         const int kb = dtype == 1 ? 64 : 32, full = dtype == 1 ? 512 : 768;          // workgroups that the chip holds at a time
-        const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = (max_k + kb - 1) / kb;
+        const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = ((long)max_k + kb - 1) / kb;
         // the second launch pays from 400 keys on in bf16, 250 in fp32 (2 heads, 120 rows of one sentence: bf16 250 keys 9.7 us whole and 11.5
         // split, 400 14.1 and 13.5, 810 25 and 15; fp32 250 13.8 and 12.5, 810 42 and 16)
         if (items < (dtype == 1 ? full / 2 : full) && tiles >= (dtype == 1 ? 7 : 8)) {

@@ -642,7 +642,7 @@ __global__ __launch_bounds__(256) void xattn_mass_sum_kernel(XArgs a, int B) {
 // 1600 47 and 26; fp32, dk = 64: 38 and 28, 106 and 29).
 static int x_dkv_split(int B, int max_q, int max_k, int H, int KV, int dtype) {
     const int kb = dtype == 1 ? 32 : 64;
-    const long items = (long)B * KV * ((max_k + kb - 1) / kb), tiles = ((long)max_q * (H / KV) + 31) / 32;
+    const long items = (long)B * KV * (((long)max_k + kb - 1) / kb), tiles = ((long)max_q * (H / KV) + 31) / 32;
     if (items >= 128 || tiles < 8) return 1;
     const long want = 256 / items, most = tiles / 4, n = want < most ? want : most;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
@@ -650,7 +650,7 @@ static int x_dkv_split(int B, int max_q, int max_k, int H, int KV, int dtype) {
 constexpr int x_mass_kt(int dtype) { return dtype == 1 ? 4 : 2; }
 static int x_mass_split(int B, int max_q, int max_k, int H, int dtype) {
     const int kb = 16 * x_mass_kt(dtype);
-    const long items = (long)B * H * ((max_k + kb - 1) / kb), trips = (max_q + 15) / 16 / X_MASS_WAVES;
+    const long items = (long)B * H * (((long)max_k + kb - 1) / kb), trips = ((long)max_q + 15) / 16 / X_MASS_WAVES;
     if (items >= 192 || trips < 8) return 1;
     const long want = 512 / items, most = trips / 2, n = want < most ? want : most;
     return (int)(n < 1 ? 1 : (n > 32 ? 32 : n));
@@ -674,10 +674,11 @@ static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipSt
     const long long nq = ((long long)max_q * a.g + 63) / 64, nk = (max_k + KEYS - 1) / KEYS;
     fs2_x_grid(a, (int)nk, a.KV, B);
     const long long line = a.pairs >= 8 ? (a.pairs + 7) / 8 * 8 : a.pairs;
-    const long long rows = (long long)B * max_q * a.H, delta = (long long)B * max_q * ((a.H + X_DELTA_HEADS - 1) / X_DELTA_HEADS);
-    FS2_CHECK_ARG(rows <= (1 << 28) && line * (nk * a.nsplit + nq) < (1 << 24),
+    const long long delta = (long long)B * max_q * ((a.H + X_DELTA_HEADS - 1) / X_DELTA_HEADS);
+    // (2^24 workgroups of 256: a launch has fewer than 2^32 work items to a dimension)
+    FS2_CHECK_ARG((delta + 15) / 16 < (1 << 24) && line * (nk * a.nsplit + nq) < (1 << 24),
                   "fs2_cross_attention_bwd: B=%d x %d heads x max_q=%d or max_k=%d in one launch", B, a.H, max_q, max_k);
-    if (rows > 0 && max_k > 0) {
+    if (delta > 0 && max_k > 0) {
         hipLaunchKernelGGL((xattn_delta_kernel<T, DK>), dim3((unsigned)((delta + 15) / 16)), dim3(256), 0, stream, a, B);
         FS2_CHECK_LAUNCH("fs2_cross_attention_bwd(delta)");
     }
@@ -698,6 +699,8 @@ static int launch_xattn_bwd(XArgs& a, int B, int max_q, int max_k, int dk, hipSt
 template <typename E, int DK>
 static int launch_xattn_mass(XArgs& a, int B, int max_k, hipStream_t stream) {
     constexpr int KT = x_mass_kt(E::PL == 1);
+    const long long blocks = ((long long)max_k + 16 * KT - 1) / (16 * KT), line = (long long)B * a.H >= 8 ? 8 * blocks : blocks;
+    FS2_CHECK_ARG(line * 64 * X_MASS_WAVES < (1ll << 32), "fs2_cross_attention_mass: B=%d x %d heads x max_k=%d in one launch", B, a.H, max_k);
     constexpr int lds = XTile<E, DK, 16 * KT, 1>::BYTES + X_MASS_WAVES * (E::PL == 1 ? 2 : 1) * XTile<E, DK, 16, 1>::BYTES;
     static unsigned long long ok = 0;
     fs2_allow_lds((const void*)xattn_mass_kernel<E, DK, KT>, lds, &ok);

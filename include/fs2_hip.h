@@ -426,10 +426,13 @@ int fs2_bn_bwd(const float* y, const float* stats, const float* gamma, const flo
  * are left as they were; offsets outside the matrices are clamped to them.)  Outputs overlap no input.  Serves one
  * query per utterance (autoregressive decoding against fixed encoder states) to whole batches; the kernel and a split of the
  * keys over workgroups follow from the shape.  Softmax statistics and sums are fp32; bf16 rounds the result alone (the
- * probabilities are held to 2^-15); fp32 products are exact to 2^-24, an infinite element of fp32 q, k, v (or dctx) counts as NaN, of bf16 as what it is.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row = packed query row, col =
- * key index inside the utterance; rate 0 = none).
- * workspace: fs2_cross_attention_workspace bytes, 16-byte aligned (0: NULL is fine).  It is written by every call: two calls
- * that may overlap (streams, captured graphs) need one each. */
+ * probabilities are held to 2^-15); fp32 products are exact to 2^-24; an infinite element of fp32 q, k, v (or dctx) counts as
+ * NaN, of bf16 as what it is.  Dropout of the probabilities as in fs2_attention_fwd (site of head h = stream_id + h; row =
+ * packed query row, col = key index inside the utterance; rate 0 = none).
+ * workspace: fs2_cross_attention_workspace bytes, 16-byte aligned (0: NULL is fine; it goes by B, max_q and the heads, not by
+ * Mq).  It is written by every call: two calls that may overlap (streams, captured graphs) need one each.
+ * Limits, of this call and the two below (more is refused): B <= 65535, B * n_heads <= 2^19, max_k <= 2^30, and with g = n_heads
+ * / n_kv_heads: g * max_q <= 2^24 and B * n_heads * ceil(max(g * max_q, max_k) / 32) < 2^30. */
 long long fs2_cross_attention_workspace(int B, int max_q, int max_k, int Mq, int n_heads, int n_kv_heads, int dk, int dtype);
 int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, float* lse, const int* cu_q, const int* cu_k,
                         void* workspace, int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk, int ldq,
@@ -438,7 +441,9 @@ int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, 
 /* Its backward, from ctx and lse as fs2_cross_attention left them and dctx [Mq, ldo] T: dq [Mq, ldq], dk_out [Mk, ldk],
  * dv [Mk, ldv] T (the leading dims of q, k, v; written, not added to; gradients of a shared head sum over its query heads).
  * Probabilities are recomputed; every element has one writer and every sum a fixed order (the same bits every time).  workspace:
- * fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, never NULL; one per call that may overlap. */
+ * fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, never NULL; one per call that may overlap.  It takes fewer rows at
+ * once than the forward: B * max_q * ceil(n_heads / 2) < 2^28 - 16, and fewer than 2^24 workgroups, B * n_kv_heads (from 8 on
+ * rounded up to a multiple of 8) times one for every 64 of g * max_q and one for every 32 (fp32: 64) of max_k. */
 long long fs2_cross_attention_bwd_workspace(int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk,
                                             int dtype);
 int fs2_cross_attention_bwd(const void* q, const void* k, const void* v, const void* ctx, const void* dctx, const float* lse,
@@ -450,7 +455,8 @@ int fs2_cross_attention_bwd(const void* q, const void* k, const void* v, const v
  * softmax(q k^T / sqrt(dk))[query, m], from lse as fs2_cross_attention left it (no dropout: the undropped probabilities).
  * With frames as queries and phones as keys this is the expected duration of each phone in frames; a head's masses of an
  * utterance sum to its frame count.  Elements of rows behind cu_k[B] are left as they were.  workspace:
- * fs2_cross_attention_mass_workspace bytes (0: NULL is fine). */
+ * fs2_cross_attention_mass_workspace bytes (0: NULL is fine), one per call that may overlap.  max_k < 2^25 in fp32, 2^26 in bf16
+ * (8 times that where B * n_heads < 8). */
 long long fs2_cross_attention_mass_workspace(int B, int max_q, int max_k, int Mk, int n_heads, int n_kv_heads, int dk, int dtype);
 int fs2_cross_attention_mass(const void* q, const void* k, const float* lse, float* mass, const int* cu_q, const int* cu_k,
                              void* workspace, int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk,
@@ -463,8 +469,9 @@ int fs2_cross_attention_mass(const void* q, const void* k, const float* lse, flo
  * [B][groups][2] = mean, 1 / sqrt(var + eps) (0, 1 / sqrt(eps) for an utterance without rows).  Dtypes 0 fp32, 1 bf16, each on
  * its own; C % 4 == 0 (fp32 x) or 8 (bf16 x), C <= 1024, any group size; ldo % 4 == 0.  The per-utterance counterpart of
  * fs2_bn_stats + fs2_bn_apply: a batch row equals the utterance alone.  Statistics in fp32 from centred squares.  Rows that no
- * utterance owns are left as they were, one longer than max_len is cut there; at most 2^22 utterances (less where they are long).
- * workspace: fs2_group_norm_workspace bytes (0: NULL is fine). */
+ * utterance owns are left as they were, one longer than max_len is cut there.  x, out, gamma and beta 16-byte aligned; outputs
+ * overlap no input.  Fewer than 2^22 workgroups: B utterances x chunks (of at least 8 rows, where max_len is long) x strips (of at
+ * least 64 bytes of a row).  workspace: fs2_group_norm_workspace bytes (0: NULL is fine), one per call that may overlap. */
 long long fs2_group_norm_workspace(int B, int max_len, int C, int groups);
 int fs2_group_norm(const void* x, const int* cu, const float* gamma, const float* beta, void* out, float* stats, void* workspace,
                    int B, int max_len, int M, int C, int groups, int ldx, int ldo, float eps, int act, int x_dtype, int out_dtype,
@@ -472,7 +479,7 @@ int fs2_group_norm(const void* x, const int* cu, const float* gamma, const float
 
 /* Its backward from x and stats alone (activation and dropout are recomputed): dout [M, ldd] (dout_dtype, ldd a multiple of 16
  * bytes of x's type), dx [M, ldg] (dx_dtype), dgamma, dbeta fp32 [C] (sums over all utterances in a fixed order).  workspace:
- * fs2_group_norm_bwd_workspace bytes, never NULL. */
+ * fs2_group_norm_bwd_workspace bytes, never NULL, one per call that may overlap. */
 long long fs2_group_norm_bwd_workspace(int B, int max_len, int C, int groups);
 int fs2_group_norm_bwd(const void* x, const float* stats, const int* cu, const float* gamma, const float* beta, const void* dout,
                        void* dx, float* dgamma, float* dbeta, void* workspace, int B, int max_len, int M, int C, int groups, int ldx,

@@ -205,6 +205,27 @@ def test_workspaces_hold_what_their_queries_say(lq, lk, H, KV, dtype):
     assert all((t[k:] == 0xAB).all() for t, k in ws)
 
 
+@pytest.mark.parametrize("nq", [1, 17])
+def test_as_many_heads_of_utterances_as_one_call_takes(nq):
+    """B * n_heads = 2^19: every result against float64.  2 dk fp32 operations behind an element of size ~10, at most"""
+    B, H, nk, dk = 32768, 16, 2, 32
+    g = torch.Generator(device=DEV).manual_seed(nq)
+    q = torch.randn(B * nq, H * dk, generator=g, device=DEV)
+    k, v = (torch.randn(B * nk, H * dk, generator=g, device=DEV) for _ in range(2))
+    cu_q, cu_k = (torch.arange(B + 1, device=DEV, dtype=torch.int32) * n for n in (nq, nk))
+    ctx, lse, mass = torch.empty_like(q), torch.empty(H, B * nq, device=DEV), torch.empty(H, B * nk, device=DEV)
+    ld, n = H * dk, (B, nq, nk, B * nq, B * nk)
+    call("fs2_cross_attention", ptr(q), ptr(k), ptr(v), ptr(ctx), ptr(lse), ptr(cu_q), ptr(cu_k), None, *n, H, H, dk, ld, ld, ld, ld, 0, 0, 0,
+         0.0, stream())
+    call("fs2_cross_attention_mass", ptr(q), ptr(k), ptr(lse), ptr(mass), ptr(cu_q), ptr(cu_k), None, *n, H, H, dk, ld, ld, 0, stream())
+    Q, K, V = q.double().view(B, nq, H, dk), k.double().view(B, nk, H, dk), v.double().view(B, nk, H, dk)
+    S = torch.stack([(Q * K[:, j, None]).sum(-1) * dk ** -0.5 for j in range(nk)], -1)           # [B, nq, H, nk]
+    P = torch.softmax(S, -1)
+    O = sum(P[..., j, None] * V[:, j, None] for j in range(nk))
+    assert (ctx.double().view(B, nq, H, dk) - O).abs().max() <= 64 * U * 10 * 4
+    assert (mass.double().view(H, B, nk) - P.sum(1).permute(1, 0, 2)).abs().max() <= 64 * U * 10 * 4
+
+
 # ---------------------------------------------------------------------------------------------------------- group norm
 @pytest.mark.parametrize("act,xt", [("tanh", "fp32"), ("tanh", "bf16"), ("silu", "fp32"), ("silu", "bf16")])
 def test_activations_and_slopes_are_fp32(act, xt):
