@@ -11,8 +11,10 @@ llvm-objdump and checked for the hazards that rounds 2 and 3 ran into (DESIGN.md
      (Packed instructions that read kernel-argument SGPRs - epilogue scales - are everywhere and are not this pattern.)
  (b) every loop that both issues an LDS-DMA (global_load_lds_* / buffer_load_* ... lds) and reads LDS (ds_read_*)
      contains an s_waitcnt with a vmcnt field followed by an s_barrier: the pair that orders a DMA's bytes in front of
-     other waves' reads; the wait alone where the buffers are private to a wave.  (attention32_kernel once had its only vmcnt wait hoisted in front of the tile loop: no test
-     failed, single utterances differed from run to run.)
+     other waves' reads.  (attention32_kernel once had its only vmcnt wait hoisted in front of the tile loop: no test
+     failed, single utterances differed from run to run.)  Loops whose buffers are private to a wave need the wait alone:
+     WAVE_PRIVATE names their kernels and how many loops with the whole pair each holds beside them, so that a shared loop
+     cannot lose its barrier and pass for a private one.
  (c) no kernel that loads asynchronously from inline asm (results land in registers the compiler considers written) or
      that counts its vmcnt by hand uses scratch memory: a spill or reload between the load and its wait would save or
      restore stale registers.  Other kernels' scratch is reported.
@@ -36,9 +38,10 @@ LLVM = "/opt/rocm/lib/llvm/bin"
 MAGIC = b"__CLANG_OFFLOAD_BUNDLE__"
 # kernels whose source waits for asynchronous loads by hand (inline-asm ds_read_b64_tr_b16, counted vmcnt)
 NO_SCRATCH = ("attention32_kernel", "attention_split_kernel", "proj_ln_kernel", "gemm_regw_kernel", "conv_gemm256_kernel", "conv_wgrad_kernelIDF16b", "attn_bwd_dq_kernelIDF16b",
-              "attn_bwd_dkv_kernelIDF16b")
-# kernels whose LDS-DMA buffers are private to a wave (no other wave reads them): the vmcnt wait alone orders a DMA's bytes
-WAVE_PRIVATE = ("xattn_few_kernel", "xattn_bwd_kernel", "xattn_mass_kernel")
+              "attn_bwd_dkv_kernelIDF16b", "xattn_mass_kernel")
+# kernels with LDS-DMA buffers that are private to a wave (no other wave reads them, the vmcnt wait alone orders a DMA's bytes), and the
+# loops they have beside those whose tiles are shared: the backward's dq workgroups stage K and V for all four waves
+WAVE_PRIVATE = {"xattn_few_kernel": 0, "xattn_bwd_kernel": 1, "xattn_mass_kernel": 0}
 READLANE_WINDOW = 8
 
 
@@ -133,6 +136,8 @@ def check_function(name, insns, findings):
             findings.append("%s: %d v_pk_mul_f32 / v_pk_fma_f32 (the SLP-vectorised form that miscomputed beside bf16 MFMAs)" % (name, n))
     # (b) loops (backward branches) with LDS-DMA and LDS reads need a vmcnt wait followed by a barrier inside
     index = {a: k for k, (a, _, _, _) in enumerate(insns)}
+    private = [n for k, n in WAVE_PRIVATE.items() if k in name]
+    shared_loops, dma_loops = set(), set()
     for k, (addr, mn, ops, word) in enumerate(insns):
         if not (mn.startswith("s_cbranch") or mn == "s_branch"):
             continue
@@ -146,18 +151,22 @@ def check_function(name, insns, findings):
             continue
         ok = False
         waited = False
+        dma_loops.add(target)
         for _, m, o, _ in body:
             if m == "s_waitcnt" and "vmcnt" in o:
                 waited = True
-                if any(k in name for k in WAVE_PRIVATE):
-                    ok = True
-                    break
             elif m == "s_barrier" and waited:
                 ok = True
+                shared_loops.add(target)
                 break
+        if private and waited:
+            ok = True
         if not ok:
             findings.append("%s: the loop %#x..%#x issues LDS-DMA and reads LDS but holds no `s_waitcnt vmcnt` + `s_barrier` pair"
                             % (name, target, addr))
+    if private and dma_loops and len(shared_loops) < private[0]:
+        findings.append("%s: %d loops hold the `s_waitcnt vmcnt` + `s_barrier` pair, its shared tiles need %d"
+                        % (name, len(shared_loops), private[0]))
 
 
 def main():
