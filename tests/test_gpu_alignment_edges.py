@@ -226,6 +226,24 @@ def test_as_many_heads_of_utterances_as_one_call_takes(nq):
     assert (mass.double().view(H, B, nk) - P.sum(1).permute(1, 0, 2)).abs().max() <= 64 * U * 10 * 4
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lq,lk", [([57, 120, 33], [9, 21, 5]), ([1, 800, 13, 7], [3, 120, 1, 40])])
+def test_durations_of_the_mass_fill_the_frames(lq, lk, dtype):
+    """from the mass to the length regulator: durations are differences of the rounded running sum, so every utterance gets its frames back, every phone within one frame of
+    its mass (rounding both ends of its span)"""
+    p = Problem(lq, lk, 2, 2, 64, dtype, seed=13)
+    mass, cu_p, B = p.mass(p.forward()[1]), p.cu_k, len(lq)
+    lens = (cu_p[1:] - cu_p[:-1]).long()
+    run = torch.cat([mass.new_zeros(1, dtype=torch.float64), mass[:, :cu_p[-1]].double().mean(0).cumsum(0)])
+    start = run[cu_p[:-1].long()].repeat_interleave(lens)
+    dur = ((run[1:] - start).round() - (run[:-1] - start).round()).int()
+    used, cum = torch.empty_like(dur), torch.empty_like(dur)
+    olens, cu_f = torch.empty(B, dtype=torch.int32, device=DEV), torch.empty(B + 1, dtype=torch.int32, device=DEV)
+    call("fs2_lr_plan", ptr(dur), ptr(cu_p), 1.0, ptr(used), ptr(cum), ptr(olens), ptr(cu_f), B, stream())
+    assert olens.tolist() == lq and torch.equal(used, dur) and (dur >= 0).all()
+    assert (dur - mass[:, :sum(lk)].double().mean(0)).abs().max() <= 1 + 1e-3
+
+
 # ---------------------------------------------------------------------------------------------------------- group norm
 @pytest.mark.parametrize("act,xt", [("tanh", "fp32"), ("tanh", "bf16"), ("silu", "fp32"), ("silu", "bf16")])
 def test_activations_and_slopes_are_fp32(act, xt):
