@@ -133,7 +133,7 @@ template <typename E, int DK, bool DROP> __device__ __forceinline__ void x_dq_bl
                 const int key = kt * KB + nt * 16 + 4 * g + e;
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[nt][e], a.scale_log2e, -lse_q));
                 float dpv = dp[nt][e];
-                if constexpr (DROP) dpv *= drop_mul(dh, (uint32_t)qrow, (uint32_t)key);
+                if constexpr (DROP) dpv = drop_keep(dh, (uint32_t)qrow, (uint32_t)key) ? dpv * dh.inv_keep : 0.f;
                 s[nt][e] = p * (dpv - del);
             }
         if (kt * KB + KB > lenk) {
@@ -392,10 +392,14 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
                     const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[rt][kt][e], a.scale_log2e, -lse_r)) : 0.f;
-                    float mul = 1.0f;
-                    if constexpr (DROP) mul = drop_mul(dh, (uint32_t)(q0 + q), (uint32_t)min(blk * KB + kt * 16 + i, lenk - 1));
-                    dp[rt][kt][e] = ok ? p * (dp[rt][kt][e] * mul - del_r) : 0.f;
-                    s[rt][kt][e] = p * mul;
+                    float pd = p, dpv = dp[rt][kt][e];
+                    if constexpr (DROP) {
+                        const bool keep = drop_keep(dh, (uint32_t)(q0 + q), (uint32_t)min(blk * KB + kt * 16 + i, lenk - 1));
+                        pd = keep ? p * dh.inv_keep : 0.f;
+                        dpv = keep ? dpv * dh.inv_keep : 0.f;
+                    }
+                    dp[rt][kt][e] = ok ? p * (dpv - del_r) : 0.f;
+                    s[rt][kt][e] = pd;
                 }
             }
         }
