@@ -77,7 +77,7 @@ __device__ __forceinline__ bool x_decode(const XArgs& a, int heads, int& b, int&
         pair = blockIdx.y;
     }
     if (pair >= a.pairs) return false;
-    b = heads == 1 ? pair : (int)__umulhi((unsigned)pair, a.kv_magic);       // pair < 2^24, heads <= 4096: exact
+    b = heads == 1 ? pair : (int)__umulhi((unsigned)pair, a.kv_magic);       // exact for pair * heads < 2^32: pair < 2^19, heads <= 4096
     h = pair - b * heads;
     return true;
 }

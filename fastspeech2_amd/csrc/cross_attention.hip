@@ -506,7 +506,10 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
         // fp32: with one, three workgroups share a CU and hide each other's LDS reads and splits (32 x 240 rows x 810 keys, dk = 96: 59 us
         // against 62; 32 x 120 x 800, dk = 32: 25 against 31), though each splits its keys for half the rows
         p.qt = rows > 64 && dtype == 1 ? 2 : 1;
-        const int kb = dtype == 1 ? 64 : 32, full = dtype == 1 ? 512 : 768;          // workgroups that the chip holds at a time
+        // as many workgroups as the chip holds at dk = 128 in bf16, at dk = 96 in fp32, and for every head dim: fp32 of 128 has two to a CU but takes
+        // 52 us with 768 and 58 with 512 (32 x 120 rows x 810 keys, 2 heads; dk = 96 38 and 48), small bf16 heads fit more but gain nothing
+        // (1024 against 512: dk = 32 18.5 and 17.5, dk = 64 22.6 and 20.4)
+        const int kb = dtype == 1 ? 64 : 32, full = dtype == 1 ? 512 : 768;
         const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = ((long)max_k + kb - 1) / kb;
         // the second launch pays from 400 keys on in bf16, 250 in fp32 (2 heads, 120 rows of one sentence: bf16 250 keys 9.7 us whole and 11.5
         // split, 400 14.1 and 13.5, 810 25 and 15; fp32 250 13.8 and 12.5, 810 42 and 16)

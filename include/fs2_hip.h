@@ -440,7 +440,7 @@ int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, 
 
 /* Its backward, from ctx and lse as fs2_cross_attention left them and dctx [Mq, ldo] T: dq [Mq, ldq], dk_out [Mk, ldk],
  * dv [Mk, ldv] T (the leading dims of q, k, v; written, not added to; gradients of a shared head sum over its query heads).
- * Probabilities are recomputed; every element has one writer and every sum a fixed order (the same bits every time).  workspace:
+ * Probabilities are recomputed, sum dctx ctx is taken from ctx as stored; every element has one writer and every sum a fixed order (the same bits every time).  workspace:
  * fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, never NULL; one per call that may overlap.  It takes fewer rows at
  * once than the forward: B * max_q * ceil(n_heads / 2) < 2^28 - 16, and fewer than 2^24 workgroups, B * n_kv_heads (from 8 on
  * rounded up to a multiple of 8) times one for every 64 of g * max_q and one for every 32 (fp32: 64) of max_k. */

@@ -303,3 +303,40 @@ def test_group_norm_of_wide_rows_in_chunks(lens, C, G, act, types):
 def test_group_norm_of_rows_that_no_power_of_two_divides(lens):
     """524 channels in 131 groups: a row of 131 lanes, one row at a time in a chunk of 256 threads"""
     base.test_group_norm(lens, 524, 131, "silu", "fp32", "fp32", "fp32", "fp32")
+
+
+def test_group_norm_of_many_chunks_in_graphs_and_streams():
+    """94 chunks: the join is a launch of its own.  Two captured graphs with a workspace each, replayed in turn with eager work between,
+    then calls on two streams at once"""
+    probs = [Norm([1500, 0, 300], 512, 1, "tanh", "fp32", seed=s) for s in (1, 2)]
+    for p in probs:
+        p.dout = p.dout.to(DEV)
+    run = lambda p: (lambda y, st: [y, st, *p.backward(st, "fp32", "fp32")])(*p.forward("fp32"))
+    want = [run(p) for p in probs]
+    torch.cuda.synchronize()
+    graphs = []
+    for p in probs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run(p)
+        graphs.append((g, out))
+    for _ in range(3):
+        for (g, out), w, p in zip(graphs, want, probs):
+            for o in out:
+                o.fill_(3.0)
+            g.replay()
+            run(p)
+            torch.cuda.synchronize()
+            for got, ref in zip(out, w):
+                assert torch.equal(got[:1800], ref[:1800]) if got.shape[0] == p.M else torch.equal(got, ref)
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for p, st in zip(probs, streams):
+            with torch.cuda.stream(st):
+                got.append(run(p))
+    for st in streams:
+        st.synchronize()
+    for k, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k % 2]))
