@@ -12,14 +12,15 @@
 //                each with its own 32-key tiles in wave-private LDS (fp32: K straight into registers); one merge.
 // Where the pairs alone do not fill the chip, ranges of keys go to `nsplit` workgroups and a second kernel merges.
 //
-// Measured (floor: bytes at 5.2 TB/s, or products at 1198 TFLOP/s bf16, 154 fp32):
-//   one frame of 256 sentences, 8 heads on 2 of 64, 160 keys, bf16: 7.5 us for 21 MB (2.8 TB/s; floor 4.1); one sentence 5.8 us, of
+// Measured (floor: bytes at 5.2 TB/s, or products at 1198 TFLOP/s bf16, a sixth of that fp32, whichever is longer):
+//   one frame of 256 sentences, 8 heads on 2 of 64, 160 keys, bf16: 8.1 us for 21 MB (2.6 TB/s; floor 4.1); one sentence 5.8 us, of
 //     which the launch is 3.8.
-//   32 x 800 frames over 120 phones, 2 heads of 128, bf16: 14.2 us for 31 MB (2.2 TB/s; floor 6.0).  Two key tiles leave nothing to
-//     overlap: a workgroup waits for its queries and first keys, multiplies, and writes.
-//   32 x 120 phones over 810 frames, 4 heads on 2 of 96, fp32: 55 us, 4.8 GFLOP = 87 TFLOP/s (floor 31), 6 of it the merge.  Each
-//     tile costs a SIMD 1150 cycles of MFMA (six bf16 products for one of fp32), 1400 of splitting and softmax and the CU 1700 of LDS;
-//     three workgroups on a CU overlap them to about 3000.
+//   32 x 800 frames over 120 phones, 2 heads of 128, bf16: 15.9 us for 31 MB (1.9 TB/s; floor 6.0), 18.9 with dropout.  Two key tiles leave
+//     nothing to overlap: a workgroup waits for its queries and first keys, multiplies, and writes.  Over 900 keys 50.8 us, 23.6 GFLOP = 465
+//     TFLOP/s (floor 20): splitting P costs 10 us of it, in vector instructions.
+//   32 x 120 phones over 810 frames, 4 heads on 2 of 96, fp32: 60 us, 4.8 GFLOP = 80 TFLOP/s (floor 24), 6 of it the merge, 67 with
+//     dropout.  The matrix pipe is busy a third of the time; splitting, softmax and LDS reads (31 % of their cycles bank conflicts) fill the
+//     rest, and three workgroups on a CU overlap only part of it.
 #include "cross_attention.h"
 
 namespace fs2 {
@@ -258,8 +259,8 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
 }
 
 // At most 16 packed rows per (utterance, shared head).  grid (nsplit, KV, B); wave w takes the 32-key tiles t0 + w, + 4, ..
-// 256 sentences x 2000 keys, 2 heads of 128, bf16: 98 us for 524 MB (5.3 TB/s, a large copy's rate); short key lists are a chain of dependent
-// reads (one sentence of 120 keys: 4.8 us in the kernel, eight waves instead of four 5.7).
+// 256 sentences x 2000 keys, 2 heads of 128, bf16: 102 us for 524 MB (5.1 TB/s, a large copy's rate); short key lists are a chain of dependent
+// reads (one sentence of 120 keys: 5.1 us in the kernel; with eight waves instead of four 0.9 more).
 template <typename E, int DK>
 __global__ __launch_bounds__(256, 1) void xattn_few_kernel(XArgs a) {
     typedef typename E::mem T;
@@ -493,26 +494,26 @@ static XPlan x_plan(int B, int max_q, int max_k, int H, int KV, int dtype) {
     p.nsplit = 1;
     if (p.few) {
         const long tiles = ((long)max_k + 31) / 32;
-        // the second launch costs 3 to 4 us, which a wave's fifth tile of a row pays (2 heads of 128, bf16, one sentence: 300 keys 7.0 us whole
-        // and 9.4 split, 600 9.2 and 9.5, 1200 14.8 and 9.6; 32 sentences: 8.1 and 9.6, 12.7 and 11.8, 21.7 and 15.2)
+        // the second launch costs 3 to 4 us, which a wave's fifth tile of a row pays (2 heads of 128, bf16, one sentence: 300 keys 7.7 us whole
+        // and 9.4 split, 600 10.5 and 9.6, 1200 17.5 and 9.8; 32 sentences: 8.8 and 9.4, 14.4 and 12.1, 25.3 and 15.9)
         if (tiles > 16 && pairs < 256) {
-            // a tile to every wave up to 32 ranges, four tiles to a wave beyond (one frame over 65000 keys, dk = 128: 127 ranges
-            // 14.5 + 7.4 us, 253 ranges 14.4 + 13.0 us, 32 ranges 26.6 + 4.5 us)
+            // a tile to every wave up to 32 ranges, four tiles to a wave beyond (one frame over 65000 keys, dk = 128: 24 us with 127
+            // ranges, 740 without; when P was one number 127 ranges took 14.5 + 7.4 us, 253 ranges 14.4 + 13.0, 32 ranges 26.6 + 4.5)
             const long want = 512 / pairs, some = tiles / 4 < 32 ? tiles / 4 : 32, most = tiles / 16 > some ? tiles / 16 : some;
             p.nsplit = (int)(want < most ? want : most);
         }
     } else {
-        // two row tiles to a wave: bf16, whose tiles cost nothing but their reads (32 x 800 rows over 120 keys: 15.2 us, one: 17.0).
-        // fp32: with one, three workgroups share a CU and hide each other's LDS reads and splits (32 x 240 rows x 810 keys, dk = 96: 59 us
-        // against 62; 32 x 120 x 800, dk = 32: 25 against 31), though each splits its keys for half the rows
+        // two row tiles to a wave: bf16, whose tiles cost nothing but their reads (32 x 800 rows over 120 keys: 15.9 us, one: 17.9).
+        // fp32: with one, three workgroups share a CU and hide each other's LDS reads and splits, though each splits its keys for half the
+        // rows (32 x 240 rows x 810 keys, dk = 96, planes still cut off: 59 us against 62 with two tiles and two workgroups)
         p.qt = rows > 64 && dtype == 1 ? 2 : 1;
         // as many workgroups as the chip holds at dk = 128 in bf16, at dk = 96 in fp32, and for every head dim: fp32 of 128 has two to a CU but takes
         // 52 us with 768 and 58 with 512 (32 x 120 rows x 810 keys, 2 heads; dk = 96 38 and 48), small bf16 heads fit more but gain nothing
         // (1024 against 512: dk = 32 18.5 and 17.5, dk = 64 22.6 and 20.4)
         const int kb = dtype == 1 ? 64 : 32, full = dtype == 1 ? 512 : 768;
         const long items = pairs * ((rows + 64 * p.qt - 1) / (64 * p.qt)), tiles = ((long)max_k + kb - 1) / kb;
-        // the second launch pays from 400 keys on in bf16, 250 in fp32 (2 heads, 120 rows of one sentence: bf16 250 keys 9.7 us whole and 11.5
-        // split, 400 14.1 and 13.5, 810 25 and 15; fp32 250 13.8 and 12.5, 810 42 and 16)
+        // the second launch pays from 400 keys on in bf16, 250 in fp32 (2 heads, 120 rows of one sentence: bf16 of 128 250 keys 11.6 us whole
+        // and 12.5 split, 400 17.2 and 14.7, 810 32 and 16.5; fp32 of 64 250 13.4 and 12.4, 810 40 and 16)
         if (items < (dtype == 1 ? full / 2 : full) && tiles >= (dtype == 1 ? 7 : 8)) {
             const long want = full / items, most = tiles / (128 / kb);
             p.nsplit = (int)(want < most ? want : most);

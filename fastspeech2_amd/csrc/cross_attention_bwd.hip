@@ -12,9 +12,9 @@
 
 namespace fs2 {
 
-// Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16: delta 6.4 us for 27 MB (4.2 TB/s), the rest 37 us
-// (floor of the whole step, forward included, 11.8 us); 3 x 1601 frames over 301 phones, 4 heads on 2 of 96, fp32: 5 + 78 + 5.5 us for
-// 4.9 GFLOP (floor 47.7 with the forward).
+// Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16: delta 6.4 us for 27 MB (4.2 TB/s), the rest 37.5 us
+// (whole step, forward included, 56 us, 71 with dropout, where the last spills 10 registers; floor 11.8); 3 x 1601 frames over 301 phones,
+// 4 heads on 2 of 96, fp32: 5 + 77 + 5.5 us for 4.9 GFLOP (whole step 114, 127 with dropout, 12 registers spilled; floor 37).
 
 template <typename T> __device__ __forceinline__ f32x4 x_load4(const T* p) {
     if constexpr (sizeof(T) == 4) return *(const f32x4*)p;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256) void xattn_dkv_sum_kernel(XArgs a, int B, int 
 // tiles.  S^T = K Q^T: a lane owns one query and 4 keys of every 16, adds up its own queries' weights over the whole loop, and the 16
 // queries of a row of lanes meet only at the end.  32 x 800 queries, 120 keys, 2 heads of 128, bf16: 9.4 us for 16 MB (1.7 TB/s; floor
 // 3.0; 11.6 with four waves): the keys' wait and the first queries' behind it, then seven tiles to a wave, in workgroups fewer than CUs.
-// 3100 queries, 512 keys, 4 heads of 64, fp32: 12.9 us with the sum over nine query ranges (floor 3.9).  64 keys to a workgroup in bf16;
+// 3100 queries, 512 keys, 4 heads of 64, fp32: 13.5 us with the sum over nine query ranges (floor 3.0).  64 keys to a workgroup in bf16;
 // 32 in fp32, whose keys take three times the registers.
 constexpr int X_MASS_WAVES = 8;
 
@@ -642,8 +642,8 @@ __global__ __launch_bounds__(256) void xattn_mass_sum_kernel(XArgs a, int B) {
 
 // Row ranges of the key workgroups, chosen from the shape: one workgroup for every CU where the keys alone do not give one (the row
 // workgroups fill the rest: 8 x 800 over 120, fp32, dk = 128: 47 us against 54 with two to a CU), and at least four row tiles to a
-// workgroup.  The join pays from 256 rows on (one sentence of 400 frames over 120 phones, whole step: bf16 25.1 us whole, 23.5 split, of
-// 1600 47 and 26; fp32, dk = 64: 38 and 28, 106 and 29).
+// workgroup.  The join pays from 256 rows on (one sentence of 400 frames over 120 phones, whole step without any split and with:
+// bf16 27.4 and 25.1 us, of 1600 52.6 and 27.3; fp32, dk = 64: 39.6 and 28.2, 110 and 29.9).
 static int x_dkv_split(int B, int max_q, int max_k, int H, int KV, int dtype) {
     const int kb = dtype == 1 ? 32 : 64;
     const long items = (long)B * KV * (((long)max_k + kb - 1) / kb), tiles = ((long)max_q * (H / KV) + 31) / 32;
