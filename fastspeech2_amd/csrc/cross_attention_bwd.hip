@@ -2,6 +2,8 @@
 // by tile from q, k and the saved log-sum-exp, never stored.  With S = q k^T / sqrt(dk), P = exp2(S log2 e - lse), D the
 // dropout multiplier, O = (P o D) v and upstream dO:
 //   delta = sum_dv dO o O                                         xattn_delta_kernel
+//         = sum_keys P o dP, which knows nothing of ctx's rounding: taken instead where a bf16 workgroup has all keys of the utterance
+//           (dq up to 64, dk up to 32 of them; the fewer keys, the more that rounding weighs: 1.4 times the result's own at two)
 //   dP = dO v^T o D,  dS = P o (dP - delta)                       xattn_bwd_kernel, two kinds of workgroups:
 //   dq = dS k / sqrt(dk)                                            x_dq_block: one wave per 16 packed rows
 //   dk = dS^T q / sqrt(dk),  dv = (P o D)^T dO                      x_dkv32_block (bf16), x_dkv_block (fp32)
@@ -13,7 +15,7 @@
 namespace fs2 {
 
 // Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16: delta 6.4 us for 27 MB (4.2 TB/s), the rest 37.5 us
-// (whole step, forward included, 56 us, 71 with dropout, where the last spills 10 registers; floor 11.8); 3 x 1601 frames over 301 phones,
+// (whole step, forward included, 57 us, 70 with dropout, where the last spills 8 registers; floor 11.8); 3 x 1601 frames over 301 phones,
 // 4 heads on 2 of 96, fp32: 5 + 77 + 5.5 us for 4.9 GFLOP (whole step 114, 127 with dropout, 12 registers spilled; floor 37).
 
 template <typename T> __device__ __forceinline__ f32x4 x_load4(const T* p) {
@@ -131,18 +133,29 @@ template <typename E, int DK, bool DROP> __device__ __forceinline__ void x_dq_bl
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int key = kt * KB + nt * 16 + 4 * g + e;
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[nt][e], a.scale_log2e, -lse_q));
-                float dpv = dp[nt][e];
-                if constexpr (DROP) dpv = drop_keep(dh, (uint32_t)qrow, (uint32_t)key) ? dpv * dh.inv_keep : 0.f;
-                s[nt][e] = p * (dpv - del);
+                s[nt][e] = __builtin_amdgcn_exp2f(fmaf(s[nt][e], a.scale_log2e, -lse_q));
+                if constexpr (DROP) dp[nt][e] = drop_keep(dh, (uint32_t)qrow, (uint32_t)key) ? dp[nt][e] * dh.inv_keep : 0.f;
             }
         if (kt * KB + KB > lenk) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (kt * KB + nt * 16 + 4 * g + e >= lenk) s[nt][e] = 0.f;
+                    if (kt * KB + nt * 16 + 4 * g + e >= lenk) s[nt][e] = dp[nt][e] = 0.f;
         }
+        if constexpr (E::PL == 1)
+            if (lenk <= KB) {            // all keys at hand: delta without ctx's rounding
+                del = 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) del = fmaf(s[nt][e], dp[nt][e], del);
+                del = rows_sum(del);
+            }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][e] *= dp[nt][e] - del;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const frag_t dsf = x_pack<E>(s[2 * c], s[2 * c + 1]);
@@ -379,7 +392,8 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
         for (int rt = 0; rt < 2; ++rt) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float lse_r = __shfl(stat, rt * 16 + 4 * g + e, 64), del_r = __shfl(stat, 32 + rt * 16 + 4 * g + e, 64);
+                const float lse_r = __shfl(stat, rt * 16 + 4 * g + e, 64);
+                float del_r = __shfl(stat, 32 + rt * 16 + 4 * g + e, 64);
                 const int r = qt * 32 + rt * 16 + 4 * g + e;
                 const bool ok = r < nrow;
                 Dropout dh = a.drop;
@@ -389,18 +403,25 @@ template <int DK, bool DROP> __device__ __forceinline__ void x_dkv32_block(const
                     q = x_query(a, rr);
                     dh.stream += (uint32_t)(kvh * a.g + rr - q * a.g);
                 }
+                float p[KT];
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[rt][kt][e], a.scale_log2e, -lse_r)) : 0.f;
-                    float pd = p, dpv = dp[rt][kt][e];
+                    p[kt] = ok ? __builtin_amdgcn_exp2f(fmaf(s[rt][kt][e], a.scale_log2e, -lse_r)) : 0.f;
+                    s[rt][kt][e] = p[kt];
                     if constexpr (DROP) {
                         const bool keep = drop_keep(dh, (uint32_t)(q0 + q), (uint32_t)min(blk * KB + kt * 16 + i, lenk - 1));
-                        pd = keep ? p * dh.inv_keep : 0.f;
-                        dpv = keep ? dpv * dh.inv_keep : 0.f;
+                        s[rt][kt][e] = keep ? p[kt] * dh.inv_keep : 0.f;
+                        dp[rt][kt][e] = keep ? dp[rt][kt][e] * dh.inv_keep : 0.f;
                     }
-                    dp[rt][kt][e] = ok ? p * (dpv - del_r) : 0.f;
-                    s[rt][kt][e] = pd;
                 }
+                if (lenk <= KB) {            // all keys at hand: delta without ctx's rounding
+                    del_r = 0.f;
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) del_r = kt * 16 + i < lenk ? fmaf(p[kt], dp[rt][kt][e], del_r) : del_r;
+                    del_r = row16_sum(del_r);
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) dp[rt][kt][e] = ok ? p[kt] * (dp[rt][kt][e] - del_r) : 0.f;
             }
         }
         frag_t pf[KT], pr[KT], dsf[KT], dsr[KT];

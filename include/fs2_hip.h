@@ -440,10 +440,11 @@ int fs2_cross_attention(const void* q, const void* k, const void* v, void* ctx, 
 
 /* Its backward, from ctx and lse as fs2_cross_attention left them and dctx [Mq, ldo] T: dq [Mq, ldq], dk_out [Mk, ldk],
  * dv [Mk, ldv] T (the leading dims of q, k, v; written, not added to; gradients of a shared head sum over its query heads).
- * Probabilities are recomputed, sum dctx ctx is taken from ctx as stored; every element has one writer and every sum a fixed order (the same bits every time).  workspace:
- * fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, never NULL; one per call that may overlap.  It takes fewer rows at
- * once than the forward: B * max_q * ceil(n_heads / 2) < 2^28 - 16, and fewer than 2^24 workgroups, B * n_kv_heads (from 8 on
- * rounded up to a multiple of 8) times one for every 64 of g * max_q and one for every 32 (fp32: 64) of max_k. */
+ * Probabilities are recomputed; sum dctx ctx is taken from ctx as stored (bf16: for an utterance of up to 64 keys in dq, of up to
+ * 32 in dk, from the probabilities).  Every element has one writer and every sum a fixed order (the same bits every time).
+ * workspace: fs2_cross_attention_bwd_workspace bytes, 16-byte aligned, never NULL; one per call that may overlap.  It takes fewer
+ * rows at once than the forward: B * max_q * ceil(n_heads / 2) <= 2^28 - 16, and fewer than 2^24 workgroups, B * n_kv_heads (from 8
+ * on rounded up to a multiple of 8) times one for every 64 of g * max_q and one for every 32 (fp32: 64) of max_k. */
 long long fs2_cross_attention_bwd_workspace(int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk,
                                             int dtype);
 int fs2_cross_attention_bwd(const void* q, const void* k, const void* v, const void* ctx, const void* dctx, const float* lse,
@@ -455,8 +456,8 @@ int fs2_cross_attention_bwd(const void* q, const void* k, const void* v, const v
  * softmax(q k^T / sqrt(dk))[query, m], from lse as fs2_cross_attention left it (no dropout: the undropped probabilities).
  * With frames as queries and phones as keys this is the expected duration of each phone in frames; a head's masses of an
  * utterance sum to its frame count.  Elements of rows behind cu_k[B] are left as they were.  workspace:
- * fs2_cross_attention_mass_workspace bytes (0: NULL is fine), one per call that may overlap.  max_k < 2^25 in fp32, 2^26 in bf16
- * (8 times that where B * n_heads < 8). */
+ * fs2_cross_attention_mass_workspace bytes (0: NULL is fine), one per call that may overlap.  max_k <= 2^25 - 32 in fp32, 2^26 -
+ * 64 in bf16 (2^28 - 32 and 2^29 - 64 where B * n_heads < 8). */
 long long fs2_cross_attention_mass_workspace(int B, int max_q, int max_k, int Mk, int n_heads, int n_kv_heads, int dk, int dtype);
 int fs2_cross_attention_mass(const void* q, const void* k, const float* lse, float* mass, const int* cu_q, const int* cu_k,
                              void* workspace, int B, int max_q, int max_k, int Mq, int Mk, int n_heads, int n_kv_heads, int dk,

@@ -66,6 +66,47 @@ def test_bf16_results_are_rounded_once(lq, lk, H, KV, dk, drop):
     _near(dkv[:, KV * dk:].contiguous(), wv, tv, sum(lk), "dv")
 
 
+@pytest.mark.parametrize("drop", [0.0, 0.2])
+@pytest.mark.parametrize("lq,lk,H,KV,dk", [
+    ([100, 33], [2, 1], 2, 2, 64), ([70, 7], [8, 31], 4, 2, 32), ([1, 1, 40], [5, 32, 17], 4, 1, 128), ([300], [16], 2, 2, 96),
+    ([100, 65], [33, 64], 2, 2, 64), ([40, 1], [50, 61], 4, 2, 128)])
+def test_bf16_score_gradients_of_few_keys_are_rounded_once(lq, lk, H, KV, dk, drop):
+    """up to 64 keys dq, up to 32 dk as well take delta = sum P dP from what is at hand and not from the rounded ctx, whose rounding weighs
+    most where few keys share it.  dP: (dk + 2) u sum|dO||V|; delta: that and P's own error, n u of its terms; dS = P (dP - delta) held to
+    2^-16 by two numbers; then half a step of the result"""
+    p = Problem(lq, lk, H, KV, dk, "bf16", seed=23)
+    drop = (77, 4, drop)
+    ctx, lse = p.forward(drop)
+    dq, dkv = p.backward(ctx, lse, drop)
+    q, kv, do, s = p.q.double(), p.kv.double(), p.dctx.double(), dk ** -0.5
+    wq, tq = torch.zeros(p.Mq, H * dk, dtype=torch.float64), torch.zeros(p.Mq, H * dk, dtype=torch.float64)
+    wk, tk = torch.zeros(p.Mk, KV * dk, dtype=torch.float64), torch.zeros(p.Mk, KV * dk, dtype=torch.float64)
+    for b, h, rq, rk, hc, kc, vc in p.pairs():
+        n, nq = rk.stop - rk.start, rq.stop - rq.start
+        Q, K, V, D = q[rq, hc], kv[rk, kc], kv[rk, vc], do[rq, hc]
+        S = Q @ K.T * s
+        P = torch.softmax(S, 1)
+        M = drop_mul(drop[0], drop[1] + h, nq, n, drop[2], rq.start) if drop[2] else torch.ones_like(P)
+        dS = (dk + 4) * U * (Q.abs() @ K.abs().T) * s
+        rP = dS + dS.max(1, keepdim=True).values + (2 * n + 16) * U + 4 * U * LOG2E * S.abs().max(1, keepdim=True).values
+        rP = rP + 8 * U * (1 + torch.logsumexp(S, 1, keepdim=True).abs() * LOG2E)
+        dP = (D @ V.T) * M
+        eP = (dk + 2) * U * (D.abs() @ V.abs().T) * M + 2 * U * dP.abs()
+        delta = (P * dP).sum(1, keepdim=True)
+        eD = (P * (eP + (rP + (n + 2) * U) * dP.abs())).sum(1, keepdim=True)
+        G = P * (dP - delta)
+        eG = rP * G.abs() + P * (eP + eD + 4 * U * (dP.abs() + delta.abs())) + 2.0 ** -16 * G.abs()
+        wq[rq, hc] = G @ K * s
+        tq[rq, hc] = (eG + (n + 2) * U * G.abs()) @ K.abs() * s
+        wk[rk, kc] += G.T @ Q * s
+        tk[rk, kc] += (eG + (H // KV * nq + 40) * U * G.abs()).T @ Q.abs() * s
+    tq += HALF["bf16"] * (wq.abs() + tq)
+    tk += HALF["bf16"] * (wk.abs() + tk)
+    _near(dq, wq, tq, sum(lq), "dq")
+    if max(lk) <= 32:
+        _near(dkv[:, :KV * dk].contiguous(), wk, tk, sum(lk), "dk")
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("lq,H,KV", [([70, 3, 129], 4, 2), ([1, 1], 2, 2)])
 def test_a_batch_without_keys(lq, H, KV, dtype):
