@@ -193,7 +193,8 @@ __global__ __launch_bounds__(256, E::PL == 3 && DK < 128 ? 3 : 2) void xattn_row
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][nt][r] = drop_keep(dh, (uint32_t)(q0 + q), (uint32_t)(kbase + nt * 16 + r)) ? s[t][nt][r] * dh.inv_keep : 0.f;
+                    for (int r = 0; r < 4; ++r)
+                        s[t][nt][r] = drop_keep(dh, (uint32_t)(q0 + q), (uint32_t)(kbase + nt * 16 + r)) ? s[t][nt][r] * dh.inv_keep : 0.f;
             }
         }
         if constexpr (E::PL == 1) __builtin_amdgcn_sched_barrier(0);

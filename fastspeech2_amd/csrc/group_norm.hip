@@ -56,8 +56,9 @@ struct GnArgs {
 // added back, and silu to 9 u.
 __device__ __forceinline__ float gn_tanh(float z) {
     const float u = fminf(z * z, 64.0f);
-    const float p = fmaf(fmaf(fmaf(fmaf(1.523053150265241e-8f, u, 2.1894744349992834e-5f), u, 3.571603214368224e-3f), u, 0.13444502651691437f), u, 1.0f);
-    const float q = fmaf(fmaf(fmaf(fmaf(8.522493430973554e-7f, u, 3.411300422158092e-4f), u, 2.616446278989315e-2f), u, 0.4677782952785492f), u, 1.0f);
+    float p = fmaf(1.523053150265241e-8f, u, 2.1894744349992834e-5f), q = fmaf(8.522493430973554e-7f, u, 3.411300422158092e-4f);
+    p = fmaf(fmaf(fmaf(p, u, 3.571603214368224e-3f), u, 0.13444502651691437f), u, 1.0f);
+    q = fmaf(fmaf(fmaf(q, u, 2.616446278989315e-2f), u, 0.4677782952785492f), u, 1.0f);
     const float t = z * p * __builtin_amdgcn_rcpf(q);
     return __builtin_elementwise_maximum(__builtin_elementwise_minimum(t, 1.0f), -1.0f);         // (these keep a NaN)
 }
