@@ -14,9 +14,9 @@
 
 namespace fs2 {
 
-// Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16: delta 6.4 us for 27 MB (4.2 TB/s), the rest 37.5 us
+// Measured on a training step of 32 x 800 frames over 120 phones, 2 heads of 128, bf16: delta 6.4 us for 27 MB (4.2 TB/s), the rest 39 us
 // (whole step, forward included, 57 us, 70 with dropout, where the last spills 8 registers; floor 11.8); 3 x 1601 frames over 301 phones,
-// 4 heads on 2 of 96, fp32: 5 + 77 + 5.5 us for 4.9 GFLOP (whole step 114, 127 with dropout, 12 registers spilled; floor 37).
+// 4 heads on 2 of 96, fp32: 5 + 79 + 5.5 us for 4.9 GFLOP (whole step 114 to 117, 128 with dropout, 12 registers spilled; floor 37).
 
 template <typename T> __device__ __forceinline__ f32x4 x_load4(const T* p) {
     if constexpr (sizeof(T) == 4) return *(const f32x4*)p;
